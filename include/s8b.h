@@ -128,6 +128,30 @@ int s8b_gemm_w8a8_tc_packed(const int8_t *xq, const float *xs, const int8_t *wpa
                             const float *ws, void *y, int out_kind, int M, int N, int K,
                             int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
+/* W8A8 linear layer with its epilogue, for any token count:
+ *   v = (f32(sum_k xq[m,k]*w[n,k]) * xs[m]) * ws[n] + bias[n];  y[m,n] = act(v) + residual[m,n],
+ * int32 sums, binary32 epilogue, one rounding to dtype. bias [N] and residual [M,N] are in dtype
+ * and nullable; y may be residual itself. With neither and S8B_ACT_NONE the result equals
+ * s8b_gemm_w8a8 bit for bit; the activations use the device's binary32 exp and erf (relative
+ * error below 1e-5), so they are not part of the bit-exact contract. Up to 256 rows (and
+ * K % 128 == 0) the weights stream through the split-K GEMM above and a second launch finishes
+ * the rows; beyond, one launch tiles the product 128 x 128 or 128 x 256 on tcgen05 kind::i8.
+ * K % 16 == 0, K < 131072; xq, w 16-byte aligned, bias, residual, y 2-byte aligned (16 bytes and
+ * N % 8 == 0 store vectors). workspace: s8b_linear_workspace_size bytes, 256-byte aligned, its
+ * first 256 bytes zero-filled once; workspace[0] (int32) receives S8B_ERR_TIMEOUT if a bounded
+ * wait gave up. Launches that share a workspace must be stream-ordered.
+ * Replaces superl8.linear and the bias and residual additions around it
+ * (superl8serve/layers/linear.py:122).                                                     */
+#define S8B_ACT_NONE 0
+#define S8B_ACT_SILU 1      /* v / (1 + exp(-v))                                            */
+#define S8B_ACT_GELU 2      /* v (1 + erf(v / sqrt 2)) / 2                                  */
+#define S8B_ACT_GELU_TANH 3 /* v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2              */
+#define S8B_ACT_RELU 4      /* max(v, 0)                                                    */
+size_t s8b_linear_workspace_size(int M, int N, int K);
+int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *w, const float *ws,
+                    const void *bias, int activation, const void *residual, void *y, int M, int N,
+                    int K, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* SwiGLU on a merged [gate | up] row (gu is [M, 2F]) followed by per-token int8 quant:
  *   a = dtype(g / (1 + exp(-g))), y = dtype(a * u), (q, s) = quant_rows(y); y_out nullable.
  * Replaces superl8.act_and_mul(x, "silu") (superl8serve/layers/activation.py:24) fused with

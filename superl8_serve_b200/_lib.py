@@ -16,6 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libs8b.so"
 
 S8B_BF16, S8B_FP16 = 0, 1
 CODEC = {"fp16": 0, "int8": 1, "int8-had": 2, "int4": 3, "int4-had": 4, "nf4": 5}
+ACTIVATION = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
 ERR_TIMEOUT = -6
 
 _vp, _i, _f, _sz, _u32, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint32, C.c_uint64
@@ -29,6 +30,9 @@ SIGNATURES: dict[str, tuple] = {
     "s8b_quant_rows": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp]),
     "s8b_rmsnorm_quant": (_i, [_vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "s8b_gemm_w8a8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "s8b_linear_workspace_size": (_sz, [_i, _i, _i]),
+    "s8b_linear_w8a8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _sz,
+                             _vp]),
     "s8b_silu_mul_quant": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
     "s8b_rmsnorm_quant_split": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _i,
                                      _i, _i, _vp]),

@@ -4,17 +4,43 @@ layer API use the allocating forms."""
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 
-from ._lib import CODEC, call, dtype_code, ptr, stream
+from ._lib import ACTIVATION, CODEC, call, dtype_code, ptr, stream
 
 __all__ = [
     "quant_rows", "rmsnorm_quant", "gemm_w8a8", "gemm_w8a8_tc", "gemm_tc_workspace",
     "silu_mul_quant", "qkv_post", "kv_write_paged",
     "paged_decode_q8", "paged_decode", "embed", "argmax", "codec_encode", "codec_decode",
     "codec_sizes", "decode_workspace_bytes", "moe_route", "moe_gemm_grouped", "moe_combine",
-    "sample",
+    "sample", "linear_w8a8", "linear_workspace",
 ]
+
+
+def _on(dev: torch.device):
+    """The context that makes ``dev`` current (a launch on a stream of another device than the
+    current one fails); nothing where it already is."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _check(what: str, dev: torch.device, *tensors):
+    """Each (name, tensor or None, dtype, shape) is a contiguous CUDA tensor of that dtype and
+    shape on ``dev``."""
+    for name, t, dt, shape in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: {name} must be a CUDA tensor (no CPU fallback)")
+        if t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on {dev}")
+        if t.dtype != dt:
+            raise ValueError(f"{what}: {name} must be {dt}, got {t.dtype}")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous")
 
 
 def quant_rows(x: torch.Tensor):
@@ -93,6 +119,49 @@ def gemm_w8a8_tc(xq, xs, w, ws, *, out=None, out_dtype=torch.bfloat16, raw=False
     else:
         call("s8b_gemm_w8a8_tc", ptr(xq), ptr(xs), ptr(w), ptr(ws), ptr(out), 1 if raw else 0, M,
              N, K, dt, ptr(workspace), workspace.numel(), stream(xq.device))
+    return out
+
+
+def linear_workspace(M: int, N: int, K: int, device) -> torch.Tensor:
+    """Workspace of ``linear_w8a8`` for these sizes (its status word zeroed)."""
+    from ._lib import load
+
+    ws = torch.empty(int(load().s8b_linear_workspace_size(M, N, K)), dtype=torch.uint8,
+                     device=device)
+    ws[:256].zero_()
+    return ws
+
+
+def linear_w8a8(xq, xs, w, ws, *, bias=None, activation=None, residual=None, out=None,
+                out_dtype=torch.bfloat16, workspace=None):
+    """``act(dequant(xq @ w^T) + bias) + residual`` rounded once to ``out_dtype``
+    (``s8b_linear_w8a8``): xq [..., K] int8, xs [...] fp32, w [N, K] int8, ws [N] fp32, bias [N]
+    and residual [..., N] in the output dtype; activation None, "silu", "gelu", "gelu_tanh" or
+    "relu". ``out`` may be ``residual``."""
+    if activation not in ACTIVATION:
+        raise ValueError(f"linear_w8a8: unknown activation {activation!r}")
+    if xq.dim() < 1 or w.dim() != 2:
+        raise ValueError("linear_w8a8: xq must be [..., K] and w [N, K]")
+    K, N, lead, dev = xq.shape[-1], w.shape[0], xq.shape[:-1], xq.device
+    M = 1
+    for n in lead:
+        M *= n
+    dt = out_dtype if out is None else out.dtype
+    _check("linear_w8a8", dev, ("xq", xq, torch.int8, xq.shape), ("xs", xs, torch.float32, lead),
+           ("w", w, torch.int8, (N, K)), ("ws", ws, torch.float32, (N,)),
+           ("bias", bias, dt, (N,)), ("residual", residual, dt, (*lead, N)),
+           ("out", out, dt, (*lead, N)))
+    code = dtype_code(dt)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((*lead, N), dtype=dt, device=dev)
+        if M == 0:
+            return out
+        if workspace is None:
+            workspace = linear_workspace(M, N, K, dev)
+        call("s8b_linear_w8a8", ptr(xq), ptr(xs), ptr(w), ptr(ws), ptr(bias),
+             ACTIVATION[activation], ptr(residual), ptr(out), M, N, K, code, ptr(workspace),
+             workspace.numel(), stream(dev))
     return out
 
 

@@ -1,0 +1,47 @@
+"""CPU: what the linear, chunk-attention and few-token MoE entry points refuse, at the C ABI
+(before anything is dereferenced or launched) and in the tensor wrappers."""
+
+import pytest
+import torch
+
+from superl8_serve_b200 import ops
+
+OK = 4096  # a non-null, well-aligned address: validation comes before any dereference
+
+
+def _linear(lib, **kw):
+    a = dict(xq=OK, xs=OK, w=OK, ws=OK, bias=None, act=0, res=None, y=OK, M=4, N=64, K=128, dt=0,
+             space=OK, size=1 << 30)
+    a.update(kw)
+    return lib.s8b_linear_w8a8(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({"xq": None}, -8), ({"xs": None}, -8), ({"w": None}, -8), ({"ws": None}, -8),
+    ({"y": None}, -8), ({"act": 5}, -8), ({"act": -1}, -8), ({"dt": 2}, -2), ({"M": -1}, -1),
+    ({"N": 0}, -1), ({"K": 0}, -1), ({"K": 136}, -1), ({"K": 131072}, -1), ({"xq": OK + 8}, -3),
+    ({"w": OK + 4}, -3), ({"xs": OK + 2}, -3), ({"y": OK + 1}, -3), ({"bias": OK + 1}, -3),
+    ({"res": OK + 1}, -3), ({"space": None}, -7), ({"size": 255}, -7), ({"space": OK + 16}, -3),
+    ({"M": 0}, 0),
+])
+def test_linear_refusals(lib, kw, code):
+    assert _linear(lib, **kw) == code
+
+
+def test_linear_workspace(lib):
+    assert lib.s8b_linear_workspace_size(257, 4096, 4096) == 256  # tiled: the status word only
+    assert lib.s8b_linear_workspace_size(4, 4096, 144) == 256
+    n = lib.s8b_linear_workspace_size(4, 4096, 4096)
+    assert n > 256 and (n - 256) % (4 * 4096 * 4) == 0
+    assert _linear(lib, M=4, N=4096, K=4096, size=n - 1) == -7
+
+
+def test_linear_wrapper_refusals():
+    z = torch.zeros
+    xq, xs, w, ws = z(2, 64, dtype=torch.int8), z(2), z(8, 64, dtype=torch.int8), z(8)
+    with pytest.raises(ValueError, match="unknown activation"):
+        ops.linear_w8a8(xq, xs, w, ws, activation="swish")
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.linear_w8a8(xq, xs, w, ws)
+    with pytest.raises(ValueError, match=r"w \[N, K\]"):
+        ops.linear_w8a8(xq, xs, w[0], ws)
