@@ -269,6 +269,37 @@ int s8b_paged_prefill_q8(const int8_t *q_i8, const float *q_s, const int8_t *kc,
                          int max_blocks, int max_ctx, float scale, void *workspace,
                          size_t workspace_bytes, int dtype, void *stream);
 
+/* Attention of a chunk of new tokens per sequence over the int8 paged cache: prompt chunks of
+ * any length, a few draft tokens to verify, or a short question after a long document.
+ * Sequence s has the rows cu_q[s] .. cu_q[s+1] of q_i8 [T,Hq,D], q_s [T,Hq] (s8b_qkv_post's
+ * queries) at the end of its context_lens[s] keys, which the cache holds already, new ones
+ * included: with n = cu_q[s+1] - cu_q[s], row i attends over positions 0 .. context_lens[s] -
+ * n + i of block-table row s ([S, max_blocks]; one row per sequence). A row that sees no
+ * position gets zeros; rows of out [T, Hq*D] (dtype) behind cu_q[S] are left as they are.
+ * cu_q [S+1] and context_lens [S] are read on the device, so a captured graph may replay with
+ * other lengths; kc/vc [num_blocks, Hkv, bs, D], ks/vs [num_blocks, Hkv, bs].
+ * Numerics: q.k exact, softmax in binary32, the weights e^(t - m) * vs rounded to bf16 before
+ * the second product (binary32 sums), one rounding to dtype. Not part of the bit-exact
+ * contract of the decode and prefill entry points (their weights have 15 bits relative to a
+ * partition's largest); the result is the same on every run, whatever the other streams do.
+ * D = 128; block_size a power of two up to 256; Hq / Hkv <= 128; S <= 1024; scale > 0. q_i8,
+ * kc, vc, out 16-byte aligned. workspace: s8b_paged_chunk_workspace_size() bytes (any shape),
+ * 256-byte aligned, its first 256 bytes zero-filled once. workspace[0] (int32) receives
+ * S8B_ERR_TIMEOUT if a bounded wait gave up, and S8B_ERR_ARG if a block id that some row
+ * attends to is outside [0, num_blocks) (block 0 stands in), a context is negative or longer
+ * than max_blocks * block_size (cut), or cu_q decreases or leaves [0, T] (cut); the output is
+ * then invalid and the caller clears the word. Launches that share a workspace must be
+ * stream-ordered. Two launches.
+ * Replaces superl8's attn_int8_varlen where the context is longer than the chunk
+ * (superl8serve/dist/pipeline.py:908-984).                                                */
+size_t s8b_paged_chunk_workspace_size(void);
+int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const int8_t *kc, const float *ks,
+                       const int8_t *vc, const float *vs, const int32_t *block_table,
+                       const int32_t *context_lens, const int32_t *cu_q, void *out, int T, int S,
+                       int Hq, int Hkv, int D, int block_size, int max_blocks, int num_blocks,
+                       float scale, void *workspace, size_t workspace_bytes, int dtype,
+                       void *stream);
+
 /* No-allocation form of s8b_paged_decode_q8, for callers that cannot allocate device
  * memory: a host-language binding (cgo, JNI, ctypes) that is handed device buffers but owns no
  * allocator, or a serving runtime that reserved all of HBM up front (KV pool sized to fill

@@ -1,0 +1,937 @@
+// Attention of a chunk of new tokens per sequence over the paged int8 KV cache
+// (s8b_paged_chunk_q8).
+//
+// Sequence s brings n new rows (cu_q[s] .. cu_q[s+1]) at the end of a context of c keys; row i
+// sees keys 0 .. c - n + i. With int8 queries, keys and values,
+//   x_j = (q . k_j) ks_j,   t_j = qs scale x_j,   o = sum_j e^(t_j - m) vs_j v_j / sum_j e^(t_j - m)
+// q . k is exact (kind::i8, int32); the softmax is binary32; the products e^(..) vs_j are
+// rounded to bf16 for the second product (kind::f16 with binary32 sums), whose other operand,
+// the value codes, bf16 holds exactly. bf16 rather than fp16: its range is binary32's, so no
+// token's scale can overflow or vanish beside another's, and half a step of it (2^-9 to 2^-8)
+// on weights that are then averaged stays below the output's own rounding to bf16.
+//
+// Unit of work. The G query heads of a kv head share its keys, so a tile's 128 rows are
+// 128 / G tokens x G heads, and an item is two such tiles (A and B) of one sequence and kv head:
+// each K/V tile of 128 keys is staged and converted once for both, and while the softmax of
+// one tile runs, the tensor pipe works for the other. All items' key tiles in a row are cut
+// into equal runs, one per CTA, whatever the lengths: a CTA takes several items, or many CTAs
+// one item's keys. An item that a cut splits leaves partials (o, m, l) in the workspace, which
+// chunk_merge_kernel joins in key order, so the result does not depend on timing.
+//
+// Roles (16 warps): 0-3 and 4-7 softmax of tiles A and B (thread = row); 8-11 convert V codes
+// to bf16; 12 issues the MMAs; 13, 14 load K and V pages (cp.async, any block size); 15 loads Q.
+// TMEM: S_A | S_B | O_A | O_B, 128 columns each; the weights P overwrite the S they came from.
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace s8b {
+namespace {
+
+using namespace tc;
+
+namespace ca {
+constexpr int kHd = 128;
+constexpr int kThreads = 512;
+constexpr int kKeys = 128;        // keys per tile
+constexpr int kRows = 128;        // rows per tile
+constexpr int kStages = 3;
+constexpr int kTile = kKeys * kHd;                 // one int8 tile (16 KB)
+constexpr int kStage = 2 * kTile + 2 * kKeys * 4;  // K | V | ks | vs
+constexpr int kOffVs = kStages * kStage;           // V in bf16: 2 buffers of 2 panels of 64 dims
+constexpr int kV16 = 2 * kTile;
+constexpr int kOffQ = kOffVs + 2 * kV16;           // Q tiles A, B
+constexpr int kOffBar = kOffQ + 2 * kTile;
+constexpr int kPieces = 4;        // pieces announced ahead
+constexpr int kOffSeq = kOffBar + 1024;             // prefix[S+1] int64, cu[S+1], ctx[S]
+constexpr int kMaxSeqs = 1024;
+constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4;
+constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
+constexpr int kItemRows = 2 * kRows;
+constexpr int kMaxCtas = 512;     // CTAs the workspace has room for
+// workspace: status word, per-CTA metadata, partials
+struct Meta {  // an item whose first piece is CTA c's (slot 2c + 1); pieces go on in slots 2c' + 0
+  int valid, t0, ntok, g, last;
+  int pad[3];
+};
+constexpr size_t kOffMeta = 256;
+constexpr size_t kOffMl = kOffMeta + sizeof(Meta) * kMaxCtas;
+constexpr size_t slot_ml = kItemRows * 2, slot_o = kItemRows * kHd;
+}  // namespace ca
+
+struct ChunkArgs {
+  const int8_t *q;
+  const float *qs;
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  const int32_t *bt, *ctx, *cu;
+  void *out;
+  uint8_t *ws;
+  float *ml, *po;
+  int T, S, Hq, Hkv, G, TA, bs_log2, max_blocks, num_blocks;
+  float c;  // scale * log2(e)
+};
+
+// ------------------------------------------------------------------- small PTX pieces ----
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+        "l"(reinterpret_cast<unsigned long long &>(c)));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float2 v) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
+        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15};" ::"r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// D[128 x 128] (+)= A (bf16 in TMEM, 8 columns per 16 keys) . B (shared memory)
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  const uint32_t z = 0;
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z));
+}
+// kind::f16: D f32 (1) at bit 4, A and B bf16 (1) at 7 and 10, B MN-major at 16, N, M.
+constexpr uint32_t kIdescPv =
+    (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+// B operand V [keys][dims], dims contiguous, two panels of 64 dims: 8-key groups 1024 B apart
+// (stride), panels 16 KB apart (leading).
+__device__ __forceinline__ uint64_t v16_desc(uint32_t saddr) {
+  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(16384 >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// Two int8 codes in the low bytes of x's halves -> two bf16: a code c is (c & 127) minus 128 if
+// its sign bit is set; 128 + (c & 127) and 128 (or 256) are bf16 numbers made by their bits,
+// and their difference is exact.
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t x) {
+  const uint32_t a = (x & 0x007F007Fu) | 0x43004300u, b = (x & 0x00800080u) | 0x43004300u;
+  __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a),
+                             reinterpret_cast<const __nv_bfloat162 &>(b));
+  return reinterpret_cast<uint32_t &>(r);
+}
+
+// ---------------------------------------------------------------------- the work list ----
+// Item (sequence, kv head, tile of 2 TA tokens). units = its key tiles, at least one.
+struct SeqTab {
+  const long long *pre;  // [S + 1] units before each sequence
+  const int *cu, *ctx;
+};
+struct Item {
+  int t0, ntok, base, keys, nk, units;  // first row, tokens, keys before row t0, keys, tiles
+};
+__device__ __forceinline__ Item item_at(const SeqTab &q, const ChunkArgs &a, int s, int t) {
+  Item it;
+  const int c0 = q.cu[s], n = q.cu[s + 1] - c0, i0 = t * 2 * a.TA;
+  const int cap = static_cast<int>(min(0x7fffffffll - 256,
+                                       static_cast<long long>(a.max_blocks) << a.bs_log2));
+  it.t0 = c0 + i0;
+  it.ntok = min(2 * a.TA, n - i0);
+  it.base = q.ctx[s] - n + i0;
+  it.keys = min(max(it.base + it.ntok, 0), cap);
+  it.nk = (it.keys + ca::kKeys - 1) / ca::kKeys;
+  it.units = max(it.nk, 1);
+  return it;
+}
+// One piece of a CTA's run: key tiles [k0, k1) of one item. Warp 15 walks the run and announces
+// the pieces to the other roles through a small ring in shared memory (a walk in every role's
+// registers made the softmax spill).
+struct Piece {
+  int valid;  // 0: the run is over
+  int s, g, t0, ntok, base, keys, k0, k1;
+  int starts, ends;  // holds the item's first / last key tile
+  int behind;        // units of the item after this piece
+};
+struct Walk {
+  int s, g, t, off, left;
+  __device__ __forceinline__ void next(const SeqTab &q, const ChunkArgs &a, Piece *p) {
+    p->valid = left > 0;
+    if (left <= 0) return;
+    const Item it = item_at(q, a, s, t);
+    const int take = min(left, it.units - off);
+    p->s = s;
+    p->g = g;
+    p->t0 = it.t0;
+    p->ntok = it.ntok;
+    p->base = it.base;
+    p->keys = it.keys;
+    p->k0 = off;
+    p->k1 = min(off + take, it.nk);
+    p->starts = off == 0;
+    p->ends = off + take == it.units;
+    p->behind = it.units - (off + take);
+    left -= take;
+    off = 0;  // only the run's first piece starts inside an item, only its last ends there
+    const int n = q.cu[s + 1] - q.cu[s];
+    if (++t * 2 * a.TA < n) return;
+    t = 0;
+    if (++g < a.Hkv) return;
+    g = 0;
+    do ++s;
+    while (s < a.S && q.cu[s + 1] == q.cu[s]);
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const ChunkArgs a) {
+  using namespace ca;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                            ~uintptr_t(1023));
+  uint64_t *full = reinterpret_cast<uint64_t *>(sm + kOffBar);  // [3] stage loaded
+  uint64_t *empty = full + 3;    // [3] K read, V converted, scales read by both softmax groups
+  uint64_t *vfull = empty + 3;   // [2] bf16 V written
+  uint64_t *vempty = vfull + 2;  // [2] bf16 V read
+  uint64_t *sfull = vempty + 2;  // [2] S of tile A / B ready
+  uint64_t *pfull = sfull + 2;   // [2] P of tile A / B written (S read, O rescaled)
+  uint64_t *ofull = pfull + 2;   // [2] O of tile A / B complete
+  uint64_t *afull = ofull + 2;         // [4] piece announced
+  uint64_t *aempty = afull + kPieces;  // [4] piece done by every other role's warp
+  uint64_t *qfull = aempty + kPieces, *qempty = qfull + 1, *drained = qempty + 1;
+  uint32_t *tmem_base = reinterpret_cast<uint32_t *>(drained + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base + 1);
+  int *first = reinterpret_cast<int *>(tmem_base + 2);  // s, g, t, off of this CTA's run
+  Piece *pieces = reinterpret_cast<Piece *>(sm + kOffBar + 512);
+  static_assert(kPieces * sizeof(Piece) <= 512, "the ring of pieces fits its 512 bytes");
+  long long *pre = reinterpret_cast<long long *>(sm + kOffSeq);
+  int *cu = reinterpret_cast<int *>(pre + kMaxSeqs + 1);
+  int *ctx = cu + kMaxSeqs + 1;
+  int32_t *status = reinterpret_cast<int32_t *>(a.ws);
+  Meta *meta = reinterpret_cast<Meta *>(a.ws + kOffMeta);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  griddep_launch();
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 2);
+      mbar_init(&empty[i], 1 + 4 + 4 + 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&vfull[i], 4);
+      mbar_init(&vempty[i], 1);
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[i], 4);
+      mbar_init(&ofull[i], 1);
+    }
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&afull[i], 1);
+      mbar_init(&aempty[i], 15);
+    }
+    mbar_init(qfull, 1);
+    mbar_init(qempty, 1);
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  griddep_wait();
+
+  // ---- this CTA's run of units ----
+  const int S = a.S;
+  for (int i = threadIdx.x; i <= S; i += kThreads) {
+    const int v = a.cu[i];
+    // rows outside the tensors, or lengths that fall: cut to what exists, and said so
+    if (v < 0 || v > a.T || (i > 0 && v < a.cu[i - 1])) *status = S8B_ERR_ARG;
+    cu[i] = min(max(v, 0), a.T);
+    if (i < S) {
+      const int c = a.ctx[i];
+      if (c < 0 || static_cast<long long>(c) > (static_cast<long long>(a.max_blocks) << a.bs_log2))
+        *status = S8B_ERR_ARG;
+      ctx[i] = max(c, 0);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int i = 1; i <= S; ++i)
+      if (cu[i] < cu[i - 1]) cu[i] = cu[i - 1];
+  __syncthreads();
+  const SeqTab tab{pre, cu, ctx};
+  for (int s = warp; s < S; s += kThreads / 32) {
+    const int n = cu[s + 1] - cu[s], nt = (n + 2 * a.TA - 1) / (2 * a.TA);
+    int w = 0;
+    for (int t = lane; t < nt; t += 32) w += item_at(tab, a, s, t).units;
+    w = warp_sum_i(w);
+    if (lane == 0) pre[s + 1] = static_cast<long long>(w) * a.Hkv;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long carry = 0;
+    for (int s0 = 0; s0 < S; s0 += 32) {
+      long long v = s0 + lane < S ? pre[s0 + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      v += carry;
+      if (s0 + lane < S) pre[s0 + lane + 1] = v;
+      carry = __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+  __syncthreads();
+  const long long W = pre[S];
+  const long long ctas = min(static_cast<long long>(gridDim.x), W);  // CTAs with work
+  const long long u0 = blockIdx.x < ctas ? blockIdx.x * W / ctas : 0;
+  const long long u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * W / ctas : 0;
+  if (u1 > u0) {
+    for (int s = threadIdx.x; s < S; s += kThreads)
+      if (pre[s] <= u0 && u0 < pre[s + 1]) first[0] = s;
+  }
+  __syncthreads();
+  if (warp == 0 && u1 > u0) {
+    const int s = first[0];
+    const long long per = (pre[s + 1] - pre[s]) / a.Hkv, rem = u0 - pre[s];
+    const int g = static_cast<int>(rem / per);
+    int r = static_cast<int>(rem - g * per), t0 = 0;
+    const int nt = (cu[s + 1] - cu[s] + 2 * a.TA - 1) / (2 * a.TA);
+    while (true) {
+      const int u = t0 + lane < nt ? item_at(tab, a, s, t0 + lane).units : 0;
+      int v = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, v > r);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) {
+          first[1] = g;
+          first[2] = t0 + lane;
+          first[3] = r - (v - u);
+        }
+        break;
+      }
+      r -= __shfl_sync(0xffffffffu, v, 31);
+      t0 += 32;
+      if (t0 >= nt) break;  // not reached: the units of the sequence hold u0
+    }
+  }
+  if (threadIdx.x == 0) meta[blockIdx.x].valid = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base;
+  // Every role goes through the same pieces; `kt` counts the key tiles so far (stage kt % 3, bf16
+  // V buffer kt % 2), `np` the pieces with keys. A piece is next()ed by all lanes of a warp.
+  int na = 0;
+  auto next = [&]() -> const Piece * {
+    const bool got = mbar_wait(&afull[na % kPieces], (na / kPieces) & 1, abort_flag, status);
+    if (!__all_sync(0xffffffffu, got)) return nullptr;
+    const Piece *p = &pieces[na % kPieces];
+    return p->valid ? p : nullptr;
+  };
+  auto done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&aempty[na % kPieces]);
+    ++na;
+  };
+  if (warp < 8) {
+    // ------------------------------------------------------------------------ softmax ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int hf = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t ts = tmem + hf * 128 + lanes, to = tmem + 256 + hf * 128 + lanes;
+    const int tok = row / a.G, head_in = row - tok * a.G;
+    int kt = 0, ns = 0, np = 0;  // tiles, S tiles of this half, pieces of this half
+    bool ok = true;
+    while (const Piece *pc = next()) {
+      const bool active = pc->ntok > hf * a.TA;  // uniform over the half
+      const int i = hf * a.TA + tok;
+      const bool valid = tok < a.TA && i < pc->ntok;
+      auto q_row = [&]() {
+        return static_cast<size_t>(pc->t0 + i) * a.Hq + pc->g * a.G + head_in;
+      };
+      const float c = valid ? a.qs[q_row()] * a.c : 0.0f;
+      // keys this row sees (rows of no token count as full, so that they mask no tile)
+      const int lim = valid ? min(max(pc->base + i + 1, 0), pc->keys) : pc->keys;
+      float m = -INFINITY, l = 0.0f;
+      for (int k = pc->k0; k < pc->k1; ++k, ++kt) {
+        const int st = kt % kStages;
+        ok = mbar_wait(&full[st], (kt / kStages) & 1, abort_flag, status);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (active) {
+          ok = mbar_wait(&sfull[hf], ns & 1, abort_flag, status);
+          ++ns;
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const float4 *ks = reinterpret_cast<const float4 *>(sm + st * kStage + 2 * kTile);
+          const float4 *vs = ks + kKeys / 4;
+          float2 x[64];
+          float mx = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t v[32];
+            tmem_ld32(ts + 32 * b, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = ks[8 * b + j];
+              x[16 * b + 2 * j] =
+                  mul2(make_float2(static_cast<float>(static_cast<int>(v[4 * j])),
+                                   static_cast<float>(static_cast<int>(v[4 * j + 1]))),
+                       make_float2(f.x, f.y));
+              x[16 * b + 2 * j + 1] =
+                  mul2(make_float2(static_cast<float>(static_cast<int>(v[4 * j + 2])),
+                                   static_cast<float>(static_cast<int>(v[4 * j + 3]))),
+                       make_float2(f.z, f.w));
+            }
+          }
+          const int seen = lim - k * kKeys;  // this row's keys in the tile (any sign)
+          const bool masked = __any_sync(0xffffffffu, seen < kKeys);
+          if (masked) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+              if (2 * j >= seen) x[j].x = -INFINITY;
+              if (2 * j + 1 >= seen) x[j].y = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 64; ++j) mx = fmaxf(mx, fmaxf(x[j].x, x[j].y));
+          // The reference m moves only when a row's maximum passed it by 2^8 (weights up to
+          // 256 lose nothing in bf16 and binary32), so O is rarely rescaled.
+          const bool move = c * (mx - m) > 8.0f;
+          if (__any_sync(0xffffffffu, move)) {
+            const float mn = fmaxf(m, mx);
+            const float al = mn == m ? 1.0f : ex2(c * (m - mn));
+            m = mn;
+            l *= al;
+            if (k > pc->k0) {
+#pragma unroll 1
+              for (int b = 0; b < 8; ++b) {
+                uint32_t v[16];
+                tmem_ld16(to + 16 * b, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * al);
+                tmem_st16(to + 16 * b, v);
+              }
+            }
+          }
+          const float nm = m == -INFINITY ? 0.0f : -c * m;
+          const float2 c2 = make_float2(c, c), nm2 = make_float2(nm, nm);
+          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = vs[8 * b + j];
+              float2 e[2];
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int at = 16 * b + 2 * j + u;
+                const float2 t = fma2(x[at], c2, nm2);
+                e[u] = make_float2(ex2(t.x), ex2(t.y));
+                if (masked) {
+                  if (2 * at >= seen) e[u].x = 0.0f;
+                  if (2 * at + 1 >= seen) e[u].y = 0.0f;
+                }
+                sum = add2(sum, e[u]);
+              }
+              e[0] = mul2(e[0], make_float2(f.x, f.y));
+              e[1] = mul2(e[1], make_float2(f.z, f.w));
+              if (masked) {  // a hidden key's scale may hold anything
+                const int at = 32 * b + 4 * j;
+                if (at >= seen) e[0].x = 0.0f;
+                if (at + 1 >= seen) e[0].y = 0.0f;
+                if (at + 2 >= seen) e[1].x = 0.0f;
+                if (at + 3 >= seen) e[1].y = 0.0f;
+              }
+              pk[2 * j] = pack_bf16(e[0]);
+              pk[2 * j + 1] = pack_bf16(e[1]);
+            }
+            tmem_st16(ts + 16 * b, pk);
+          }
+          l += sum.x + sum.y;
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[hf]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+      }
+      if (!ok) break;
+      if (active) {
+        const bool whole = pc->starts && pc->ends;
+        const bool keys = pc->k1 > pc->k0;
+        if (keys) {
+          ok = mbar_wait(&ofull[hf], np & 1, abort_flag, status);
+          ++np;
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        const int slot = 2 * blockIdx.x + (pc->starts ? 1 : 0);
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // sees no key: zero
+        T *orow = static_cast<T *>(a.out) + q_row() * kHd;
+        float *prow = a.po + slot * slot_o + (hf * kRows + row) * kHd;
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          uint32_t v[32];
+          if (keys) {
+            tmem_ld32(to + 32 * b, v);
+            tmem_wait_ld();
+          }
+          if (!valid) continue;
+          if (whole) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              T o[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                o[u] = from_f32<T>(l == 0.0f ? 0.0f : __uint_as_float(v[j + u]) * inv);
+              uint4 raw;
+              memcpy(&raw, o, 16);
+              *reinterpret_cast<uint4 *>(orow + 32 * b + j) = raw;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<uint4 *>(prow + 32 * b + j) =
+                  make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          }
+        }
+        tc_fence_before();
+        if (!whole && valid) {
+          float *ml = a.ml + slot * slot_ml + (hf * kRows + row) * 2;
+          ml[0] = m == -INFINITY ? -INFINITY : c * m;
+          ml[1] = l;
+        }
+      }
+      done();
+    }
+  } else if (warp < 12) {
+    // --------------------------------------------------------------- V codes to bf16 ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const int ct = threadIdx.x - 256;
+    const int ch = ct & 7, key0 = ct >> 3;  // 16-byte chunk, first key; keys step by 16
+    int kt = 0;
+    bool ok = true;
+    while (const Piece *pc = next()) {
+      for (int k = pc->k0; k < pc->k1; ++k, ++kt) {
+        const int st = kt % kStages, vb = kt & 1;
+        ok = mbar_wait(&full[st], (kt / kStages) & 1, abort_flag, status) &&
+             mbar_wait(&vempty[vb], ((kt >> 1) & 1) ^ 1, abort_flag, status);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        const uint8_t *src = sm + st * kStage + kTile + key0 * kHd + ch * 16;
+        uint8_t *dst = sm + kOffVs + vb * kV16 + (ch >> 2) * 16384 + key0 * 128;
+        const int un = (ch & 3) * 2, sw = key0 & 7;  // keys step by 16: the swizzle stays
+        // the chunks of panel 1 store their halves in the other order: banks stay apart
+        const int f = ch >> 2;
+        uint8_t *d0 = dst + ((un + f) ^ sw) * 16, *d1 = dst + ((un + 1 - f) ^ sw) * 16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 q = *reinterpret_cast<const uint4 *>(src + i * 16 * kHd);
+          uint4 lo, hi;
+          lo.x = codes_bf16(__byte_perm(q.x, 0, 0x4140));
+          lo.y = codes_bf16(__byte_perm(q.x, 0, 0x4342));
+          lo.z = codes_bf16(__byte_perm(q.y, 0, 0x4140));
+          lo.w = codes_bf16(__byte_perm(q.y, 0, 0x4342));
+          hi.x = codes_bf16(__byte_perm(q.z, 0, 0x4140));
+          hi.y = codes_bf16(__byte_perm(q.z, 0, 0x4342));
+          hi.z = codes_bf16(__byte_perm(q.w, 0, 0x4140));
+          hi.w = codes_bf16(__byte_perm(q.w, 0, 0x4342));
+          *reinterpret_cast<uint4 *>(d0 + i * 16 * 128) = f ? hi : lo;
+          *reinterpret_cast<uint4 *>(d1 + i * 16 * 128) = f ? lo : hi;
+        }
+        fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&vfull[vb]);
+          mbar_arrive(&empty[st]);
+        }
+      }
+      if (!ok) break;
+      done();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 12) {
+      // ------------------------------------------------------------------ MMA issuer ----
+      constexpr uint32_t id_s = i8_idesc(128, 128);
+      const uint64_t qd = sw128_desc(smem_u32(sm + kOffQ));
+      int kt = 0, np = 0, npv[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, int par) {
+        ok = ok && mbar_wait(bar, par, abort_flag, status);
+        tc_fence_after();
+        return ok;
+      };
+      // O_hf (+)= P_hf V of key tile j (the count of tiles before it), first: overwrite
+      auto pv = [&](int hf, int j, bool first_tile) {
+        if (!wait(&vfull[j & 1], (j >> 1) & 1) || !wait(&pfull[hf], npv[hf] & 1)) return;
+        ++npv[hf];
+        const uint64_t vd = v16_desc(smem_u32(sm + kOffVs + (j & 1) * kV16));
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          mma_bf16_ts(tmem + 256 + 128 * hf, tmem + 128 * hf + 8 * i, vd + i * (2048 >> 4),
+                      kIdescPv, !(first_tile && i == 0));
+      };
+      while (const Piece *pc = next()) {
+        const int k0 = pc->k0, k1 = pc->k1, two = pc->ntok > a.TA;
+        if (k1 > k0 && lane == 0 && wait(qfull, np & 1)) {
+          for (int k = k0; k < k1 && ok; ++k, ++kt) {
+            const int st = kt % kStages;
+            const uint64_t kd = sw128_desc(smem_u32(sm + st * kStage));
+            for (int hf = 0; hf <= two; ++hf) {
+              if (k > k0) pv(hf, kt - 1, k - 1 == k0);
+              if (!ok) break;
+              if (hf == two && k > k0) mma_commit(&vempty[(kt - 1) & 1]);
+              if (hf == 0 && !wait(&full[st], (kt / kStages) & 1)) break;
+#pragma unroll
+              for (int i = 0; i < kHd / 32; ++i)
+                mma_i8(tmem + 128 * hf, qd + hf * (kTile >> 4) + 2 * i, kd + 2 * i, id_s, i != 0);
+              mma_commit(&sfull[hf]);
+            }
+            if (ok) mma_commit(&empty[st]);
+          }
+          if (ok) mma_commit(qempty);
+          for (int hf = 0; hf <= two && ok; ++hf) {
+            pv(hf, kt - 1, k1 - 1 == k0);
+            if (ok) mma_commit(&ofull[hf]);
+          }
+          if (ok) mma_commit(&vempty[(kt - 1) & 1]);
+          ++np;
+        }
+        if (!__all_sync(0xffffffffu, ok)) break;
+        done();
+      }
+      if (lane == 0) {
+        // nothing may read shared memory or write TMEM any more when they are given back
+        mma_commit(drained);
+        mbar_drain(drained, 0);
+      }
+    } else if (warp < 15) {
+      // --------------------------------------------------------------- K / V loaders ----
+      const bool vwarp = warp == 14;
+      const int8_t *codes = vwarp ? a.vc : a.kc;
+      const float *scales = vwarp ? a.vs : a.ks;
+      const int bs = 1 << a.bs_log2;
+      int kt = 0, sent = 0;  // tiles issued, tiles published
+      bool ok = true;
+      auto publish = [&](int pending) {  // the oldest unpublished tile has landed
+        if (pending >= 3) cp_wait<2>();
+        else if (pending == 2) cp_wait<1>();
+        else cp_wait<0>();
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[sent % kStages]);
+        ++sent;
+      };
+      while (true) {
+        // what has been issued is published before this warp can wait for another piece: the
+        // walk goes on only when the pieces before it are through
+        while (sent < kt && !__all_sync(0xffffffffu, mbar_try_wait(&afull[na % kPieces],
+                                                                   (na / kPieces) & 1)))
+          publish(kt - sent);
+        const Piece *pc = next();
+        if (!pc) break;
+        const int32_t *bt = a.bt + static_cast<size_t>(pc->s) * a.max_blocks;
+        const int keys = pc->keys, g = pc->g, k1 = pc->k1;
+        for (int k = pc->k0; k < k1; ++k) {
+          const int st = kt % kStages;
+          // tiles that fill the ring are published before their reader must make room
+          while (true) {
+            const bool room = __all_sync(0xffffffffu,
+                                         mbar_try_wait(&empty[st], ((kt / kStages) & 1) ^ 1));
+            if (room) break;
+            if (sent < kt) {
+              publish(kt - sent);
+              continue;
+            }
+            ok = mbar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
+            ok = __all_sync(0xffffffffu, ok);
+            break;
+          }
+          if (!ok) break;
+          // rows lane, lane + 32, .. of the tile: their rows in the pool
+          uint32_t prow[4];
+          const uint32_t base = smem_u32(sm + st * kStage);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int pos = k * kKeys + lane + 32 * q;
+            prow[q] = 0xffffffffu;
+            if (pos < keys) {
+              int blk = __ldg(bt + (pos >> a.bs_log2));
+              if (static_cast<uint32_t>(blk) >= static_cast<uint32_t>(a.num_blocks)) {
+                *status = S8B_ERR_ARG;  // a page that does not exist: page 0 stands in
+                blk = 0;
+              }
+              prow[q] = ((static_cast<uint32_t>(blk) * a.Hkv + g) << a.bs_log2) + (pos & (bs - 1));
+              cp4(base + 2 * kTile + (vwarp ? kKeys * 4 : 0) + (lane + 32 * q) * 4, scales + prow[q]);
+            }
+          }
+          const int ch = lane & 7;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int r = (lane >> 3) + 4 * j;
+            const uint32_t p = __shfl_sync(0xffffffffu, prow[j >> 3], r & 31);
+            const uint32_t dst = base + (vwarp ? kTile + r * kHd + ch * 16
+                                               : r * kHd + ((ch ^ (r & 7)) * 16));
+            if (p != 0xffffffffu) cp16(dst, codes + static_cast<size_t>(p) * kHd + ch * 16);
+          }
+          cp_commit();
+          ++kt;
+        }
+        if (!ok) break;
+        done();
+      }
+      while (ok && sent < kt) publish(kt - sent);
+      cp_wait<0>();
+    } else {
+      // ----------------------------------------------------- the walk, and Q's loader ----
+      Walk w;
+      w.s = first[0];
+      w.g = first[1];
+      w.t = first[2];
+      w.off = first[3];
+      w.left = static_cast<int>(u1 - u0);
+      int np = 0;
+      const int ch = lane & 7;
+      while (true) {
+        bool ok = mbar_wait(&aempty[na % kPieces], ((na / kPieces) & 1) ^ 1, abort_flag, status);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        Piece *pc = &pieces[na % kPieces];
+        if (lane == 0) {
+          w.next(tab, a, pc);
+          if (pc->valid && pc->starts && !pc->ends) {
+            // the pieces of this item run up to the CTA that holds its last unit
+            Meta &me = meta[blockIdx.x];
+            me.t0 = pc->t0;
+            me.ntok = pc->ntok;
+            me.g = pc->g;
+            me.last = static_cast<int>(((u1 + pc->behind) * ctas - 1) / W);
+            me.valid = 1;
+          }
+          mbar_arrive(&afull[na % kPieces]);
+        }
+        __syncwarp();
+        ++na;
+        if (!pc->valid) break;
+        if (pc->k1 <= pc->k0) continue;
+        ok = mbar_wait(qempty, (np & 1) ^ 1, abort_flag, status);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int ntok = pc->ntok, t0 = pc->t0, g = pc->g;
+        for (int r = lane >> 3; r < kItemRows; r += 4) {
+          const int hf = r >> 7, rr = r & 127, tok = rr / a.G;
+          const int i = hf * a.TA + tok;
+          if (tok < a.TA && i < ntok) {
+            const size_t qrow = static_cast<size_t>(t0 + i) * a.Hq + g * a.G + (rr - tok * a.G);
+            cp16(smem_u32(sm + kOffQ + r * kHd + ((ch ^ (r & 7)) * 16)), a.q + qrow * kHd + ch * 16);
+          }
+        }
+        cp_commit();
+        cp_wait<0>();
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qfull);
+        ++np;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+}
+
+// -------------------------------------------------------------------------------- merge ----
+// Joins the pieces of an item that CTA boundaries split, in key order: grid (CTAs, row groups),
+// one warp per row at a time, four values per lane.
+constexpr int kMergeWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const ChunkArgs a) {
+  using namespace ca;
+  griddep_launch();
+  griddep_wait();
+  const Meta me = reinterpret_cast<const Meta *>(a.ws + kOffMeta)[blockIdx.x];
+  if (!me.valid) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * kMergeWarps + warp; r < kItemRows; r += gridDim.y * kMergeWarps) {
+    const int hf = r >> 7, rr = r & 127, tok = rr / a.G, i = hf * a.TA + tok;
+    if (tok >= a.TA || i >= me.ntok) continue;
+    float m = -INFINITY;
+    for (int c = blockIdx.x; c <= me.last; ++c)
+      m = fmaxf(m, a.ml[(2 * c + (c == static_cast<int>(blockIdx.x))) * slot_ml + r * 2]);
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = blockIdx.x; c <= me.last; ++c) {
+      const size_t slot = 2 * c + (c == static_cast<int>(blockIdx.x));
+      const float mi = a.ml[slot * slot_ml + r * 2], li = a.ml[slot * slot_ml + r * 2 + 1];
+      if (mi == -INFINITY && li == 0.0f) continue;  // sees no key of this piece
+      const float wgt = mi == m ? 1.0f : ex2(mi - m);
+      const float4 v = *reinterpret_cast<const float4 *>(a.po + slot * slot_o + r * kHd + 4 * lane);
+      l += wgt * li;
+      o[0] += wgt * v.x;
+      o[1] += wgt * v.y;
+      o[2] += wgt * v.z;
+      o[3] += wgt * v.w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = from_f32<T>(l == 0.0f ? 0.0f : o[j] * inv);
+    uint2 raw;
+    memcpy(&raw, t, 8);
+    const size_t qrow = static_cast<size_t>(me.t0 + i) * a.Hq + me.g * a.G + (rr - tok * a.G);
+    *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + qrow * kHd + 4 * lane) = raw;
+  }
+}
+
+int chunk_ctas() { return min(sm_count(), ca::kMaxCtas); }
+
+}  // namespace
+}  // namespace s8b
+
+using namespace s8b;
+
+extern "C" size_t s8b_paged_chunk_workspace_size(void) {
+  using namespace ca;
+  return kOffMl + static_cast<size_t>(2 * chunk_ctas()) * (slot_ml + slot_o) * sizeof(float);
+}
+
+extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const int8_t *kc,
+                                  const float *ks, const int8_t *vc, const float *vs,
+                                  const int32_t *block_table, const int32_t *context_lens,
+                                  const int32_t *cu_q, void *out, int T_, int S, int Hq, int Hkv,
+                                  int D, int block_size, int max_blocks, int num_blocks,
+                                  float scale, void *workspace, size_t workspace_bytes, int dtype,
+                                  void *stream) {
+  using namespace ca;
+  if (!q_i8 || !q_s || !kc || !ks || !vc || !vs || !block_table || !context_lens || !cu_q || !out)
+    return S8B_ERR_ARG;
+  if (!(scale > 0.0f) || scale > 1e30f) return S8B_ERR_ARG;
+  if (dtype != S8B_BF16 && dtype != S8B_FP16) return S8B_ERR_DTYPE;
+  if (T_ < 0 || S < 0 || S > kMaxSeqs || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq / Hkv > kRows ||
+      D != kHd || max_blocks <= 0 || num_blocks <= 0)
+    return S8B_ERR_SHAPE;
+  int bs_log2 = 0;
+  while ((1 << bs_log2) < block_size && bs_log2 < 8) ++bs_log2;
+  if (block_size != (1 << bs_log2)) return S8B_ERR_SHAPE;
+  // rows of the pool and rows x heads of the queries are counted in 32 bits
+  if (static_cast<unsigned long long>(num_blocks) * Hkv * block_size >= 0xffffffffull ||
+      static_cast<long long>(T_) * Hq > 0x7fffffffll)
+    return S8B_ERR_SHAPE;
+  if (!aligned(q_i8, 16) || !aligned(kc, 16) || !aligned(vc, 16) || !aligned(out, 16) ||
+      !aligned(ks, 4) || !aligned(vs, 4) || !aligned(q_s, 4) || !aligned(block_table, 4) ||
+      !aligned(context_lens, 4) || !aligned(cu_q, 4))
+    return S8B_ERR_ALIGN;
+  if (T_ == 0 || S == 0) return S8B_OK;
+  if (!workspace || workspace_bytes < s8b_paged_chunk_workspace_size()) return S8B_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return S8B_ERR_ALIGN;
+  ChunkArgs a = {};
+  a.q = q_i8;
+  a.qs = q_s;
+  a.kc = kc;
+  a.vc = vc;
+  a.ks = ks;
+  a.vs = vs;
+  a.bt = block_table;
+  a.ctx = context_lens;
+  a.cu = cu_q;
+  a.out = out;
+  a.ws = static_cast<uint8_t *>(workspace);
+  const int ctas = chunk_ctas();
+  a.ml = reinterpret_cast<float *>(a.ws + kOffMl);
+  a.po = a.ml + static_cast<size_t>(2 * ctas) * slot_ml;
+  a.T = T_;
+  a.S = S;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.G = Hq / Hkv;
+  a.TA = kRows / a.G;
+  a.bs_log2 = bs_log2;
+  a.max_blocks = max_blocks;
+  a.num_blocks = num_blocks;
+  a.c = scale * 1.4426950408889634f;
+  const cudaStream_t st = (cudaStream_t)stream;
+  S8B_DISPATCH_DTYPE(dtype, T, {
+    ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T>), kSmem);
+    cudaError_t e = launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(kThreads), kSmem, st, a);
+    if (e == cudaSuccess)
+      e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, 8), dim3(kMergeWarps * 32), 0, st, a);
+    if (e != cudaSuccess) {
+      record_cuda_error(e);
+      return S8B_ERR_CUDA;
+    }
+  });
+  return check_launch(2);
+}

@@ -15,7 +15,7 @@ __all__ = [
     "silu_mul_quant", "qkv_post", "kv_write_paged",
     "paged_decode_q8", "paged_decode", "embed", "argmax", "codec_encode", "codec_decode",
     "codec_sizes", "decode_workspace_bytes", "moe_route", "moe_gemm_grouped", "moe_combine",
-    "sample", "linear_w8a8", "linear_workspace",
+    "sample", "linear_w8a8", "linear_workspace", "paged_chunk_q8", "chunk_workspace",
 ]
 
 
@@ -339,6 +339,47 @@ def paged_prefill_q8(q_i8, q_s, kc, ks, vc, vs, block_table, context_lens, row_b
          ptr(block_table), ptr(context_lens), ptr(row_blocks), row_blocks.shape[0], ptr(out),
          ptr(out_q), ptr(out_s), B, Hq, Hkv, D, bs, block_table.shape[-1], int(max_ctx),
          float(scale), ptr(workspace), workspace.numel(), dtype_code(out.dtype), stream(dev))
+    return out
+
+
+def chunk_workspace(device) -> torch.Tensor:
+    """Workspace of ``paged_chunk_q8``, for calls of any shape (its status word zeroed)."""
+    from ._lib import load
+
+    dev = torch.device(device)
+    with _on(dev if dev.index is not None else torch.device(dev.type, torch.cuda.current_device())):
+        ws = torch.empty(int(load().s8b_paged_chunk_workspace_size()), dtype=torch.uint8, device=dev)
+        ws[:256].zero_()
+    return ws
+
+
+def paged_chunk_q8(q_i8, q_s, kc, ks, vc, vs, block_table, context_lens, cu_q, scale, *, out=None,
+                   workspace=None, dtype=torch.bfloat16):
+    """Attention of each sequence's chunk of new rows over its paged context, causal at the
+    context's end (``s8b_paged_chunk_q8``): q_i8 [T, Hq, 128], q_s [T, Hq], one layer's pool kc,
+    vc [num_blocks, Hkv, bs, 128] and ks, vs [num_blocks, Hkv, bs], block_table [S, max_blocks],
+    context_lens [S] (new rows included) and cu_q [S + 1] int32 on the device. Returns
+    [T, Hq * 128]; rows behind cu_q[S] are not written."""
+    T, Hq, D = q_i8.shape
+    S, maxb = block_table.shape
+    nb, Hkv, bs, _ = kc.shape
+    dev = q_i8.device
+    dt = dtype if out is None else out.dtype
+    f32, i32 = torch.float32, torch.int32
+    _check("paged_chunk_q8", dev, ("q_i8", q_i8, torch.int8, (T, Hq, D)), ("q_s", q_s, f32, (T, Hq)),
+           ("kc", kc, torch.int8, (nb, Hkv, bs, D)), ("ks", ks, f32, (nb, Hkv, bs)),
+           ("vc", vc, torch.int8, (nb, Hkv, bs, D)), ("vs", vs, f32, (nb, Hkv, bs)),
+           ("block_table", block_table, i32, (S, maxb)), ("context_lens", context_lens, i32, (S,)),
+           ("cu_q", cu_q, i32, (S + 1,)), ("out", out, dt, (T, Hq * D)))
+    code = dtype_code(dt)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((T, Hq * D), dtype=dt, device=dev)
+        if workspace is None:
+            workspace = chunk_workspace(dev)
+        call("s8b_paged_chunk_q8", ptr(q_i8), ptr(q_s), ptr(kc), ptr(ks), ptr(vc), ptr(vs),
+             ptr(block_table), ptr(context_lens), ptr(cu_q), ptr(out), T, S, Hq, Hkv, D, bs, maxb,
+             nb, float(scale), ptr(workspace), workspace.numel(), code, stream(dev))
     return out
 
 

@@ -45,3 +45,33 @@ def test_linear_wrapper_refusals():
         ops.linear_w8a8(xq, xs, w, ws)
     with pytest.raises(ValueError, match=r"w \[N, K\]"):
         ops.linear_w8a8(xq, xs, w[0], ws)
+
+
+def _chunk(lib, **kw):
+    a = dict(q=OK, qs=OK, kc=OK, ks=OK, vc=OK, vs=OK, bt=OK, ctx=OK, cu=OK, out=OK, T=8, S=2, Hq=8,
+             Hkv=2, D=128, bs=16, maxb=4, nb=9, scale=0.1, space=OK, size=1 << 30, dt=0)
+    a.update(kw)
+    return lib.s8b_paged_chunk_q8(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    *[({n: None}, -8) for n in ("q", "qs", "kc", "ks", "vc", "vs", "bt", "ctx", "cu", "out")],
+    ({"scale": 0.0}, -8), ({"scale": -1.0}, -8), ({"scale": float("nan")}, -8),
+    ({"scale": float("inf")}, -8), ({"dt": 2}, -2), ({"T": -1}, -1), ({"S": -1}, -1),
+    ({"S": 1025}, -1), ({"Hq": 9}, -1), ({"Hkv": 0}, -1), ({"Hq": 258}, -1), ({"D": 64}, -1),
+    ({"bs": 12}, -1), ({"bs": 512}, -1), ({"bs": 0}, -1), ({"maxb": 0}, -1), ({"nb": 0}, -1),
+    ({"nb": 2 ** 31 - 1}, -1), ({"T": 2 ** 30}, -1), ({"q": OK + 8}, -3), ({"kc": OK + 4}, -3),
+    ({"out": OK + 2}, -3), ({"ks": OK + 2}, -3), ({"cu": OK + 1}, -3), ({"space": None}, -7),
+    ({"size": 1024}, -7), ({"space": OK + 16}, -3), ({"T": 0}, 0), ({"S": 0}, 0),
+])
+def test_chunk_refusals(lib, kw, code):
+    assert _chunk(lib, **kw) == code
+
+
+def test_chunk_wrapper_refusals():
+    z = torch.zeros
+    q, qs = z(4, 8, 128, dtype=torch.int8), z(4, 8)
+    kc, ks = z(3, 2, 16, 128, dtype=torch.int8), z(3, 2, 16)
+    bt, ctx, cu = (z(s, dtype=torch.int32) for s in ((1, 2), (1,), (2,)))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.paged_chunk_q8(q, qs, kc, ks, kc, ks, bt, ctx, cu, 0.1)
