@@ -47,6 +47,7 @@ constexpr int kMaxSeqs = 1024;
 constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4;
 constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
 constexpr int kItemRows = 2 * kRows;
+constexpr float kSumMax = 0x1p60f;  // a tile's sum of e^(t - reference) above: a new reference
 constexpr int kMaxCtas = 512;     // CTAs the workspace has room for
 // workspace: status word, per-CTA metadata, partials
 struct Meta {  // an item whose first piece is CTA c's (slot 2c + 1); pieces go on in slots 2c' + 0
@@ -115,12 +116,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *v) {
         "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15};" ::"r"(v[0]),
-      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr));
+__device__ __forceinline__ void tmem_ld_16x256_x1(uint32_t addr, uint32_t *v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t addr, uint32_t *v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_16x256_x1(uint32_t addr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%4], {%0,%1,%2,%3};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_16x128_x1(uint32_t addr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x1.b32 [%2], {%0,%1};" ::"r"(v[0]), "r"(v[1]), "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_16x128_x4(uint32_t addr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -135,6 +148,17 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Whether the phase is over, without waiting (try_wait may suspend the thread for microseconds).
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -392,24 +416,37 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   };
   if (warp < 8) {
     // ------------------------------------------------------------------------ softmax ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const int hf = warp >> 2, row = threadIdx.x & 127;
+    // S comes in the 16x256b shape: lane l holds keys 2 (l % 4), + 1 of each group of 8 for the
+    // rows l / 4 + 8 j (j = 0..3) of its warp's 32, so that a scale read from shared memory
+    // serves four rows (with a row per lane the broadcast reads alone took as long as the
+    // exponentials: 512 bytes of register writes for 4 values).
+    const int hf = warp >> 2, quad = lane & 3;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + hf * 128 + lanes, to = tmem + 256 + hf * 128 + lanes;
-    const int tok = row / a.G, head_in = row - tok * a.G;
-    int kt = 0, ns = 0, np = 0;  // tiles, S tiles of this half, pieces of this half
+    constexpr uint32_t kLow = 16u << 16;  // rows 16..31 of the warp
+    int kt = 0, ns = 0, np = 0;           // tiles, S tiles of this half, pieces of this half
     bool ok = true;
     while (const Piece *pc = next()) {
       const bool active = pc->ntok > hf * a.TA;  // uniform over the half
-      const int i = hf * a.TA + tok;
-      const bool valid = tok < a.TA && i < pc->ntok;
-      auto q_row = [&]() {
-        return static_cast<size_t>(pc->t0 + i) * a.Hq + pc->g * a.G + head_in;
+      auto q_row = [&](int rr) {  // tile row -> row of q (valid rows)
+        const int tok = rr / a.G;
+        return static_cast<size_t>(pc->t0 + hf * a.TA + tok) * a.Hq + pc->g * a.G + (rr - tok * a.G);
       };
-      const float c = valid ? a.qs[q_row()] * a.c : 0.0f;
-      // keys this row sees (rows of no token count as full, so that they mask no tile)
-      const int lim = valid ? min(max(pc->base + i + 1, 0), pc->keys) : pc->keys;
-      float m = -INFINITY, l = 0.0f;
+      auto is_row = [&](int rr) {
+        const int tok = rr / a.G;
+        return tok < a.TA && hf * a.TA + tok < pc->ntok;
+      };
+      float c[4], mr[4], l[4];  // log2(e) scale q_s, reference (a power of 2), sum of own keys
+      int lim[4];               // keys the row sees (rows of no token: all, they mask no tile)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int rr = 32 * (warp & 3) + (lane >> 2) + 8 * j;
+        const bool valid = is_row(rr);
+        c[j] = valid ? a.qs[q_row(rr)] * a.c : 0.0f;
+        lim[j] = valid ? min(max(pc->base + hf * a.TA + rr / a.G + 1, 0), pc->keys) : pc->keys;
+        mr[j] = -INFINITY;
+        l[j] = 0.0f;
+      }
       for (int k = pc->k0; k < pc->k1; ++k, ++kt) {
         const int st = kt % kStages;
         ok = mbar_wait(&full[st], (kt / kStages) & 1, abort_flag, status);
@@ -425,95 +462,160 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
             break;
           }
           tc_fence_after();
-          const float4 *ks = reinterpret_cast<const float4 *>(sm + st * kStage + 2 * kTile);
-          const float4 *vs = ks + kKeys / 4;
-          float2 x[64];
-          float mx = -INFINITY;
+          // this lane's keys: float2 index 4 * group + quad
+          const float2 *ks = reinterpret_cast<const float2 *>(sm + st * kStage + 2 * kTile) + quad;
+          const float2 *vs = ks + kKeys / 2;
+          // A piece's first tile and a tile that some row does not see whole take the general
+          // path below. The others take one pass with the reference at hand: binary32 and bf16
+          // keep their precision at any magnitude, so the reference has to be near the row's
+          // maximum, not at it, and the tile's sum alone shows whether it still is.
+          const int least = min(min(lim[0], lim[1]), min(lim[2], lim[3]));
+          bool general = __any_sync(0xffffffffu, k == pc->k0 || least < (k + 1) * kKeys);
+          if (!general) {
+            float2 sum[4];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t v[32];
-            tmem_ld32(ts + 32 * b, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 f = ks[8 * b + j];
-              x[16 * b + 2 * j] =
-                  mul2(make_float2(static_cast<float>(static_cast<int>(v[4 * j])),
-                                   static_cast<float>(static_cast<int>(v[4 * j + 1]))),
-                       make_float2(f.x, f.y));
-              x[16 * b + 2 * j + 1] =
-                  mul2(make_float2(static_cast<float>(static_cast<int>(v[4 * j + 2])),
-                                   static_cast<float>(static_cast<int>(v[4 * j + 3]))),
-                       make_float2(f.z, f.w));
-            }
-          }
-          const int seen = lim - k * kKeys;  // this row's keys in the tile (any sign)
-          const bool masked = __any_sync(0xffffffffu, seen < kKeys);
-          if (masked) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              if (2 * j >= seen) x[j].x = -INFINITY;
-              if (2 * j + 1 >= seen) x[j].y = -INFINITY;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 64; ++j) mx = fmaxf(mx, fmaxf(x[j].x, x[j].y));
-          // The reference m moves only when a row's maximum passed it by 2^8 (weights up to
-          // 256 lose nothing in bf16 and binary32), so O is rarely rescaled.
-          const bool move = c * (mx - m) > 8.0f;
-          if (__any_sync(0xffffffffu, move)) {
-            const float mn = fmaxf(m, mx);
-            const float al = mn == m ? 1.0f : ex2(c * (m - mn));
-            m = mn;
-            l *= al;
-            if (k > pc->k0) {
+            for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
-              for (int b = 0; b < 8; ++b) {
-                uint32_t v[16];
-                tmem_ld16(to + 16 * b, v);
+            for (int b = 0; b < 4; ++b) {  // P's columns 16 b .. end before S's from 32 (b + 1) on
+              uint32_t v[2][16], pk[2][8];
+              tmem_ld_16x256_x4(ts + 32 * b, v[0]);
+              tmem_ld_16x256_x4(ts + kLow + 32 * b, v[1]);
+              tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float2 kf = ks[16 * b + 4 * q], vf = vs[16 * b + 4 * q];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
+                  const float2 x =
+                      mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
+                  const float2 t = fma2(x, make_float2(c[j], c[j]), make_float2(-mr[j], -mr[j]));
+                  const float2 e = make_float2(ex2(t.x), ex2(t.y));
+                  sum[j] = add2(sum[j], e);
+                  pk[j >> 1][2 * q + (j & 1)] = pack_bf16(mul2(e, vf));
+                }
+              }
+              tmem_st_16x128_x4(ts + 16 * b, pk[0]);
+              tmem_st_16x128_x4(ts + kLow + 16 * b, pk[1]);
+            }
+            bool fits = true;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              // the row's sum over its four lanes decides, so that they decide alike
+              float r = sum[j].x + sum[j].y;
+              r += __shfl_xor_sync(0xffffffffu, r, 1);
+              r += __shfl_xor_sync(0xffffffffu, r, 2);
+              fits = fits && r < kSumMax;
+            }
+            general = !__all_sync(0xffffffffu, fits);
+            if (!general) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) l[j] += sum[j].x + sum[j].y;
+            } else {
+              // Rare (a maximum 2^60 times the last reference): P took S's place, so this
+              // warp's S is computed again, from the staged keys and the queries.
+              tmem_wait_st();
+              const uint8_t *kb = sm + st * kStage;
+#pragma unroll 1
+              for (int q = 0; q < 16; ++q) {
+                uint32_t v[8];
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
+                  const int rr = 32 * (warp & 3) + (lane >> 2) + 8 * j, key = 8 * q + 2 * quad;
+                  const int8_t *qr = a.q + (is_row(rr) ? q_row(rr) : 0) * kHd;
+                  int s0 = 0, s1 = 0;
+                  for (int ch = 0; ch < 8; ++ch) {
+                    const int4 x = __ldg(reinterpret_cast<const int4 *>(qr) + ch);
+                    const int4 y = *reinterpret_cast<const int4 *>(
+                        kb + key * kHd + ((ch ^ (key & 7)) * 16));
+                    const int4 z = *reinterpret_cast<const int4 *>(
+                        kb + (key + 1) * kHd + ((ch ^ ((key + 1) & 7)) * 16));
+                    s0 = __dp4a(x.w, y.w, __dp4a(x.z, y.z, __dp4a(x.y, y.y, __dp4a(x.x, y.x, s0))));
+                    s1 = __dp4a(x.w, z.w, __dp4a(x.z, z.z, __dp4a(x.y, z.y, __dp4a(x.x, z.x, s1))));
+                  }
+#pragma unroll
+                  for (int u = 0; u < 4; ++u)
+                    if (u == j) v[2 * u] = s0, v[2 * u + 1] = s1;
+                }
+                tmem_st_16x256_x1(ts + 8 * q, v);
+                tmem_st_16x256_x1(ts + kLow + 8 * q, v + 4);
+              }
+              tmem_wait_st();
+            }
+          }
+          if (general) {
+            // Two passes, keys masked by row: the maximum first. The reference moves only where
+            // the maximum passed it by 2^8, so that O is rarely rescaled.
+            float mx[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx[j] = -INFINITY;
+#pragma unroll 1
+            for (int q = 0; q < 16; ++q) {
+              uint32_t v[8];
+              tmem_ld_16x256_x1(ts + 8 * q, v);
+              tmem_ld_16x256_x1(ts + kLow + 8 * q, v + 4);
+              tmem_wait_ld();
+              const float2 kf = ks[4 * q];
+              const int key = k * kKeys + 8 * q + 2 * quad;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float x0 = static_cast<float>(static_cast<int>(v[2 * j])) * kf.x;
+                const float x1 = static_cast<float>(static_cast<int>(v[2 * j + 1])) * kf.y;
+                if (key < lim[j]) mx[j] = fmaxf(mx[j], x0);
+                if (key + 1 < lim[j]) mx[j] = fmaxf(mx[j], x1);
+              }
+            }
+            float al[4];
+            bool moved = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
+              const float tm = mx[j] == -INFINITY ? -INFINITY : c[j] * mx[j];
+              const bool move = tm > -INFINITY && (mr[j] == -INFINITY || tm - mr[j] > 8.0f);
+              al[j] = move && mr[j] != -INFINITY ? ex2(mr[j] - tm) : 1.0f;
+              if (move) mr[j] = tm;
+              l[j] *= al[j];
+              moved = moved || move;
+            }
+            if (__any_sync(0xffffffffu, moved) && k > pc->k0) {
+#pragma unroll 1
+              for (int q = 0; q < 16; ++q) {
+                uint32_t v[8];
+                tmem_ld_16x256_x1(to + 8 * q, v);
+                tmem_ld_16x256_x1(to + kLow + 8 * q, v + 4);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * al);
-                tmem_st16(to + 16 * b, v);
+                for (int j = 0; j < 8; ++j)
+                  v[j] = __float_as_uint(__uint_as_float(v[j]) * al[j >> 1]);
+                tmem_st_16x256_x1(to + 8 * q, v);
+                tmem_st_16x256_x1(to + kLow + 8 * q, v + 4);
               }
             }
-          }
-          const float nm = m == -INFINITY ? 0.0f : -c * m;
-          const float2 c2 = make_float2(c, c), nm2 = make_float2(nm, nm);
-          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+            for (int q = 0; q < 16; ++q) {  // P's columns 4 q .. end before S's from 8 q on
+              uint32_t v[8], pk[4];
+              tmem_ld_16x256_x1(ts + 8 * q, v);
+              tmem_ld_16x256_x1(ts + kLow + 8 * q, v + 4);
+              tmem_wait_ld();
+              const float2 kf = ks[4 * q], vf = vs[4 * q];
+              const int key = k * kKeys + 8 * q + 2 * quad;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 f = vs[8 * b + j];
-              float2 e[2];
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int at = 16 * b + 2 * j + u;
-                const float2 t = fma2(x[at], c2, nm2);
-                e[u] = make_float2(ex2(t.x), ex2(t.y));
-                if (masked) {
-                  if (2 * at >= seen) e[u].x = 0.0f;
-                  if (2 * at + 1 >= seen) e[u].y = 0.0f;
-                }
-                sum = add2(sum, e[u]);
+              for (int j = 0; j < 4; ++j) {
+                const float nm = mr[j] == -INFINITY ? 0.0f : -mr[j];
+                const float x0 = static_cast<float>(static_cast<int>(v[2 * j])) * kf.x;
+                const float x1 = static_cast<float>(static_cast<int>(v[2 * j + 1])) * kf.y;
+                // a hidden key's codes and scales may hold anything
+                const bool s0 = key < lim[j], s1 = key + 1 < lim[j];
+                const float e0 = s0 ? ex2(fmaf(x0, c[j], nm)) : 0.0f;
+                const float e1 = s1 ? ex2(fmaf(x1, c[j], nm)) : 0.0f;
+                l[j] += e0 + e1;
+                pk[j] = pack_bf16(make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f));
               }
-              e[0] = mul2(e[0], make_float2(f.x, f.y));
-              e[1] = mul2(e[1], make_float2(f.z, f.w));
-              if (masked) {  // a hidden key's scale may hold anything
-                const int at = 32 * b + 4 * j;
-                if (at >= seen) e[0].x = 0.0f;
-                if (at + 1 >= seen) e[0].y = 0.0f;
-                if (at + 2 >= seen) e[1].x = 0.0f;
-                if (at + 3 >= seen) e[1].y = 0.0f;
-              }
-              pk[2 * j] = pack_bf16(e[0]);
-              pk[2 * j + 1] = pack_bf16(e[1]);
+              tmem_st_16x128_x1(ts + 4 * q, pk);
+              tmem_st_16x128_x1(ts + kLow + 4 * q, pk + 2);
             }
-            tmem_st16(ts + 16 * b, pk);
           }
-          l += sum.x + sum.y;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -535,9 +637,22 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
           }
           tc_fence_after();
         }
+        // from here on a lane has one row: its sum and reference come from the lanes 4 (r % 8)
+        float lr = 0.0f, rr_m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float s = l[j];
+          s += __shfl_xor_sync(0xffffffffu, s, 1);
+          s += __shfl_xor_sync(0xffffffffu, s, 2);
+          s = __shfl_sync(0xffffffffu, s, 4 * (lane & 7));
+          const float m = __shfl_sync(0xffffffffu, mr[j], 4 * (lane & 7));
+          if (lane >> 3 == j) lr = s, rr_m = m;
+        }
+        const int row = 32 * (warp & 3) + lane;
+        const bool valid = is_row(row);
         const int slot = 2 * blockIdx.x + (pc->starts ? 1 : 0);
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // sees no key: zero
-        T *orow = static_cast<T *>(a.out) + q_row() * kHd;
+        const float inv = 1.0f / lr;  // not used where lr is 0
+        T *orow = static_cast<T *>(a.out) + (valid ? q_row(row) : 0) * kHd;
         float *prow = a.po + slot * slot_o + (hf * kRows + row) * kHd;
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
@@ -552,8 +667,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
             for (int j = 0; j < 32; j += 8) {
               T o[8];
 #pragma unroll
-              for (int u = 0; u < 8; ++u)
-                o[u] = from_f32<T>(l == 0.0f ? 0.0f : __uint_as_float(v[j + u]) * inv);
+              for (int u = 0; u < 8; ++u)  // a row that sees no key: zero
+                o[u] = from_f32<T>(lr == 0.0f ? 0.0f : __uint_as_float(v[j + u]) * inv);
               uint4 raw;
               memcpy(&raw, o, 16);
               *reinterpret_cast<uint4 *>(orow + 32 * b + j) = raw;
@@ -568,15 +683,14 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
         tc_fence_before();
         if (!whole && valid) {
           float *ml = a.ml + slot * slot_ml + (hf * kRows + row) * 2;
-          ml[0] = m == -INFINITY ? -INFINITY : c * m;
-          ml[1] = l;
+          ml[0] = rr_m;
+          ml[1] = lr;
         }
       }
       done();
     }
   } else if (warp < 12) {
     // --------------------------------------------------------------- V codes to bf16 ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int ct = threadIdx.x - 256;
     const int ch = ct & 7, key0 = ct >> 3;  // 16-byte chunk, first key; keys step by 16
     int kt = 0;
@@ -596,7 +710,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
         // the chunks of panel 1 store their halves in the other order: banks stay apart
         const int f = ch >> 2;
         uint8_t *d0 = dst + ((un + f) ^ sw) * 16, *d1 = dst + ((un + 1 - f) ^ sw) * 16;
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < 8; ++i) {
           const uint4 q = *reinterpret_cast<const uint4 *>(src + i * 16 * kHd);
           uint4 lo, hi;
@@ -622,7 +736,6 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
       done();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12) {
       // ------------------------------------------------------------------ MMA issuer ----
       constexpr uint32_t id_s = i8_idesc(128, 128);
@@ -698,8 +811,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
       while (true) {
         // what has been issued is published before this warp can wait for another piece: the
         // walk goes on only when the pieces before it are through
-        while (sent < kt && !__all_sync(0xffffffffu, mbar_try_wait(&afull[na % kPieces],
-                                                                   (na / kPieces) & 1)))
+        while (sent < kt && !__all_sync(0xffffffffu, mbar_test(&afull[na % kPieces],
+                                                               (na / kPieces) & 1)))
           publish(kt - sent);
         const Piece *pc = next();
         if (!pc) break;
@@ -710,7 +823,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
           // tiles that fill the ring are published before their reader must make room
           while (true) {
             const bool room = __all_sync(0xffffffffu,
-                                         mbar_try_wait(&empty[st], ((kt / kStages) & 1) ^ 1));
+                                         mbar_test(&empty[st], ((kt / kStages) & 1) ^ 1));
             if (room) break;
             if (sent < kt) {
               publish(kt - sent);

@@ -77,7 +77,11 @@ class Case:
     def check(self, out, rows=None):
         o, A = self.exact()
         out = out[:self.T].view(self.T, self.Hq, 128)
-        tol = (2 ** -8 + 2e-4) * A + torch.finfo(out.dtype).eps / 2 * o.abs() + 1e-30
+        # below a type's normal range its steps are those of the range's lower end: 2^-24 in fp16
+        # (a value that ought to be 1e-15 becomes 0), so half a step is 2^-25 there; bf16 has
+        # binary32's range
+        least = 2.0 ** -25 if out.dtype == torch.float16 else 1e-30
+        tol = (2 ** -8 + 2e-4) * A + torch.finfo(out.dtype).eps / 2 * o.abs() + least
         bad = ~((out.double() - o).abs() <= tol)
         if rows is not None:
             bad = bad[rows]
@@ -130,6 +134,17 @@ def test_sharp_softmax_moves_the_reference():
     pos = torch.arange(1500, device=DEV)
     c.ks[c.bt[0].long()[pos // 16], :, pos % 16] *= ramp[:, None]
     c.check(c.run())
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_jumps_beyond_the_reference(n):
+    """Single keys far into the context whose scores lie hundreds above all before them: the
+    weights of the tile overflow against the last reference."""
+    c = Case([(n, 1400)], 8, 2, 16, seed=17)
+    for pos, k in ((300, 40.0), (777, 120.0), (778, 119.0), (1250, 300.0)):
+        c.ks[int(c.bt[0, pos // 16]), :, pos % 16] = k * 0.02
+    c.check(c.run())
+    c.check(c.run(torch.float16))
 
 
 def test_rows_that_see_nothing():
