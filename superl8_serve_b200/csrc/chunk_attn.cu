@@ -21,6 +21,8 @@
 // Roles (16 warps): 0-3 and 4-7 softmax of tiles A and B (thread = row); 8-11 convert V codes
 // to bf16; 12 issues the MMAs; 13, 14 load K and V pages (cp.async, any block size); 15 loads Q.
 // TMEM: S_A | S_B | O_A | O_B, 128 columns each; the weights P overwrite the S they came from.
+#include <cstring>
+
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -42,7 +44,8 @@ constexpr int kV16 = 2 * kTile;
 constexpr int kOffQ = kOffVs + 2 * kV16;           // Q tiles A, B
 constexpr int kOffBar = kOffQ + 2 * kTile;
 constexpr int kPieces = 4;        // pieces announced ahead
-constexpr int kOffSeq = kOffBar + 1024;             // prefix[S+1] int64, cu[S+1], ctx[S]
+constexpr int kOffSums = kOffBar + 1024;
+constexpr int kOffSeq = kOffSums + 1024;             // prefix[S+1] int64, cu[S+1], ctx[S]
 constexpr int kMaxSeqs = 1024;
 constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4;
 constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
@@ -69,7 +72,8 @@ struct ChunkArgs {
   uint8_t *ws;
   float *ml, *po;
   int T, S, Hq, Hkv, G, TA, bs_log2, max_blocks, num_blocks;
-  float c;  // scale * log2(e)
+  int copies;  // pages go by bulk copies
+  float c;     // scale * log2(e)
 };
 
 // ------------------------------------------------------------------- small PTX pieces ----
@@ -129,11 +133,16 @@ __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t addr, uint32_t *v) {
 __device__ __forceinline__ void tmem_st_16x256_x1(uint32_t addr, const uint32_t *v) {
   asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%4], {%0,%1,%2,%3};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(addr));
 }
-__device__ __forceinline__ void tmem_st_16x128_x1(uint32_t addr, const uint32_t *v) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x1.b32 [%2], {%0,%1};" ::"r"(v[0]), "r"(v[1]), "r"(addr));
+__device__ __forceinline__ void tmem_st_16x128_x8(uint32_t addr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr));
 }
-__device__ __forceinline__ void tmem_st_16x128_x4(uint32_t addr, const uint32_t *v) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr));
+__device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t addr, uint32_t *v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_16x128_x2(uint32_t addr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%4], {%0,%1,%2,%3};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -149,19 +158,34 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// Whether the phase is over, without waiting (try_wait may suspend the thread for microseconds).
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
+// Bounded wait, about a second. Short on purpose: instruction fetch bounds this kernel's
+// single-thread roles, because all roles' code competes for the SM's instruction caches (with
+// longer waits and every loop unrolled, 200 KB of it, a wait already satisfied took 350 cycles).
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort,
+                                         int32_t *status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t t0 = static_cast<uint32_t>(clock());
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort) return false;
+    if (static_cast<uint32_t>(clock()) - t0 > 2000000000u) {
+      *abort = 1;
+      *reinterpret_cast<volatile int32_t *>(status) = S8B_ERR_TIMEOUT;
+      return false;
+    }
+  }
+  return true;
 }
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t *bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
 // D[128 x 128] (+)= A (bf16 in TMEM, 8 columns per 16 keys) . B (shared memory)
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
@@ -257,7 +281,7 @@ struct Walk {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k, const ChunkArgs a) {
   using namespace ca;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -266,10 +290,13 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   uint64_t *empty = full + 3;    // [3] K read, V converted, scales read by both softmax groups
   uint64_t *vfull = empty + 3;   // [2] bf16 V written
   uint64_t *vempty = vfull + 2;  // [2] bf16 V read
-  uint64_t *sfull = vempty + 2;  // [2] S of tile A / B ready
-  uint64_t *pfull = sfull + 2;   // [2] P of tile A / B written (S read, O rescaled)
-  uint64_t *ofull = pfull + 2;   // [2] O of tile A / B complete
-  uint64_t *afull = ofull + 2;         // [4] piece announced
+  uint64_t *sfull = vempty + 2;  // [2] a group's S ready
+  uint64_t *pfull = sfull + 2;   // [group][64 keys] P written (S read, O rescaled)
+  uint64_t *pv0 = pfull + 4;     // [2] the first 64 keys' P V is in O
+  uint64_t *ofull = pv0 + 2;     // [2] a piece's O complete
+  uint64_t *bdone = ofull + 2;   // group B left its sums for A (split pieces)
+  uint64_t *btaken = bdone + 1;  // A has read B's O
+  uint64_t *afull = btaken + 1;        // [4] piece announced
   uint64_t *aempty = afull + kPieces;  // [4] piece done by every other role's warp
   uint64_t *qfull = aempty + kPieces, *qempty = qfull + 1, *drained = qempty + 1;
   uint32_t *tmem_base = reinterpret_cast<uint32_t *>(drained + 1);
@@ -277,6 +304,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   int *first = reinterpret_cast<int *>(tmem_base + 2);  // s, g, t, off of this CTA's run
   Piece *pieces = reinterpret_cast<Piece *>(sm + kOffBar + 512);
   static_assert(kPieces * sizeof(Piece) <= 512, "the ring of pieces fits its 512 bytes");
+  float *bsum = reinterpret_cast<float *>(sm + kOffSums);  // [128] reference, sum of B's rows
   long long *pre = reinterpret_cast<long long *>(sm + kOffSeq);
   int *cu = reinterpret_cast<int *>(pre + kMaxSeqs + 1);
   int *ctx = cu + kMaxSeqs + 1;
@@ -292,16 +320,19 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 2);
+      mbar_init(&full[i], a.copies ? 1 : 64);
       mbar_init(&empty[i], 1 + 4 + 4 + 4);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&vfull[i], 4);
       mbar_init(&vempty[i], 1);
-      mbar_init(&sfull[i], 1);
-      mbar_init(&pfull[i], 4);
+      mbar_init(&sfull[i], 2);
+      mbar_init(&pv0[i], 1);
       mbar_init(&ofull[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&pfull[i], 4);
+    mbar_init(bdone, 4);
+    mbar_init(btaken, 4);
     for (int i = 0; i < kPieces; ++i) {
       mbar_init(&afull[i], 1);
       mbar_init(&aempty[i], 15);
@@ -316,6 +347,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
 
   // ---- this CTA's run of units ----
   const int S = a.S;
+#pragma unroll 1
   for (int i = threadIdx.x; i <= S; i += kThreads) {
     const int v = a.cu[i];
     // rows outside the tensors, or lengths that fall: cut to what exists, and said so
@@ -330,13 +362,16 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   }
   __syncthreads();
   if (threadIdx.x == 0)
+#pragma unroll 1
     for (int i = 1; i <= S; ++i)
       if (cu[i] < cu[i - 1]) cu[i] = cu[i - 1];
   __syncthreads();
   const SeqTab tab{pre, cu, ctx};
+#pragma unroll 1
   for (int s = warp; s < S; s += kThreads / 32) {
     const int n = cu[s + 1] - cu[s], nt = (n + 2 * a.TA - 1) / (2 * a.TA);
     int w = 0;
+#pragma unroll 1
     for (int t = lane; t < nt; t += 32) w += item_at(tab, a, s, t).units;
     w = warp_sum_i(w);
     if (lane == 0) pre[s + 1] = static_cast<long long>(w) * a.Hkv;
@@ -344,6 +379,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   __syncthreads();
   if (warp == 0) {
     long long carry = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < S; s0 += 32) {
       long long v = s0 + lane < S ? pre[s0 + lane + 1] : 0;
 #pragma unroll
@@ -363,6 +399,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   const long long u0 = blockIdx.x < ctas ? blockIdx.x * W / ctas : 0;
   const long long u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * W / ctas : 0;
   if (u1 > u0) {
+#pragma unroll 1
     for (int s = threadIdx.x; s < S; s += kThreads)
       if (pre[s] <= u0 && u0 < pre[s + 1]) first[0] = s;
   }
@@ -404,7 +441,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
   // V buffer kt % 2), `np` the pieces with keys. A piece is next()ed by all lanes of a warp.
   int na = 0;
   auto next = [&]() -> const Piece * {
-    const bool got = mbar_wait(&afull[na % kPieces], (na / kPieces) & 1, abort_flag, status);
+    const bool got = bar_wait(&afull[na % kPieces], (na / kPieces) & 1, abort_flag, status);
     if (!__all_sync(0xffffffffu, got)) return nullptr;
     const Piece *p = &pieces[na % kPieces];
     return p->valid ? p : nullptr;
@@ -420,246 +457,283 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
     // rows l / 4 + 8 j (j = 0..3) of its warp's 32, so that a scale read from shared memory
     // serves four rows (with a row per lane the broadcast reads alone took as long as the
     // exponentials: 512 bytes of register writes for 4 values).
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     const int hf = warp >> 2, quad = lane & 3;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + hf * 128 + lanes, to = tmem + 256 + hf * 128 + lanes;
     constexpr uint32_t kLow = 16u << 16;  // rows 16..31 of the warp
-    int kt = 0, ns = 0, np = 0;           // tiles, S tiles of this half, pieces of this half
+    int kt = 0, ns = 0, np = 0, nsp = 0;  // tiles, this group's tiles, its pieces, split pieces
     bool ok = true;
+    auto wait = [&](uint64_t *bar, int par) {
+      ok = bar_wait(bar, par, abort_flag, status);
+      return ok = __all_sync(0xffffffffu, ok);
+    };
     while (const Piece *pc = next()) {
-      const bool active = pc->ntok > hf * a.TA;  // uniform over the half
+      const bool split = pc->ntok <= a.TA;  // one tile of rows: the groups share its key tiles
+      const int tok0 = split ? 0 : hf * a.TA;
       auto q_row = [&](int rr) {  // tile row -> row of q (valid rows)
         const int tok = rr / a.G;
-        return static_cast<size_t>(pc->t0 + hf * a.TA + tok) * a.Hq + pc->g * a.G + (rr - tok * a.G);
+        return static_cast<size_t>(pc->t0 + tok0 + tok) * a.Hq + pc->g * a.G + (rr - tok * a.G);
       };
       auto is_row = [&](int rr) {
         const int tok = rr / a.G;
-        return tok < a.TA && hf * a.TA + tok < pc->ntok;
+        return tok < a.TA && tok0 + tok < pc->ntok;
       };
       float c[4], mr[4], l[4];  // log2(e) scale q_s, reference (a power of 2), sum of own keys
       int lim[4];               // keys the row sees (rows of no token: all, they mask no tile)
+      int least = pc->keys;
+      bool rows = false;        // the warp has rows to answer for
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int rr = 32 * (warp & 3) + (lane >> 2) + 8 * j;
         const bool valid = is_row(rr);
         c[j] = valid ? a.qs[q_row(rr)] * a.c : 0.0f;
-        lim[j] = valid ? min(max(pc->base + hf * a.TA + rr / a.G + 1, 0), pc->keys) : pc->keys;
+        lim[j] = valid ? min(max(pc->base + tok0 + rr / a.G + 1, 0), pc->keys) : pc->keys;
         mr[j] = -INFINITY;
         l[j] = 0.0f;
+        least = min(least, lim[j]);
+        rows = rows || valid;
       }
-      for (int k = pc->k0; k < pc->k1; ++k, ++kt) {
-        const int st = kt % kStages;
-        ok = mbar_wait(&full[st], (kt / kStages) & 1, abort_flag, status);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (active) {
-          ok = mbar_wait(&sfull[hf], ns & 1, abort_flag, status);
+      rows = __any_sync(0xffffffffu, rows);
+      const int whole_tiles = __reduce_min_sync(0xffffffffu, least) / kKeys;
+      const int k0 = pc->k0, k1 = pc->k1;
+      bool fresh = true;  // O holds nothing yet
+      const int step = split ? 2 : 1;
+      for (int k = k0 + (split ? hf : 0); k < k1; k += step) {
+        const int st = (kt + k - k0) % kStages;
+        {
+          uint64_t *pf = pfull + 2 * hf;
+          const int par = ns & 1;
           ++ns;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
+          if (!wait(&sfull[hf], par)) break;
           tc_fence_after();
           // this lane's keys: float2 index 4 * group + quad
           const float2 *ks = reinterpret_cast<const float2 *>(sm + st * kStage + 2 * kTile) + quad;
           const float2 *vs = ks + kKeys / 2;
-          // A piece's first tile and a tile that some row does not see whole take the general
+          // A group's first tile and a tile that some row does not see whole take the general
           // path below. The others take one pass with the reference at hand: binary32 and bf16
           // keep their precision at any magnitude, so the reference has to be near the row's
-          // maximum, not at it, and the tile's sum alone shows whether it still is.
-          const int least = min(min(lim[0], lim[1]), min(lim[2], lim[3]));
-          bool general = __any_sync(0xffffffffu, k == pc->k0 || least < (k + 1) * kKeys);
-          if (!general) {
-            float2 sum[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
+          // maximum, not at it, and the sum of 64 keys alone shows whether it still is.
+          int from = fresh || k >= whole_tiles ? 0 : kKeys;  // general path from this key on
+          if (from != 0 && rows) {
 #pragma unroll 1
-            for (int b = 0; b < 4; ++b) {  // P's columns 16 b .. end before S's from 32 (b + 1) on
-              uint32_t v[2][16], pk[2][8];
-              tmem_ld_16x256_x4(ts + 32 * b, v[0]);
-              tmem_ld_16x256_x4(ts + kLow + 32 * b, v[1]);
-              tmem_wait_ld();
+            for (int sg = 0; sg < 2; ++sg) {
+              float2 sum[4];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float2 kf = ks[16 * b + 4 * q], vf = vs[16 * b + 4 * q];
+              for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
+              uint32_t v[2][2][16], pk[2][16];
+              tmem_ld_16x256_x4(ts + 64 * sg, v[0][0]);
+              tmem_ld_16x256_x4(ts + kLow + 64 * sg, v[0][1]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
-                  const float2 x =
-                      mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
-                  const float2 t = fma2(x, make_float2(c[j], c[j]), make_float2(-mr[j], -mr[j]));
-                  const float2 e = make_float2(ex2(t.x), ex2(t.y));
-                  sum[j] = add2(sum[j], e);
-                  pk[j >> 1][2 * q + (j & 1)] = pack_bf16(mul2(e, vf));
+              for (int b = 0; b < 2; ++b) {
+                tmem_wait_ld();
+                if (b == 0) {
+                  tmem_ld_16x256_x4(ts + 64 * sg + 32, v[1][0]);
+                  tmem_ld_16x256_x4(ts + kLow + 64 * sg + 32, v[1][1]);
                 }
-              }
-              tmem_st_16x128_x4(ts + 16 * b, pk[0]);
-              tmem_st_16x128_x4(ts + kLow + 16 * b, pk[1]);
-            }
-            bool fits = true;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              // the row's sum over its four lanes decides, so that they decide alike
-              float r = sum[j].x + sum[j].y;
-              r += __shfl_xor_sync(0xffffffffu, r, 1);
-              r += __shfl_xor_sync(0xffffffffu, r, 2);
-              fits = fits && r < kSumMax;
-            }
-            general = !__all_sync(0xffffffffu, fits);
-            if (!general) {
+                for (int q = 0; q < 4; ++q) {
+                  const float2 kf = ks[32 * sg + 16 * b + 4 * q], vf = vs[32 * sg + 16 * b + 4 * q];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) l[j] += sum[j].x + sum[j].y;
-            } else {
-              // Rare (a maximum 2^60 times the last reference): P took S's place, so this
-              // warp's S is computed again, from the staged keys and the queries.
-              tmem_wait_st();
-              const uint8_t *kb = sm + st * kStage;
-#pragma unroll 1
-              for (int q = 0; q < 16; ++q) {
-                uint32_t v[8];
-#pragma unroll 1
-                for (int j = 0; j < 4; ++j) {
-                  const int rr = 32 * (warp & 3) + (lane >> 2) + 8 * j, key = 8 * q + 2 * quad;
-                  const int8_t *qr = a.q + (is_row(rr) ? q_row(rr) : 0) * kHd;
-                  int s0 = 0, s1 = 0;
-                  for (int ch = 0; ch < 8; ++ch) {
-                    const int4 x = __ldg(reinterpret_cast<const int4 *>(qr) + ch);
-                    const int4 y = *reinterpret_cast<const int4 *>(
-                        kb + key * kHd + ((ch ^ (key & 7)) * 16));
-                    const int4 z = *reinterpret_cast<const int4 *>(
-                        kb + (key + 1) * kHd + ((ch ^ ((key + 1) & 7)) * 16));
-                    s0 = __dp4a(x.w, y.w, __dp4a(x.z, y.z, __dp4a(x.y, y.y, __dp4a(x.x, y.x, s0))));
-                    s1 = __dp4a(x.w, z.w, __dp4a(x.z, z.z, __dp4a(x.y, z.y, __dp4a(x.x, z.x, s1))));
+                  for (int j = 0; j < 4; ++j) {
+                    const int *s = reinterpret_cast<const int *>(v[b][j >> 1]) + 4 * q + 2 * (j & 1);
+                    const float2 x =
+                        mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
+                    const float2 t = fma2(x, make_float2(c[j], c[j]), make_float2(-mr[j], -mr[j]));
+                    const float2 e = make_float2(ex2(t.x), ex2(t.y));
+                    sum[j] = add2(sum[j], e);
+                    pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(mul2(e, vf));
                   }
-#pragma unroll
-                  for (int u = 0; u < 4; ++u)
-                    if (u == j) v[2 * u] = s0, v[2 * u + 1] = s1;
                 }
-                tmem_st_16x256_x1(ts + 8 * q, v);
-                tmem_st_16x256_x1(ts + kLow + 8 * q, v + 4);
               }
+              bool fits = true;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                sum[j].x += sum[j].y;
+                fits = fits && sum[j].x < kSumMax;
+              }
+              if (!__all_sync(0xffffffffu, fits)) {  // S is still there: again, with its maximum
+                from = 64 * sg;
+                break;
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
+              tmem_st_16x128_x8(ts + 32 * sg, pk[0]);
+              tmem_st_16x128_x8(ts + kLow + 32 * sg, pk[1]);
               tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&pf[sg]);
             }
           }
-          if (general) {
+          if (from != kKeys || !rows) {
             // Two passes, keys masked by row: the maximum first. The reference moves only where
             // the maximum passed it by 2^8, so that O is rarely rescaled.
-            float mx[4];
+            if (rows) {
+              float mx[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mx[j] = -INFINITY;
+              for (int j = 0; j < 4; ++j) mx[j] = -INFINITY;
 #pragma unroll 1
-            for (int q = 0; q < 16; ++q) {
-              uint32_t v[8];
-              tmem_ld_16x256_x1(ts + 8 * q, v);
-              tmem_ld_16x256_x1(ts + kLow + 8 * q, v + 4);
-              tmem_wait_ld();
-              const float2 kf = ks[4 * q];
-              const int key = k * kKeys + 8 * q + 2 * quad;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float x0 = static_cast<float>(static_cast<int>(v[2 * j])) * kf.x;
-                const float x1 = static_cast<float>(static_cast<int>(v[2 * j + 1])) * kf.y;
-                if (key < lim[j]) mx[j] = fmaxf(mx[j], x0);
-                if (key + 1 < lim[j]) mx[j] = fmaxf(mx[j], x1);
-              }
-            }
-            float al[4];
-            bool moved = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
-              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
-              const float tm = mx[j] == -INFINITY ? -INFINITY : c[j] * mx[j];
-              const bool move = tm > -INFINITY && (mr[j] == -INFINITY || tm - mr[j] > 8.0f);
-              al[j] = move && mr[j] != -INFINITY ? ex2(mr[j] - tm) : 1.0f;
-              if (move) mr[j] = tm;
-              l[j] *= al[j];
-              moved = moved || move;
-            }
-            if (__any_sync(0xffffffffu, moved) && k > pc->k0) {
-#pragma unroll 1
-              for (int q = 0; q < 16; ++q) {
-                uint32_t v[8];
-                tmem_ld_16x256_x1(to + 8 * q, v);
-                tmem_ld_16x256_x1(to + kLow + 8 * q, v + 4);
+              for (int b = from; b < kKeys; b += 16) {
+                uint32_t v[2][8];
+                tmem_ld_16x256_x2(ts + b, v[0]);
+                tmem_ld_16x256_x2(ts + kLow + b, v[1]);
                 tmem_wait_ld();
+                const int key = k * kKeys + b + 2 * quad;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  v[j] = __float_as_uint(__uint_as_float(v[j]) * al[j >> 1]);
-                tmem_st_16x256_x1(to + 8 * q, v);
-                tmem_st_16x256_x1(to + kLow + 8 * q, v + 4);
+                for (int q = 0; q < 2; ++q) {
+                  const float2 kf = ks[b / 2 + 4 * q];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
+                    const float x0 = static_cast<float>(s[0]) * kf.x;
+                    const float x1 = static_cast<float>(s[1]) * kf.y;
+                    if (key + 8 * q < lim[j]) mx[j] = fmaxf(mx[j], x0);
+                    if (key + 8 * q + 1 < lim[j]) mx[j] = fmaxf(mx[j], x1);
+                  }
+                }
               }
-            }
-#pragma unroll 1
-            for (int q = 0; q < 16; ++q) {  // P's columns 4 q .. end before S's from 8 q on
-              uint32_t v[8], pk[4];
-              tmem_ld_16x256_x1(ts + 8 * q, v);
-              tmem_ld_16x256_x1(ts + kLow + 8 * q, v + 4);
-              tmem_wait_ld();
-              const float2 kf = ks[4 * q], vf = vs[4 * q];
-              const int key = k * kKeys + 8 * q + 2 * quad;
+              float al[4];
+              bool moved = false;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float nm = mr[j] == -INFINITY ? 0.0f : -mr[j];
-                const float x0 = static_cast<float>(static_cast<int>(v[2 * j])) * kf.x;
-                const float x1 = static_cast<float>(static_cast<int>(v[2 * j + 1])) * kf.y;
-                // a hidden key's codes and scales may hold anything
-                const bool s0 = key < lim[j], s1 = key + 1 < lim[j];
-                const float e0 = s0 ? ex2(fmaf(x0, c[j], nm)) : 0.0f;
-                const float e1 = s1 ? ex2(fmaf(x1, c[j], nm)) : 0.0f;
-                l[j] += e0 + e1;
-                pk[j] = pack_bf16(make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f));
+                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
+                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
+                const float tm = mx[j] == -INFINITY ? -INFINITY : c[j] * mx[j];
+                const bool move = tm > -INFINITY && (mr[j] == -INFINITY || tm - mr[j] > 8.0f);
+                al[j] = move && mr[j] != -INFINITY ? ex2(mr[j] - tm) : 1.0f;
+                if (move) mr[j] = tm;
+                l[j] *= al[j];
+                moved = moved || move;
               }
-              tmem_st_16x128_x1(ts + 4 * q, pk);
-              tmem_st_16x128_x1(ts + kLow + 4 * q, pk + 2);
+              if (__any_sync(0xffffffffu, moved) && !fresh) {
+                // the first half's product must be in O before O is rescaled
+                if (from != 0 && !wait(&pv0[hf], par)) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int q = 0; q < 16; ++q) {
+                  uint32_t v[8];
+                  tmem_ld_16x256_x1(to + 8 * q, v);
+                  tmem_ld_16x256_x1(to + kLow + 8 * q, v + 4);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int j = 0; j < 8; ++j)
+                    v[j] = __float_as_uint(__uint_as_float(v[j]) * al[j >> 1]);
+                  tmem_st_16x256_x1(to + 8 * q, v);
+                  tmem_st_16x256_x1(to + kLow + 8 * q, v + 4);
+                }
+              }
+#pragma unroll 1
+              for (int b = from; b < kKeys; b += 16) {  // P's columns b / 2 .. end before S's
+                uint32_t v[2][8], pk[2][4];
+                tmem_ld_16x256_x2(ts + b, v[0]);
+                tmem_ld_16x256_x2(ts + kLow + b, v[1]);
+                tmem_wait_ld();
+                const int key = k * kKeys + b + 2 * quad;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const float2 kf = ks[b / 2 + 4 * q], vf = vs[b / 2 + 4 * q];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
+                    const float nm = mr[j] == -INFINITY ? 0.0f : -mr[j];
+                    const float x0 = static_cast<float>(s[0]) * kf.x;
+                    const float x1 = static_cast<float>(s[1]) * kf.y;
+                    // a hidden key's codes and scales may hold anything
+                    const bool s0 = key + 8 * q < lim[j], s1 = key + 8 * q + 1 < lim[j];
+                    const float e0 = s0 ? ex2(fmaf(x0, c[j], nm)) : 0.0f;
+                    const float e1 = s1 ? ex2(fmaf(x1, c[j], nm)) : 0.0f;
+                    l[j] += e0 + e1;
+                    pk[j >> 1][2 * q + (j & 1)] =
+                        pack_bf16(make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f));
+                  }
+                }
+                tmem_st_16x128_x2(ts + b / 2, pk[0]);
+                tmem_st_16x128_x2(ts + kLow + b / 2, pk[1]);
+              }
+              tmem_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (from == 0 || !rows) mbar_arrive(&pf[0]);
+              mbar_arrive(&pf[1]);
             }
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[hf]);
+          fresh = false;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
+        if (lane == 0) mbar_arrive_n(&empty[st], step);  // for the other group too where split
       }
       if (!ok) break;
-      if (active) {
-        const bool whole = pc->starts && pc->ends;
-        const bool keys = pc->k1 > pc->k0;
-        if (keys) {
-          ok = mbar_wait(&ofull[hf], np & 1, abort_flag, status);
-          ++np;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-        }
-        // from here on a lane has one row: its sum and reference come from the lanes 4 (r % 8)
-        float lr = 0.0f, rr_m = -INFINITY;
+      kt += k1 - k0;
+      // ---- the piece's result ----
+      const bool mine = !fresh;  // this group took some key tile
+      if (mine) {
+        if (!wait(&ofull[hf], np & 1)) break;
+        ++np;
+        tc_fence_after();
+      }
+      // from here on a lane has one row: its sum and reference come from the lanes 4 (r % 8)
+      float lr = 0.0f, rm = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float s = l[j];
-          s += __shfl_xor_sync(0xffffffffu, s, 1);
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
-          s = __shfl_sync(0xffffffffu, s, 4 * (lane & 7));
-          const float m = __shfl_sync(0xffffffffu, mr[j], 4 * (lane & 7));
-          if (lane >> 3 == j) lr = s, rr_m = m;
+      for (int j = 0; j < 4; ++j) {
+        float s = l[j];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s = __shfl_sync(0xffffffffu, s, 4 * (lane & 7));
+        const float m = __shfl_sync(0xffffffffu, mr[j], 4 * (lane & 7));
+        if (lane >> 3 == j) lr = s, rm = m;
+      }
+      const int row = 32 * (warp & 3) + lane;
+      float wa = 1.0f, wb = 0.0f;  // weights of A's and B's O
+      if (split && k1 > k0 + 1) {
+        // both groups took key tiles of the same rows: A joins B's sums and reads B's O
+        if (hf == 1) {
+          bsum[2 * row] = rm;
+          bsum[2 * row + 1] = lr;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bdone);
+          if (!wait(btaken, nsp & 1)) break;
+          tc_fence_after();
+        } else {
+          if (!wait(bdone, nsp & 1)) break;
+          tc_fence_after();
+          const float mb = bsum[2 * row], lb = bsum[2 * row + 1], m = fmaxf(rm, mb);
+          if (m != -INFINITY) {
+            wa = rm == m ? 1.0f : ex2(rm - m);
+            wb = mb == m ? 1.0f : ex2(mb - m);
+          }
+          lr = (wa == 0.0f ? 0.0f : wa * lr) + (wb == 0.0f ? 0.0f : wb * lb);
+          rm = m;
         }
-        const int row = 32 * (warp & 3) + lane;
-        const bool valid = is_row(row);
+        ++nsp;
+      }
+      if (split ? hf == 0 : pc->ntok > hf * a.TA) {
+        const bool whole = pc->starts && pc->ends;
+        const bool valid = is_row(row), join = split && k1 > k0 + 1;
         const int slot = 2 * blockIdx.x + (pc->starts ? 1 : 0);
         const float inv = 1.0f / lr;  // not used where lr is 0
         T *orow = static_cast<T *>(a.out) + (valid ? q_row(row) : 0) * kHd;
-        float *prow = a.po + slot * slot_o + (hf * kRows + row) * kHd;
+        float *prow = a.po + slot * slot_o + ((tok0 ? kRows : 0) + row) * kHd;
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
           uint32_t v[32];
-          if (keys) {
+          if (mine) {
             tmem_ld32(to + 32 * b, v);
             tmem_wait_ld();
+          }
+          if (join) {
+            uint32_t u[32];
+            tmem_ld32(to + 128 + 32 * b, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float z = wa == 0.0f ? 0.0f : wa * __uint_as_float(v[j]);
+              if (wb != 0.0f) z = fmaf(wb, __uint_as_float(u[j]), z);
+              v[j] = __float_as_uint(z);
+            }
           }
           if (!valid) continue;
           if (whole) {
@@ -682,15 +756,20 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
         }
         tc_fence_before();
         if (!whole && valid) {
-          float *ml = a.ml + slot * slot_ml + (hf * kRows + row) * 2;
-          ml[0] = rr_m;
+          float *ml = a.ml + slot * slot_ml + ((tok0 ? kRows : 0) + row) * 2;
+          ml[0] = rm;
           ml[1] = lr;
+        }
+        if (join) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(btaken);
         }
       }
       done();
     }
   } else if (warp < 12) {
     // --------------------------------------------------------------- V codes to bf16 ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int ct = threadIdx.x - 256;
     const int ch = ct & 7, key0 = ct >> 3;  // 16-byte chunk, first key; keys step by 16
     int kt = 0;
@@ -698,8 +777,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
     while (const Piece *pc = next()) {
       for (int k = pc->k0; k < pc->k1; ++k, ++kt) {
         const int st = kt % kStages, vb = kt & 1;
-        ok = mbar_wait(&full[st], (kt / kStages) & 1, abort_flag, status) &&
-             mbar_wait(&vempty[vb], ((kt >> 1) & 1) ^ 1, abort_flag, status);
+        ok = bar_wait(&full[st], (kt / kStages) & 1, abort_flag, status) &&
+             bar_wait(&vempty[vb], ((kt >> 1) & 1) ^ 1, abort_flag, status);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -736,138 +815,175 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
       done();
     }
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 12) {
       // ------------------------------------------------------------------ MMA issuer ----
+      // All lanes walk the steps, one elected lane issues: descriptors then stay in uniform
+      // registers (in code under `lane == 0` every MMA paid for moving them there, 100 to 190
+      // cycles an MMA against its 65). P goes by 64 keys, so that the tensor pipe starts on the
+      // first half while the softmax is at the second.
       constexpr uint32_t id_s = i8_idesc(128, 128);
+      const bool lead = elect_one();
       const uint64_t qd = sw128_desc(smem_u32(sm + kOffQ));
-      int kt = 0, np = 0, npv[2] = {0, 0};
+      const uint64_t kd0 = sw128_desc(smem_u32(sm)), vd0 = v16_desc(smem_u32(sm + kOffVs));
+      int np = 0, par[2] = {0, 0};
+      int st = 0, stp = 0, vb = 0, vbp = 0;  // next S's stage and phase, next P V's buffer and phase
       bool ok = true;
-      auto wait = [&](uint64_t *bar, int par) {
-        ok = ok && mbar_wait(bar, par, abort_flag, status);
+      auto wait = [&](uint64_t *bar, int parity) {
+        ok = __all_sync(0xffffffffu, bar_wait(bar, parity, abort_flag, status));
         tc_fence_after();
         return ok;
       };
-      // O_hf (+)= P_hf V of key tile j (the count of tiles before it), first: overwrite
-      auto pv = [&](int hf, int j, bool first_tile) {
-        if (!wait(&vfull[j & 1], (j >> 1) & 1) || !wait(&pfull[hf], npv[hf] & 1)) return;
-        ++npv[hf];
-        const uint64_t vd = v16_desc(smem_u32(sm + kOffVs + (j & 1) * kV16));
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          mma_bf16_ts(tmem + 256 + 128 * hf, tmem + 128 * hf + 8 * i, vd + i * (2048 >> 4),
-                      kIdescPv, !(first_tile && i == 0));
-      };
       while (const Piece *pc = next()) {
-        const int k0 = pc->k0, k1 = pc->k1, two = pc->ntok > a.TA;
-        if (k1 > k0 && lane == 0 && wait(qfull, np & 1)) {
-          for (int k = k0; k < k1 && ok; ++k, ++kt) {
-            const int st = kt % kStages;
-            const uint64_t kd = sw128_desc(smem_u32(sm + st * kStage));
-            for (int hf = 0; hf <= two; ++hf) {
-              if (k > k0) pv(hf, kt - 1, k - 1 == k0);
-              if (!ok) break;
-              if (hf == two && k > k0) mma_commit(&vempty[(kt - 1) & 1]);
-              if (hf == 0 && !wait(&full[st], (kt / kStages) & 1)) break;
-#pragma unroll
-              for (int i = 0; i < kHd / 32; ++i)
-                mma_i8(tmem + 128 * hf, qd + hf * (kTile >> 4) + 2 * i, kd + 2 * i, id_s, i != 0);
-              mma_commit(&sfull[hf]);
-            }
-            if (ok) mma_commit(&empty[st]);
-          }
-          if (ok) mma_commit(qempty);
-          for (int hf = 0; hf <= two && ok; ++hf) {
-            pv(hf, kt - 1, k1 - 1 == k0);
-            if (ok) mma_commit(&ofull[hf]);
-          }
-          if (ok) mma_commit(&vempty[(kt - 1) & 1]);
-          ++np;
-        }
-        if (!__all_sync(0xffffffffu, ok)) break;
+        const int n = __shfl_sync(0xffffffffu, pc->k1 - pc->k0, 0);
+        const bool split = __shfl_sync(0xffffffffu, pc->ntok, 0) <= a.TA;
         done();
+        if (n <= 0) continue;
+        if (!wait(qfull, np & 1)) break;
+        // Step e serves group e % 2: P V of its last key tile, then S of its next. Split pieces:
+        // tile e belongs to group e % 2; others: tile e / 2 goes to both groups.
+        const int back = split ? 2 : 1, steps = split ? n + 2 : 2 * (n + 1);
+#pragma unroll 1
+        for (int e = 0; e < steps; ++e) {
+          const int hf = e & 1, i = split ? e : e >> 1, ip = i - back;
+          const bool last_user = split || hf == 1;
+          if (ip >= 0 && ip < n) {
+            if (!wait(&vfull[vb], vbp)) break;
+            const uint64_t vd = vd0 + vb * (kV16 >> 4);
+            const uint32_t d = tmem + 256 + 128 * hf, pa = tmem + 128 * hf;
+            const uint32_t pp = hf ? par[1] : par[0];
+            if (!wait(&pfull[2 * hf], pp)) break;
+            if (lead) {
+              mma_bf16_ts(d, pa, vd, kIdescPv, ip >= back);  // a group's first tile overwrites O
+#pragma unroll
+              for (int q = 1; q < 4; ++q) mma_bf16_ts(d, pa + 8 * q, vd + q * (2048 >> 4), kIdescPv, 1);
+              mma_commit(&pv0[hf]);
+            }
+            __syncwarp();
+            if (!wait(&pfull[2 * hf + 1], pp)) break;
+            if (lead) {
+#pragma unroll
+              for (int q = 4; q < 8; ++q) mma_bf16_ts(d, pa + 8 * q, vd + q * (2048 >> 4), kIdescPv, 1);
+              if (last_user) mma_commit(&vempty[vb]);
+              if (ip >= n - back) mma_commit(&ofull[hf]);
+            }
+            __syncwarp();
+            (hf ? par[1] : par[0]) ^= 1;
+            if (last_user) vb ^= 1, vbp ^= vb == 0;
+          }
+          if (i < n) {
+            if (!wait(&full[st], stp)) break;
+            if (!a.copies) fence_async();  // K was written by plain copies
+            const uint64_t q = qd + (split ? 0 : hf) * (kTile >> 4), kd = kd0 + st * (kStage >> 4);
+            if (lead) {
+              mma_i8(tmem + 128 * hf, q, kd, id_s, 0);
+#pragma unroll
+              for (int x = 1; x < kHd / 32; ++x) mma_i8(tmem + 128 * hf, q + 2 * x, kd + 2 * x, id_s, 1);
+              mma_commit(&sfull[hf]);
+              mbar_arrive(&sfull[hf]);  // passes on what `full` showed: the scales are there
+              if (last_user) mma_commit(&empty[st]);
+            }
+            __syncwarp();
+            if (last_user && ++st == kStages) st = 0, stp ^= 1;
+          }
+        }
+        if (!ok) break;
+        if (lead) mma_commit(qempty);
+        __syncwarp();
+        ++np;
       }
-      if (lane == 0) {
+      if (lead) {
         // nothing may read shared memory or write TMEM any more when they are given back
         mma_commit(drained);
         mbar_drain(drained, 0);
       }
+      __syncwarp();
     } else if (warp < 15) {
-      // --------------------------------------------------------------- K / V loaders ----
-      const bool vwarp = warp == 14;
-      const int8_t *codes = vwarp ? a.vc : a.kc;
-      const float *scales = vwarp ? a.vs : a.ks;
+      // ------------------------------------------------------------------ K / V pages ----
       const int bs = 1 << a.bs_log2;
-      int kt = 0, sent = 0;  // tiles issued, tiles published
+      int kt = 0;
       bool ok = true;
-      auto publish = [&](int pending) {  // the oldest unpublished tile has landed
-        if (pending >= 3) cp_wait<2>();
-        else if (pending == 2) cp_wait<1>();
-        else cp_wait<0>();
-        fence_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[sent % kStages]);
-        ++sent;
-      };
-      while (true) {
-        // what has been issued is published before this warp can wait for another piece: the
-        // walk goes on only when the pieces before it are through
-        while (sent < kt && !__all_sync(0xffffffffu, mbar_test(&afull[na % kPieces],
-                                                               (na / kPieces) & 1)))
-          publish(kt - sent);
-        const Piece *pc = next();
-        if (!pc) break;
+      while (const Piece *pc = next()) {
         const int32_t *bt = a.bt + static_cast<size_t>(pc->s) * a.max_blocks;
-        const int keys = pc->keys, g = pc->g, k1 = pc->k1;
-        for (int k = pc->k0; k < k1; ++k) {
-          const int st = kt % kStages;
-          // tiles that fill the ring are published before their reader must make room
-          while (true) {
-            const bool room = __all_sync(0xffffffffu,
-                                         mbar_test(&empty[st], ((kt / kStages) & 1) ^ 1));
-            if (room) break;
-            if (sent < kt) {
-              publish(kt - sent);
-              continue;
-            }
-            ok = mbar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
-            ok = __all_sync(0xffffffffu, ok);
-            break;
+        const int keys = pc->keys, g = pc->g, k0 = pc->k0, k1 = pc->k1;
+        done();
+        // the page of position pos, as its first row in the pool; -1 behind the keys
+        auto page_row = [&](int pos) -> long long {
+          if (pos >= keys) return -1;
+          int blk = __ldg(bt + (pos >> a.bs_log2));
+          if (static_cast<uint32_t>(blk) >= static_cast<uint32_t>(a.num_blocks)) {
+            *status = S8B_ERR_ARG;  // a page that does not exist: page 0 stands in
+            blk = 0;
           }
-          if (!ok) break;
-          // rows lane, lane + 32, .. of the tile: their rows in the pool
-          uint32_t prow[4];
-          const uint32_t base = smem_u32(sm + st * kStage);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int pos = k * kKeys + lane + 32 * q;
-            prow[q] = 0xffffffffu;
-            if (pos < keys) {
-              int blk = __ldg(bt + (pos >> a.bs_log2));
-              if (static_cast<uint32_t>(blk) >= static_cast<uint32_t>(a.num_blocks)) {
-                *status = S8B_ERR_ARG;  // a page that does not exist: page 0 stands in
-                blk = 0;
+          return (static_cast<long long>(blk) * a.Hkv + g) << a.bs_log2;
+        };
+        if (a.copies) {
+          // A page's rows of one kv head are contiguous: lane i of warp 13 moves the tile's i-th
+          // page by one tensor copy (K, which the MMA wants swizzled) and three plain ones.
+          if (warp == 14) continue;
+          const int rows = min(bs, kKeys), pages = kKeys / rows;
+          long long row = lane < pages ? page_row(k0 * kKeys + lane * rows) : -1;
+          for (int k = k0; k < k1; ++k, ++kt) {
+            const int st = kt % kStages, pos = k * kKeys + lane * rows;
+            const long long at = row < 0 ? -1 : row + (pos & (bs - 1));
+            // the next tile's page ids are on their way while this tile waits for its stage
+            row = k + 1 < k1 && lane < pages ? page_row(pos + kKeys) : -1;
+            ok = bar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            const int n = __popc(__ballot_sync(0xffffffffu, at >= 0));
+            if (lane == 0) mbar_expect_tx(&full[st], n * rows * (2 * kHd + 8));
+            __syncwarp();
+            if (at >= 0) {
+              uint8_t *base = sm + st * kStage, *sc = base + 2 * kTile + lane * rows * 4;
+              tma_load_2d(base + lane * rows * kHd, &map_k, 0, static_cast<int>(at), &full[st]);
+              bulk_load(base + kTile + lane * rows * kHd, a.vc + at * kHd, rows * kHd, &full[st]);
+              bulk_load(sc, a.ks + at, rows * 4, &full[st]);
+              bulk_load(sc + kKeys * 4, a.vs + at, rows * 4, &full[st]);
+            }
+          }
+        } else {
+          // Pages of 1, 2 or 4 keys (less than a swizzle atom), or scales off a 16-byte boundary:
+          // 16-byte copies per row, K by warp 13, V by warp 14.
+          const bool vwarp = warp == 14;
+          const int8_t *codes = vwarp ? a.vc : a.kc;
+          const float *scales = vwarp ? a.vs : a.ks;
+          for (int k = k0; k < k1; ++k, ++kt) {
+            const int st = kt % kStages;
+            ok = bar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            const uint32_t base = smem_u32(sm + st * kStage);
+            const int ch = lane & 7;
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {  // rows 32 q + lane
+              const int pos = k * kKeys + 32 * q + lane;
+              long long at = page_row(pos);
+              if (at >= 0) {
+                at += pos & (bs - 1);
+                cp4(base + 2 * kTile + (vwarp ? kKeys * 4 : 0) + (32 * q + lane) * 4, scales + at);
               }
-              prow[q] = ((static_cast<uint32_t>(blk) * a.Hkv + g) << a.bs_log2) + (pos & (bs - 1));
-              cp4(base + 2 * kTile + (vwarp ? kKeys * 4 : 0) + (lane + 32 * q) * 4, scales + prow[q]);
+#pragma unroll 2
+              for (int j = 0; j < 8; ++j) {
+                const int r = 32 * q + (lane >> 3) + 4 * j;
+                const long long src = __shfl_sync(0xffffffffu, at, r & 31);
+                const uint32_t dst = base + (vwarp ? kTile + r * kHd + ch * 16
+                                                   : r * kHd + ((ch ^ (r & 7)) * 16));
+                if (src >= 0) cp16(dst, codes + src * kHd + ch * 16);
+              }
             }
+            // arrives when this lane's copies have landed; the MMA's warp fences for its proxy
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                             smem_u32(&full[st])) : "memory");
           }
-          const int ch = lane & 7;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int r = (lane >> 3) + 4 * j;
-            const uint32_t p = __shfl_sync(0xffffffffu, prow[j >> 3], r & 31);
-            const uint32_t dst = base + (vwarp ? kTile + r * kHd + ch * 16
-                                               : r * kHd + ((ch ^ (r & 7)) * 16));
-            if (p != 0xffffffffu) cp16(dst, codes + static_cast<size_t>(p) * kHd + ch * 16);
-          }
-          cp_commit();
-          ++kt;
         }
         if (!ok) break;
-        done();
       }
-      while (ok && sent < kt) publish(kt - sent);
-      cp_wait<0>();
+      // nothing may still be on its way when the shared memory goes
+      if (a.copies) {
+        for (int i = max(0, kt - kStages); i < kt; ++i)
+          mbar_drain(&full[i % kStages], (i / kStages) & 1);
+      } else {
+        cp_wait<0>();
+      }
     } else {
       // ----------------------------------------------------- the walk, and Q's loader ----
       Walk w;
@@ -879,7 +995,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
       int np = 0;
       const int ch = lane & 7;
       while (true) {
-        bool ok = mbar_wait(&aempty[na % kPieces], ((na / kPieces) & 1) ^ 1, abort_flag, status);
+        bool ok = bar_wait(&aempty[na % kPieces], ((na / kPieces) & 1) ^ 1, abort_flag, status);
         if (!__all_sync(0xffffffffu, ok)) break;
         Piece *pc = &pieces[na % kPieces];
         if (lane == 0) {
@@ -899,9 +1015,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const Chunk
         ++na;
         if (!pc->valid) break;
         if (pc->k1 <= pc->k0) continue;
-        ok = mbar_wait(qempty, (np & 1) ^ 1, abort_flag, status);
+        ok = bar_wait(qempty, (np & 1) ^ 1, abort_flag, status);
         if (!__all_sync(0xffffffffu, ok)) break;
         const int ntok = pc->ntok, t0 = pc->t0, g = pc->g;
+#pragma unroll 2
         for (int r = lane >> 3; r < kItemRows; r += 4) {
           const int hf = r >> 7, rr = r & 127, tok = rr / a.G;
           const int i = hf * a.TA + tok;
@@ -1036,9 +1153,19 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
   a.num_blocks = num_blocks;
   a.c = scale * 1.4426950408889634f;
   const cudaStream_t st = (cudaStream_t)stream;
+  // bulk copies want 16-byte boundaries, the tensor copy whole 8-row swizzle atoms and row
+  // numbers below 2^31
+  const unsigned long long rows = static_cast<unsigned long long>(num_blocks) * Hkv * block_size;
+  CUtensorMap map_k;
+  memset(&map_k, 0, sizeof(map_k));
+  a.copies = block_size >= 8 && aligned(ks, 16) && aligned(vs, 16) && rows < (1ull << 31);
+  if (a.copies) {
+    const int rc = make_map_2d(&map_k, kc, kHd, rows, kHd, kHd, block_size < kKeys ? block_size : kKeys);
+    if (rc) return rc;
+  }
   S8B_DISPATCH_DTYPE(dtype, T, {
     ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T>), kSmem);
-    cudaError_t e = launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(kThreads), kSmem, st, a);
+    cudaError_t e = launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(kThreads), kSmem, st, map_k, a);
     if (e == cudaSuccess)
       e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, 8), dim3(kMergeWarps * 32), 0, st, a);
     if (e != cudaSuccess) {

@@ -110,6 +110,18 @@ def test_block_sizes(bs):
     c.check(c.run())
 
 
+def test_scales_off_a_16_byte_boundary():
+    """Scale arrays that bulk copies cannot read give the same result."""
+    c = Case([(40, 300), (130, 131)], 8, 2, 16, seed=61)
+    want = c.run()
+    for name in ("ks", "vs"):
+        t = getattr(c, name)
+        buf = torch.zeros(t.numel() + 1, device=DEV)
+        buf[1:] = t.flatten()
+        setattr(c, name, buf[1:].view(t.shape))
+        assert torch.equal(c.run(), want)
+
+
 def test_ragged_batch_with_idle_sequences():
     lens = [(0, 50), (5, 5), (0, 0), (1, 700), (40, 90), (0, 1), (128, 128), (2, 257), (0, 9)]
     c = Case(lens, 32, 8, 16, seed=5)
