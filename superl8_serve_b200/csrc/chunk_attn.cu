@@ -154,6 +154,10 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Arrives on `bar` when all of this thread's cp.async so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], a.copies ? 1 : 64);
+      mbar_init(&full[i], a.copies ? 2 + 32 : 64);
       mbar_init(&empty[i], 1 + 4 + 4 + 4);
     }
     for (int i = 0; i < 2; ++i) {
@@ -527,6 +531,12 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
 #pragma unroll
               for (int b = 0; b < 2; ++b) {
                 tmem_wait_ld();
+                if (sg == 1 && b == 1) {  // the first half's stores have ended meanwhile
+                  tmem_wait_st();
+                  tc_fence_before();
+                  __syncwarp();
+                  if (lane == 0) mbar_arrive(&pf[0]);
+                }
                 if (b == 0) {
                   tmem_ld_16x256_x4(ts + 64 * sg + 32, v[1][0]);
                   tmem_ld_16x256_x4(ts + kLow + 64 * sg + 32, v[1][1]);
@@ -560,10 +570,12 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
               for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
               tmem_st_16x128_x8(ts + 32 * sg, pk[0]);
               tmem_st_16x128_x8(ts + kLow + 32 * sg, pk[1]);
+            }
+            if (from == kKeys) {
               tmem_wait_st();
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&pf[sg]);
+              if (lane == 0) mbar_arrive(&pf[1]);
             }
           }
           if (from != kKeys || !rows) {
@@ -789,9 +801,12 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
         // the chunks of panel 1 store their halves in the other order: banks stay apart
         const int f = ch >> 2;
         uint8_t *d0 = dst + ((un + f) ^ sw) * 16, *d1 = dst + ((un + 1 - f) ^ sw) * 16;
-#pragma unroll 2
+        const uint8_t *s0 = src + 8 * f, *s1 = src + 8 - 8 * f;
+#pragma unroll 4
         for (int i = 0; i < 8; ++i) {
-          const uint4 q = *reinterpret_cast<const uint4 *>(src + i * 16 * kHd);
+          const uint2 a0 = *reinterpret_cast<const uint2 *>(s0 + i * 16 * kHd);
+          const uint2 a1 = *reinterpret_cast<const uint2 *>(s1 + i * 16 * kHd);
+          const uint4 q = make_uint4(a0.x, a0.y, a1.x, a1.y);
           uint4 lo, hi;
           lo.x = codes_bf16(__byte_perm(q.x, 0, 0x4140));
           lo.y = codes_bf16(__byte_perm(q.x, 0, 0x4342));
@@ -801,8 +816,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
           hi.y = codes_bf16(__byte_perm(q.z, 0, 0x4342));
           hi.z = codes_bf16(__byte_perm(q.w, 0, 0x4140));
           hi.w = codes_bf16(__byte_perm(q.w, 0, 0x4342));
-          *reinterpret_cast<uint4 *>(d0 + i * 16 * 128) = f ? hi : lo;
-          *reinterpret_cast<uint4 *>(d1 + i * 16 * 128) = f ? lo : hi;
+          *reinterpret_cast<uint4 *>(d0 + i * 16 * 128) = lo;
+          *reinterpret_cast<uint4 *>(d1 + i * 16 * 128) = hi;
         }
         fence_async();
         __syncwarp();
@@ -918,9 +933,11 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
           return (static_cast<long long>(blk) * a.Hkv + g) << a.bs_log2;
         };
         if (a.copies) {
-          // A page's rows of one kv head are contiguous: lane i of warp 13 moves the tile's i-th
-          // page by one tensor copy (K, which the MMA wants swizzled) and three plain ones.
-          if (warp == 14) continue;
+          // A page's rows of one kv head are contiguous: lane i moves the tile's i-th page, warp 13
+          // its K (a tensor copy, the MMA wants it swizzled), warp 14 its V. One lane's copies
+          // cost the warp some 80 cycles each, so the 32 chunks of 16 bytes of each scale array
+          // go by one cp.async per lane.
+          const bool vwarp = warp == 14;
           const int rows = min(bs, kKeys), pages = kKeys / rows;
           long long row = lane < pages ? page_row(k0 * kKeys + lane * rows) : -1;
           for (int k = k0; k < k1; ++k, ++kt) {
@@ -930,15 +947,22 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
             row = k + 1 < k1 && lane < pages ? page_row(pos + kKeys) : -1;
             ok = bar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            uint8_t *base = sm + st * kStage;
             const int n = __popc(__ballot_sync(0xffffffffu, at >= 0));
-            if (lane == 0) mbar_expect_tx(&full[st], n * rows * (2 * kHd + 8));
+            if (lane == 0) mbar_expect_tx(&full[st], n * rows * kHd);
             __syncwarp();
-            if (at >= 0) {
-              uint8_t *base = sm + st * kStage, *sc = base + 2 * kTile + lane * rows * 4;
+            if (vwarp) {
+              if (at >= 0) bulk_load(base + kTile + lane * rows * kHd, a.vc + at * kHd, rows * kHd, &full[st]);
+              const long long pg = __shfl_sync(0xffffffffu, at, 4 * lane / rows);
+              if (pg >= 0) {
+                const uint32_t sc = smem_u32(base + 2 * kTile) + 16 * lane;
+                const long long s4 = pg + (4 * lane & (rows - 1));
+                cp16(sc, a.ks + s4);
+                cp16(sc + kKeys * 4, a.vs + s4);
+              }
+              cp_arrive(&full[st]);
+            } else if (at >= 0) {
               tma_load_2d(base + lane * rows * kHd, &map_k, 0, static_cast<int>(at), &full[st]);
-              bulk_load(base + kTile + lane * rows * kHd, a.vc + at * kHd, rows * kHd, &full[st]);
-              bulk_load(sc, a.ks + at, rows * 4, &full[st]);
-              bulk_load(sc + kKeys * 4, a.vs + at, rows * 4, &full[st]);
             }
           }
         } else {
@@ -970,9 +994,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                 if (src >= 0) cp16(dst, codes + src * kHd + ch * 16);
               }
             }
-            // arrives when this lane's copies have landed; the MMA's warp fences for its proxy
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
-                             smem_u32(&full[st])) : "memory");
+            cp_arrive(&full[st]);  // the MMA's warp fences for its proxy
           }
         }
         if (!ok) break;
@@ -981,9 +1003,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
       if (a.copies) {
         for (int i = max(0, kt - kStages); i < kt; ++i)
           mbar_drain(&full[i % kStages], (i / kStages) & 1);
-      } else {
-        cp_wait<0>();
       }
+      cp_wait<0>();
     } else {
       // ----------------------------------------------------- the walk, and Q's loader ----
       Walk w;
