@@ -18,10 +18,14 @@
 // one item's keys. An item that a cut splits leaves partials (o, m, l) in the workspace, which
 // chunk_merge_kernel joins in key order, so the result does not depend on timing.
 //
-// Roles (16 warps): 0-3 and 4-7 softmax of tiles A and B (thread = row); 8-11 convert V codes
-// to bf16; 12 issues the MMAs; 13, 14 load K and V pages (cp.async, any block size); 15 loads Q.
+// Roles (16 warps): 0-3 and 4-7 softmax of groups A and B; 8-11 convert V codes to bf16; 12 and
+// 13 issue the MMAs of A and B (one warp for both was the bottleneck: a wait that is already
+// satisfied takes 110 cycles and more, and each tile needs four); 14 walks the work list and
+// loads K pages and scales, 15 loads Q and V pages. Items of one tile of rows (few new tokens)
+// give group B the odd key tiles of the same rows.
 // TMEM: S_A | S_B | O_A | O_B, 128 columns each; the weights P overwrite the S they came from.
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -72,6 +76,7 @@ struct ChunkArgs {
   uint8_t *ws;
   float *ml, *po;
   int T, S, Hq, Hkv, G, TA, bs_log2, max_blocks, num_blocks;
+  int cap;     // positions that a block-table row reaches
   int copies;  // pages go by bulk copies
   float c;     // scale * log2(e)
 };
@@ -183,6 +188,14 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int c0, int c1, int c2,
+                                            uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
@@ -235,8 +248,7 @@ struct Item {
 __device__ __forceinline__ Item item_at(const SeqTab &q, const ChunkArgs &a, int s, int t) {
   Item it;
   const int c0 = q.cu[s], n = q.cu[s + 1] - c0, i0 = t * 2 * a.TA;
-  const int cap = static_cast<int>(min(0x7fffffffll - 256,
-                                       static_cast<long long>(a.max_blocks) << a.bs_log2));
+  const int cap = a.cap;
   it.t0 = c0 + i0;
   it.ntok = min(2 * a.TA, n - i0);
   it.base = q.ctx[s] - n + i0;
@@ -244,6 +256,11 @@ __device__ __forceinline__ Item item_at(const SeqTab &q, const ChunkArgs &a, int
   it.nk = (it.keys + ca::kKeys - 1) / ca::kKeys;
   it.units = max(it.nk, 1);
   return it;
+}
+// Tiles of sequence s (none if it brings no row, or its range is no range).
+__device__ __forceinline__ int tiles_of(const SeqTab &q, const ChunkArgs &a, int s) {
+  const int n = q.cu[s + 1] - q.cu[s];
+  return n <= 0 ? 0 : n <= 2 * a.TA ? 1 : (n + 2 * a.TA - 1) / (2 * a.TA);
 }
 // One piece of a CTA's run: key tiles [k0, k1) of one item. Warp 15 walks the run and announces
 // the pieces to the other roles through a small ring in shared memory (a walk in every role's
@@ -280,18 +297,21 @@ struct Walk {
     if (++g < a.Hkv) return;
     g = 0;
     do ++s;
-    while (s < a.S && q.cu[s + 1] == q.cu[s]);
+    while (s < a.S && q.cu[s + 1] <= q.cu[s]);
   }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k, const ChunkArgs a) {
+__global__ void __launch_bounds__(ca::kThreads, 1) 
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_q, const ChunkArgs a) {
   using namespace ca;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~uintptr_t(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(sm + kOffBar);  // [3] stage loaded
-  uint64_t *empty = full + 3;    // [3] K read, V converted, scales read by both softmax groups
+  uint64_t *full = reinterpret_cast<uint64_t *>(sm + kOffBar);  // [3] K and scales loaded
+  uint64_t *vland = full + 3;    // [3] V codes loaded
+  uint64_t *empty = vland + 3;   // [3] K read, V converted, scales read by both softmax groups
   uint64_t *vfull = empty + 3;   // [2] bf16 V written
   uint64_t *vempty = vfull + 2;  // [2] bf16 V read
   uint64_t *sfull = vempty + 2;  // [2] a group's S ready
@@ -303,7 +323,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
   uint64_t *afull = btaken + 1;        // [4] piece announced
   uint64_t *aempty = afull + kPieces;  // [4] piece done by every other role's warp
   uint64_t *qfull = aempty + kPieces, *qempty = qfull + 1, *drained = qempty + 1;
-  uint32_t *tmem_base = reinterpret_cast<uint32_t *>(drained + 1);
+  uint32_t *tmem_base = reinterpret_cast<uint32_t *>(drained + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base + 1);
   int *first = reinterpret_cast<int *>(tmem_base + 2);  // s, g, t, off of this CTA's run
   Piece *pieces = reinterpret_cast<Piece *>(sm + kOffBar + 512);
@@ -324,12 +344,13 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], a.copies ? 2 + 32 : 64);
-      mbar_init(&empty[i], 1 + 4 + 4 + 4);
+      mbar_init(&full[i], a.copies ? 1 + 32 : 32);
+      mbar_init(&vland[i], a.copies ? 1 : 32);
+      mbar_init(&empty[i], 2 + 4 + 4 + 4);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&vfull[i], 4);
-      mbar_init(&vempty[i], 1);
+      mbar_init(&vempty[i], 2);
       mbar_init(&sfull[i], 2);
       mbar_init(&pv0[i], 1);
       mbar_init(&ofull[i], 1);
@@ -342,8 +363,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
       mbar_init(&aempty[i], 15);
     }
     mbar_init(qfull, 1);
-    mbar_init(qempty, 1);
-    mbar_init(drained, 1);
+    mbar_init(qempty, 2);
+    mbar_init(&drained[0], 1);
+    mbar_init(&drained[1], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -365,19 +387,26 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0)
-#pragma unroll 1
-    for (int i = 1; i <= S; ++i)
-      if (cu[i] < cu[i - 1]) cu[i] = cu[i - 1];
-  __syncthreads();
   const SeqTab tab{pre, cu, ctx};
+  // units of each sequence: a thread adds up few tiles, a warp many
+  constexpr int kFewTiles = 4;
+#pragma unroll 1
+  for (int s = threadIdx.x; s < S; s += kThreads) {
+    const int nt = tiles_of(tab, a, s);
+    if (nt > kFewTiles) continue;
+    int w = 0;
+#pragma unroll 1
+    for (int t = 0; t < nt; ++t) w += item_at(tab, a, s, t).units;
+    pre[s + 1] = static_cast<long long>(w) * a.Hkv;
+  }
 #pragma unroll 1
   for (int s = warp; s < S; s += kThreads / 32) {
-    const int n = cu[s + 1] - cu[s], nt = (n + 2 * a.TA - 1) / (2 * a.TA);
+    const int nt = tiles_of(tab, a, s);
+    if (nt <= kFewTiles) continue;
     int w = 0;
 #pragma unroll 1
     for (int t = lane; t < nt; t += 32) w += item_at(tab, a, s, t).units;
-    w = warp_sum_i(w);
+    w = __reduce_add_sync(0xffffffffu, w);
     if (lane == 0) pre[s + 1] = static_cast<long long>(w) * a.Hkv;
   }
   __syncthreads();
@@ -413,7 +442,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
     const long long per = (pre[s + 1] - pre[s]) / a.Hkv, rem = u0 - pre[s];
     const int g = static_cast<int>(rem / per);
     int r = static_cast<int>(rem - g * per), t0 = 0;
-    const int nt = (cu[s + 1] - cu[s] + 2 * a.TA - 1) / (2 * a.TA);
+    const int nt = tiles_of(tab, a, s);
     while (true) {
       const int u = t0 + lane < nt ? item_at(tab, a, s, t0 + lane).units : 0;
       int v = u;
@@ -514,12 +543,12 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
           // this lane's keys: float2 index 4 * group + quad
           const float2 *ks = reinterpret_cast<const float2 *>(sm + st * kStage + 2 * kTile) + quad;
           const float2 *vs = ks + kKeys / 2;
-          // A group's first tile and a tile that some row does not see whole take the general
-          // path below. The others take one pass with the reference at hand: binary32 and bf16
-          // keep their precision at any magnitude, so the reference has to be near the row's
-          // maximum, not at it, and the sum of 64 keys alone shows whether it still is.
-          int from = fresh || k >= whole_tiles ? 0 : kKeys;  // general path from this key on
-          if (from != 0 && rows) {
+          // One pass with the reference at hand, P released by 64 keys: binary32 and bf16 keep
+          // their precision at any magnitude, so the reference has to be near the row's maximum,
+          // not at it, and the sum of 64 keys alone shows whether it still is. A group's first
+          // tile takes the maximum of its first 16 keys. Returns the key from which the general
+          // path below has to take over (kKeys: none).
+          auto pass = [&](auto masked) -> int {
 #pragma unroll 1
             for (int sg = 0; sg < 2; ++sg) {
               float2 sum[4];
@@ -541,6 +570,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                   tmem_ld_16x256_x4(ts + 64 * sg + 32, v[1][0]);
                   tmem_ld_16x256_x4(ts + kLow + 64 * sg + 32, v[1][1]);
                 }
+                const int key = k * kKeys + 64 * sg + 32 * b + 2 * quad;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                   const float2 kf = ks[32 * sg + 16 * b + 4 * q], vf = vs[32 * sg + 16 * b + 4 * q];
@@ -550,9 +580,15 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                     const float2 x =
                         mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
                     const float2 t = fma2(x, make_float2(c[j], c[j]), make_float2(-mr[j], -mr[j]));
-                    const float2 e = make_float2(ex2(t.x), ex2(t.y));
+                    float2 e = make_float2(ex2(t.x), ex2(t.y));
+                    float2 w = mul2(e, vf);
+                    if constexpr (decltype(masked)::value) {
+                      // a hidden key's codes and scales may hold anything
+                      if (key + 8 * q >= lim[j]) e.x = w.x = 0.0f;
+                      if (key + 8 * q + 1 >= lim[j]) e.y = w.y = 0.0f;
+                    }
                     sum[j] = add2(sum[j], e);
-                    pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(mul2(e, vf));
+                    pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(w);
                   }
                 }
               }
@@ -562,23 +598,44 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                 sum[j].x += sum[j].y;
                 fits = fits && sum[j].x < kSumMax;
               }
-              if (!__all_sync(0xffffffffu, fits)) {  // S is still there: again, with its maximum
-                from = 64 * sg;
-                break;
-              }
+              if (!__all_sync(0xffffffffu, fits)) return 64 * sg;  // S of these keys is still there
 #pragma unroll
               for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
               tmem_st_16x128_x8(ts + 32 * sg, pk[0]);
               tmem_st_16x128_x8(ts + kLow + 32 * sg, pk[1]);
             }
-            if (from == kKeys) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&pf[1]);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pf[1]);
+            return kKeys;
+          };
+          int from = 0;
+          const bool masked = k >= whole_tiles;
+          if (rows && !(fresh && masked)) {
+            if (fresh) {
+              uint32_t v[2][8];
+              tmem_ld_16x256_x2(ts, v[0]);
+              tmem_ld_16x256_x2(ts + kLow, v[1]);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 2 * (j & 1);
+                float m = fmaxf(fmaxf(static_cast<float>(s[0]) * ks[0].x, static_cast<float>(s[1]) * ks[0].y),
+                                fmaxf(static_cast<float>(s[4]) * ks[4].x, static_cast<float>(s[5]) * ks[4].y));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                mr[j] = c[j] * fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+              }
+            }
+            from = masked ? pass(std::true_type{}) : pass(std::false_type{});
+            if (fresh && from != kKeys) {  // as if this had not been: nothing is in O or in l
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (from == 0) mr[j] = -INFINITY;
+              }
             }
           }
-          if (from != kKeys || !rows) {
+          if (from != kKeys) {
             // Two passes, keys masked by row: the maximum first. The reference moves only where
             // the maximum passed it by 2^8, so that O is rarely rescaled.
             if (rows) {
@@ -618,7 +675,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                 l[j] *= al[j];
                 moved = moved || move;
               }
-              if (__any_sync(0xffffffffu, moved) && !fresh) {
+              if (__any_sync(0xffffffffu, moved) && !(fresh && from == 0)) {
                 // the first half's product must be in O before O is rescaled
                 if (from != 0 && !wait(&pv0[hf], par)) break;
                 tc_fence_after();
@@ -668,7 +725,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              if (from == 0 || !rows) mbar_arrive(&pf[0]);
+              if (from == 0) mbar_arrive(&pf[0]);  // released already where the pass stopped later
               mbar_arrive(&pf[1]);
             }
           }
@@ -789,7 +846,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
     while (const Piece *pc = next()) {
       for (int k = pc->k0; k < pc->k1; ++k, ++kt) {
         const int st = kt % kStages, vb = kt & 1;
-        ok = bar_wait(&full[st], (kt / kStages) & 1, abort_flag, status) &&
+        ok = bar_wait(&vland[st], (kt / kStages) & 1, abort_flag, status) &&
              bar_wait(&vempty[vb], ((kt >> 1) & 1) ^ 1, abort_flag, status);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -831,18 +888,19 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == 12) {
-      // ------------------------------------------------------------------ MMA issuer ----
-      // All lanes walk the steps, one elected lane issues: descriptors then stay in uniform
+    if (warp < 14) {
+      // ----------------------------------------------------------------- MMA issuers ----
+      // All lanes walk the tiles, one elected lane issues: descriptors then stay in uniform
       // registers (in code under `lane == 0` every MMA paid for moving them there, 100 to 190
-      // cycles an MMA against its 65). P goes by 64 keys, so that the tensor pipe starts on the
+      // cycles an MMA against its 65). P comes by 64 keys, so that the tensor pipe starts on the
       // first half while the softmax is at the second.
       constexpr uint32_t id_s = i8_idesc(128, 128);
+      const int hf = warp - 12;
       const bool lead = elect_one();
       const uint64_t qd = sw128_desc(smem_u32(sm + kOffQ));
       const uint64_t kd0 = sw128_desc(smem_u32(sm)), vd0 = v16_desc(smem_u32(sm + kOffVs));
-      int np = 0, par[2] = {0, 0};
-      int st = 0, stp = 0, vb = 0, vbp = 0;  // next S's stage and phase, next P V's buffer and phase
+      const uint32_t tmem_s = tmem + 128 * hf, tmem_o = tmem + 256 + 128 * hf;
+      int kt = 0, np = 0, nt = 0;  // tiles before the piece, pieces, this group's tiles
       bool ok = true;
       auto wait = [&](uint64_t *bar, int parity) {
         ok = __all_sync(0xffffffffu, bar_wait(bar, parity, abort_flag, status));
@@ -855,73 +913,126 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
         done();
         if (n <= 0) continue;
         if (!wait(qfull, np & 1)) break;
-        // Step e serves group e % 2: P V of its last key tile, then S of its next. Split pieces:
-        // tile e belongs to group e % 2; others: tile e / 2 goes to both groups.
-        const int back = split ? 2 : 1, steps = split ? n + 2 : 2 * (n + 1);
+        ++np;
+        // a split piece's tile has one reader, which answers for two
+        const int step = split ? 2 : 1;
+        const uint64_t q = qd + (split ? 0 : hf) * (kTile >> 4);
+        auto scores = [&](int j) {  // by the elected lane; K of tile j is there
+          const uint64_t kd = kd0 + (j % kStages) * (kStage >> 4);
+          mma_i8(tmem_s, q, kd, id_s, 0);
+#pragma unroll
+          for (int x = 1; x < kHd / 32; ++x) mma_i8(tmem_s, q + 2 * x, kd + 2 * x, id_s, 1);
+          mma_commit(&sfull[hf]);
+          mbar_arrive(&sfull[hf]);  // passes on what `full` showed: the scales are there
+          mma_commit(&empty[j % kStages]);
+          if (split) mma_commit(&empty[j % kStages]);
+        };
+        auto keys_there = [&](int j) {
+          const bool got = wait(&full[j % kStages], (j / kStages) & 1);
+          if (!a.copies) fence_async();  // K was written by plain copies
+          return got;
+        };
+        int i = split ? hf : 0;
+        if (i < n) {
+          if (!keys_there(kt + i)) break;
+          if (lead) scores(kt + i);
+          __syncwarp();
+        }
 #pragma unroll 1
-        for (int e = 0; e < steps; ++e) {
-          const int hf = e & 1, i = split ? e : e >> 1, ip = i - back;
-          const bool last_user = split || hf == 1;
-          if (ip >= 0 && ip < n) {
-            if (!wait(&vfull[vb], vbp)) break;
-            const uint64_t vd = vd0 + vb * (kV16 >> 4);
-            const uint32_t d = tmem + 256 + 128 * hf, pa = tmem + 128 * hf;
-            const uint32_t pp = hf ? par[1] : par[0];
-            if (!wait(&pfull[2 * hf], pp)) break;
-            if (lead) {
-              mma_bf16_ts(d, pa, vd, kIdescPv, ip >= back);  // a group's first tile overwrites O
+        for (bool first_tile = true; i < n; i += step, first_tile = false, ++nt) {
+          const int j = kt + i, vb = j & 1;
+          const uint64_t vd = vd0 + vb * (kV16 >> 4);
+          if (!wait(&vfull[vb], (j >> 1) & 1) || !wait(&pfull[2 * hf], nt & 1)) break;
+          if (lead) {
+            mma_bf16_ts(tmem_o, tmem_s, vd, kIdescPv, !first_tile);
 #pragma unroll
-              for (int q = 1; q < 4; ++q) mma_bf16_ts(d, pa + 8 * q, vd + q * (2048 >> 4), kIdescPv, 1);
-              mma_commit(&pv0[hf]);
-            }
-            __syncwarp();
-            if (!wait(&pfull[2 * hf + 1], pp)) break;
-            if (lead) {
-#pragma unroll
-              for (int q = 4; q < 8; ++q) mma_bf16_ts(d, pa + 8 * q, vd + q * (2048 >> 4), kIdescPv, 1);
-              if (last_user) mma_commit(&vempty[vb]);
-              if (ip >= n - back) mma_commit(&ofull[hf]);
-            }
-            __syncwarp();
-            (hf ? par[1] : par[0]) ^= 1;
-            if (last_user) vb ^= 1, vbp ^= vb == 0;
+            for (int x = 1; x < 4; ++x)
+              mma_bf16_ts(tmem_o, tmem_s + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
+            mma_commit(&pv0[hf]);
           }
-          if (i < n) {
-            if (!wait(&full[st], stp)) break;
-            if (!a.copies) fence_async();  // K was written by plain copies
-            const uint64_t q = qd + (split ? 0 : hf) * (kTile >> 4), kd = kd0 + st * (kStage >> 4);
-            if (lead) {
-              mma_i8(tmem + 128 * hf, q, kd, id_s, 0);
+          __syncwarp();
+          const bool more = i + step < n;
+          if (more && !keys_there(j + step)) break;
+          if (!wait(&pfull[2 * hf + 1], nt & 1)) break;
+          if (lead) {
 #pragma unroll
-              for (int x = 1; x < kHd / 32; ++x) mma_i8(tmem + 128 * hf, q + 2 * x, kd + 2 * x, id_s, 1);
-              mma_commit(&sfull[hf]);
-              mbar_arrive(&sfull[hf]);  // passes on what `full` showed: the scales are there
-              if (last_user) mma_commit(&empty[st]);
-            }
-            __syncwarp();
-            if (last_user && ++st == kStages) st = 0, stp ^= 1;
+            for (int x = 4; x < 8; ++x)
+              mma_bf16_ts(tmem_o, tmem_s + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
+            mma_commit(&vempty[vb]);
+            if (split) mma_commit(&vempty[vb]);
+            if (more) scores(j + step);
+            else mma_commit(&ofull[hf]);
           }
+          __syncwarp();
         }
         if (!ok) break;
         if (lead) mma_commit(qempty);
         __syncwarp();
-        ++np;
+        kt += n;
       }
       if (lead) {
         // nothing may read shared memory or write TMEM any more when they are given back
-        mma_commit(drained);
-        mbar_drain(drained, 0);
+        mma_commit(&drained[hf]);
+        mbar_drain(&drained[hf], 0);
       }
       __syncwarp();
-    } else if (warp < 15) {
-      // ------------------------------------------------------------------ K / V pages ----
+    } else {
+      // ------------------------------------ the walk, K pages and scales; Q and V pages ----
+      const bool vwarp = warp == 15;
       const int bs = 1 << a.bs_log2;
-      int kt = 0;
+      Walk w;
+      w.s = first[0];
+      w.g = first[1];
+      w.t = first[2];
+      w.off = first[3];
+      w.left = static_cast<int>(u1 - u0);
+      int kt = 0, np = 0;
       bool ok = true;
-      while (const Piece *pc = next()) {
+      while (true) {
+        const Piece *pc;
+        if (vwarp) {
+          pc = next();
+          if (!pc) break;
+        } else {
+          ok = bar_wait(&aempty[na % kPieces], ((na / kPieces) & 1) ^ 1, abort_flag, status);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          Piece *p = &pieces[na % kPieces];
+          if (lane == 0) {
+            w.next(tab, a, p);
+            if (p->valid && p->starts && !p->ends) {
+              // the pieces of this item run up to the CTA that holds its last unit
+              Meta &me = meta[blockIdx.x];
+              me.t0 = p->t0;
+              me.ntok = p->ntok;
+              me.g = p->g;
+              me.last = static_cast<int>(((u1 + p->behind) * ctas - 1) / W);
+              me.valid = 1;
+            }
+            mbar_arrive(&afull[na % kPieces]);
+          }
+          __syncwarp();
+          ++na;
+          if (!p->valid) break;
+          pc = p;
+        }
         const int32_t *bt = a.bt + static_cast<size_t>(pc->s) * a.max_blocks;
         const int keys = pc->keys, g = pc->g, k0 = pc->k0, k1 = pc->k1;
-        done();
+        if (vwarp) {
+          const int t0 = pc->t0, both = pc->ntok > a.TA;
+          done();
+          if (k1 > k0) {
+            // a tile's rows are TA tokens x G heads, which one box of the queries holds in order
+            ok = bar_wait(qempty, (np & 1) ^ 1, abort_flag, status);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            if (lane == 0) {
+              mbar_expect_tx(qfull, (1 + both) * a.TA * a.G * kHd);
+              tma_load_3d(sm + kOffQ, &map_q, 0, g * a.G, t0, qfull);
+              if (both) tma_load_3d(sm + kOffQ + kTile, &map_q, 0, g * a.G, t0 + a.TA, qfull);
+            }
+            __syncwarp();
+            ++np;
+          }
+        }
         // the page of position pos, as its first row in the pool; -1 behind the keys
         auto page_row = [&](int pos) -> long long {
           if (pos >= keys) return -1;
@@ -933,13 +1044,13 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
           return (static_cast<long long>(blk) * a.Hkv + g) << a.bs_log2;
         };
         if (a.copies) {
-          // A page's rows of one kv head are contiguous: lane i moves the tile's i-th page, warp 13
-          // its K (a tensor copy, the MMA wants it swizzled), warp 14 its V. One lane's copies
-          // cost the warp some 80 cycles each, so the 32 chunks of 16 bytes of each scale array
-          // go by one cp.async per lane.
-          const bool vwarp = warp == 14;
+          // A page's rows of one kv head are contiguous: lane i moves the tile's i-th page, K by a
+          // tensor copy (the MMA wants it swizzled), V by a plain one. One lane's copies cost
+          // the warp some 80 cycles each, so the 32 chunks of 16 bytes of each scale array go by
+          // one cp.async per lane.
           const int rows = min(bs, kKeys), pages = kKeys / rows;
           long long row = lane < pages ? page_row(k0 * kKeys + lane * rows) : -1;
+#pragma unroll 1
           for (int k = k0; k < k1; ++k, ++kt) {
             const int st = kt % kStages, pos = k * kKeys + lane * rows;
             const long long at = row < 0 ? -1 : row + (pos & (bs - 1));
@@ -948,11 +1059,16 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
             ok = bar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             uint8_t *base = sm + st * kStage;
+            uint64_t *bar = vwarp ? &vland[st] : &full[st];
             const int n = __popc(__ballot_sync(0xffffffffu, at >= 0));
-            if (lane == 0) mbar_expect_tx(&full[st], n * rows * kHd);
+            if (lane == 0) mbar_expect_tx(bar, n * rows * kHd);
             __syncwarp();
             if (vwarp) {
-              if (at >= 0) bulk_load(base + kTile + lane * rows * kHd, a.vc + at * kHd, rows * kHd, &full[st]);
+              if (at >= 0)
+                bulk_load(base + kTile + lane * rows * kHd, a.vc + at * kHd, rows * kHd, bar);
+            } else {
+              if (at >= 0) tma_load_2d(base + lane * rows * kHd, &map_k, 0, static_cast<int>(at), bar);
+              __syncwarp();
               const long long pg = __shfl_sync(0xffffffffu, at, 4 * lane / rows);
               if (pg >= 0) {
                 const uint32_t sc = smem_u32(base + 2 * kTile) + 16 * lane;
@@ -960,17 +1076,13 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                 cp16(sc, a.ks + s4);
                 cp16(sc + kKeys * 4, a.vs + s4);
               }
-              cp_arrive(&full[st]);
-            } else if (at >= 0) {
-              tma_load_2d(base + lane * rows * kHd, &map_k, 0, static_cast<int>(at), &full[st]);
+              cp_arrive(bar);
             }
           }
         } else {
           // Pages of 1, 2 or 4 keys (less than a swizzle atom), or scales off a 16-byte boundary:
-          // 16-byte copies per row, K by warp 13, V by warp 14.
-          const bool vwarp = warp == 14;
-          const int8_t *codes = vwarp ? a.vc : a.kc;
-          const float *scales = vwarp ? a.vs : a.ks;
+          // 16-byte copies per row.
+#pragma unroll 1
           for (int k = k0; k < k1; ++k, ++kt) {
             const int st = kt % kStages;
             ok = bar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
@@ -981,9 +1093,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
             for (int q = 0; q < 4; ++q) {  // rows 32 q + lane
               const int pos = k * kKeys + 32 * q + lane;
               long long at = page_row(pos);
-              if (at >= 0) {
-                at += pos & (bs - 1);
-                cp4(base + 2 * kTile + (vwarp ? kKeys * 4 : 0) + (32 * q + lane) * 4, scales + at);
+              if (at >= 0) at += pos & (bs - 1);
+              if (at >= 0 && !vwarp) {
+                cp4(base + 2 * kTile + (32 * q + lane) * 4, a.ks + at);
+                cp4(base + 2 * kTile + kKeys * 4 + (32 * q + lane) * 4, a.vs + at);
               }
 #pragma unroll 2
               for (int j = 0; j < 8; ++j) {
@@ -991,70 +1104,20 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
                 const long long src = __shfl_sync(0xffffffffu, at, r & 31);
                 const uint32_t dst = base + (vwarp ? kTile + r * kHd + ch * 16
                                                    : r * kHd + ((ch ^ (r & 7)) * 16));
-                if (src >= 0) cp16(dst, codes + src * kHd + ch * 16);
+                if (src >= 0) cp16(dst, (vwarp ? a.vc : a.kc) + src * kHd + ch * 16);
               }
             }
-            cp_arrive(&full[st]);  // the MMA's warp fences for its proxy
+            cp_arrive(vwarp ? &vland[st] : &full[st]);  // the MMA's warps fence for their proxy
           }
         }
         if (!ok) break;
       }
       // nothing may still be on its way when the shared memory goes
-      if (a.copies) {
+      if (a.copies)
         for (int i = max(0, kt - kStages); i < kt; ++i)
-          mbar_drain(&full[i % kStages], (i / kStages) & 1);
-      }
+          mbar_drain(vwarp ? &vland[i % kStages] : &full[i % kStages], (i / kStages) & 1);
+      if (vwarp && np > 0) mbar_drain(qfull, (np - 1) & 1);
       cp_wait<0>();
-    } else {
-      // ----------------------------------------------------- the walk, and Q's loader ----
-      Walk w;
-      w.s = first[0];
-      w.g = first[1];
-      w.t = first[2];
-      w.off = first[3];
-      w.left = static_cast<int>(u1 - u0);
-      int np = 0;
-      const int ch = lane & 7;
-      while (true) {
-        bool ok = bar_wait(&aempty[na % kPieces], ((na / kPieces) & 1) ^ 1, abort_flag, status);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        Piece *pc = &pieces[na % kPieces];
-        if (lane == 0) {
-          w.next(tab, a, pc);
-          if (pc->valid && pc->starts && !pc->ends) {
-            // the pieces of this item run up to the CTA that holds its last unit
-            Meta &me = meta[blockIdx.x];
-            me.t0 = pc->t0;
-            me.ntok = pc->ntok;
-            me.g = pc->g;
-            me.last = static_cast<int>(((u1 + pc->behind) * ctas - 1) / W);
-            me.valid = 1;
-          }
-          mbar_arrive(&afull[na % kPieces]);
-        }
-        __syncwarp();
-        ++na;
-        if (!pc->valid) break;
-        if (pc->k1 <= pc->k0) continue;
-        ok = bar_wait(qempty, (np & 1) ^ 1, abort_flag, status);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        const int ntok = pc->ntok, t0 = pc->t0, g = pc->g;
-#pragma unroll 2
-        for (int r = lane >> 3; r < kItemRows; r += 4) {
-          const int hf = r >> 7, rr = r & 127, tok = rr / a.G;
-          const int i = hf * a.TA + tok;
-          if (tok < a.TA && i < ntok) {
-            const size_t qrow = static_cast<size_t>(t0 + i) * a.Hq + g * a.G + (rr - tok * a.G);
-            cp16(smem_u32(sm + kOffQ + r * kHd + ((ch ^ (r & 7)) * 16)), a.q + qrow * kHd + ch * 16);
-          }
-        }
-        cp_commit();
-        cp_wait<0>();
-        fence_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(qfull);
-        ++np;
-      }
     }
   }
   tc_fence_before();
@@ -1067,8 +1130,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1) chunk_attn_kernel(const __gri
 
 // -------------------------------------------------------------------------------- merge ----
 // Joins the pieces of an item that CTA boundaries split, in key order: grid (CTAs, row groups),
-// one warp per row at a time, four values per lane.
-constexpr int kMergeWarps = 8;
+// one warp per row at a time; lanes are pieces while the weights are found (a pass over 32
+// pieces at a time), then four output values each.
+constexpr int kMergeWarps = 8, kMergeGroups = 16;
 template <typename T>
 __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const ChunkArgs a) {
   using namespace ca;
@@ -1077,34 +1141,65 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
   const Meta me = reinterpret_cast<const Meta *>(a.ws + kOffMeta)[blockIdx.x];
   if (!me.valid) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x, n = me.last - c0 + 1;
+  auto slot = [&](int i) { return static_cast<size_t>(2 * (c0 + i) + (i == 0)); };
   for (int r = blockIdx.y * kMergeWarps + warp; r < kItemRows; r += gridDim.y * kMergeWarps) {
     const int hf = r >> 7, rr = r & 127, tok = rr / a.G, i = hf * a.TA + tok;
     if (tok >= a.TA || i >= me.ntok) continue;
-    float m = -INFINITY;
-    for (int c = blockIdx.x; c <= me.last; ++c)
-      m = fmaxf(m, a.ml[(2 * c + (c == static_cast<int>(blockIdx.x))) * slot_ml + r * 2]);
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = blockIdx.x; c <= me.last; ++c) {
-      const size_t slot = 2 * c + (c == static_cast<int>(blockIdx.x));
-      const float mi = a.ml[slot * slot_ml + r * 2], li = a.ml[slot * slot_ml + r * 2 + 1];
-      if (mi == -INFINITY && li == 0.0f) continue;  // sees no key of this piece
-      const float wgt = mi == m ? 1.0f : ex2(mi - m);
-      const float4 v = *reinterpret_cast<const float4 *>(a.po + slot * slot_o + r * kHd + 4 * lane);
-      l += wgt * li;
-      o[0] += wgt * v.x;
-      o[1] += wgt * v.y;
-      o[2] += wgt * v.z;
-      o[3] += wgt * v.w;
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b = 0; b < n; b += 32) {
+      float mi = -INFINITY, li = 0.0f;
+      if (b + lane < n) {
+        const float2 v = *reinterpret_cast<const float2 *>(a.ml + slot(b + lane) * slot_ml + r * 2);
+        mi = v.x, li = v.y;
+      }
+      const float mb = fmaxf(m, warp_max(mi));
+      // a piece of which the row sees no key has no weight, and nothing of it is read
+      const float w = mi == -INFINITY ? 0.0f : mi == mb ? 1.0f : ex2(mi - mb);
+      const float old = m == -INFINITY ? 0.0f : m == mb ? 1.0f : ex2(m - mb);
+      m = mb;
+      float s = w == 0.0f ? 0.0f : w * li;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      l = old * l + s;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[x] *= old;
+      const int nb = min(32, n - b);
+#pragma unroll 4
+      for (int x = 0; x < nb; ++x) {
+        const float wx = __shfl_sync(0xffffffffu, w, x);
+        if (wx == 0.0f) continue;
+        const float4 v = *reinterpret_cast<const float4 *>(a.po + slot(b + x) * slot_o + r * kHd + 4 * lane);
+        o[0] += wx * v.x;
+        o[1] += wx * v.y;
+        o[2] += wx * v.z;
+        o[3] += wx * v.w;
+      }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;  // not used where l is 0
     T t[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = from_f32<T>(l == 0.0f ? 0.0f : o[j] * inv);
+    for (int x = 0; x < 4; ++x) t[x] = from_f32<T>(l == 0.0f ? 0.0f : o[x] * inv);
     uint2 raw;
     memcpy(&raw, t, 8);
     const size_t qrow = static_cast<size_t>(me.t0 + i) * a.Hq + me.g * a.G + (rr - tok * a.G);
     *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + qrow * kHd + 4 * lane) = raw;
   }
+}
+
+// 3-D map over the queries [T][Hq][128 B], box {128, G, TA}: a tile's rows in order.
+int make_map_q(CUtensorMap *map, const int8_t *q, int T, int Hq, int G, int TA) {
+  auto fn = encode_fn();
+  if (!fn) return S8B_ERR_CUDA;
+  const cuuint64_t dims[3] = {ca::kHd, static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(T)};
+  const cuuint64_t strides[2] = {ca::kHd, static_cast<cuuint64_t>(Hq) * ca::kHd};
+  const cuuint32_t box[3] = {ca::kHd, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(TA)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t *>(q), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? S8B_OK : S8B_ERR_ALIGN;
 }
 
 int chunk_ctas() { return min(sm_count(), ca::kMaxCtas); }
@@ -1172,13 +1267,16 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
   a.bs_log2 = bs_log2;
   a.max_blocks = max_blocks;
   a.num_blocks = num_blocks;
+  const long long reach = static_cast<long long>(max_blocks) << bs_log2;
+  a.cap = static_cast<int>(reach < 0x7fffff00ll ? reach : 0x7fffff00ll);
   a.c = scale * 1.4426950408889634f;
   const cudaStream_t st = (cudaStream_t)stream;
   // bulk copies want 16-byte boundaries, the tensor copy whole 8-row swizzle atoms and row
   // numbers below 2^31
   const unsigned long long rows = static_cast<unsigned long long>(num_blocks) * Hkv * block_size;
-  CUtensorMap map_k;
+  CUtensorMap map_k, map_q;
   memset(&map_k, 0, sizeof(map_k));
+  if (const int rc = make_map_q(&map_q, q_i8, T_, Hq, a.G, a.TA)) return rc;
   a.copies = block_size >= 8 && aligned(ks, 16) && aligned(vs, 16) && rows < (1ull << 31);
   if (a.copies) {
     const int rc = make_map_2d(&map_k, kc, kHd, rows, kHd, kHd, block_size < kKeys ? block_size : kKeys);
@@ -1186,9 +1284,9 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
   }
   S8B_DISPATCH_DTYPE(dtype, T, {
     ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T>), kSmem);
-    cudaError_t e = launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(kThreads), kSmem, st, map_k, a);
+    cudaError_t e = launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(kThreads), kSmem, st, map_k, map_q, a);
     if (e == cudaSuccess)
-      e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, 8), dim3(kMergeWarps * 32), 0, st, a);
+      e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, kMergeGroups), dim3(kMergeWarps * 32), 0, st, a);
     if (e != cudaSuccess) {
       record_cuda_error(e);
       return S8B_ERR_CUDA;
