@@ -314,10 +314,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
   uint64_t *empty = vland + 3;   // [3] K read, V converted, scales read by both softmax groups
   uint64_t *vfull = empty + 3;   // [2] bf16 V written
   uint64_t *vempty = vfull + 2;  // [2] bf16 V read
-  uint64_t *sfull = vempty + 2;  // [2] a group's S ready
-  uint64_t *pfull = sfull + 2;   // [group][64 keys] P written (S read, O rescaled)
-  uint64_t *pv0 = pfull + 4;     // [2] the first 64 keys' P V is in O
-  uint64_t *ofull = pv0 + 2;     // [2] a piece's O complete
+  uint64_t *sfull = vempty + 2;  // [group][half tile] S ready
+  uint64_t *pfull = sfull + 4;   // [group][half tile] P written (S read, O rescaled)
+  uint64_t *pvin = pfull + 4;    // [group][half tile] P V is in O
+  uint64_t *ofull = pvin + 4;    // [2] a piece's O complete
   uint64_t *bdone = ofull + 2;   // group B left its sums for A (split pieces)
   uint64_t *btaken = bdone + 1;  // A has read B's O
   uint64_t *afull = btaken + 1;        // [4] piece announced
@@ -351,11 +351,13 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&vfull[i], 4);
       mbar_init(&vempty[i], 2);
-      mbar_init(&sfull[i], 2);
-      mbar_init(&pv0[i], 1);
       mbar_init(&ofull[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&pfull[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sfull[i], 2);
+      mbar_init(&pfull[i], 4);
+      mbar_init(&pvin[i], 1);
+    }
     mbar_init(bdone, 4);
     mbar_init(btaken, 4);
     for (int i = 0; i < kPieces; ++i) {
@@ -532,207 +534,186 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       const int k0 = pc->k0, k1 = pc->k1;
       bool fresh = true;  // O holds nothing yet
       const int step = split ? 2 : 1;
-      for (int k = k0 + (split ? hf : 0); k < k1; k += step) {
+      for (int k = k0 + (split ? hf : 0); ok && k < k1; k += step) {
         const int st = (kt + k - k0) % kStages;
-        {
-          uint64_t *pf = pfull + 2 * hf;
-          const int par = ns & 1;
-          ++ns;
-          if (!wait(&sfull[hf], par)) break;
-          tc_fence_after();
-          // this lane's keys: float2 index 4 * group + quad
-          const float2 *ks = reinterpret_cast<const float2 *>(sm + st * kStage + 2 * kTile) + quad;
-          const float2 *vs = ks + kKeys / 2;
-          // One pass with the reference at hand, P released by 64 keys: binary32 and bf16 keep
-          // their precision at any magnitude, so the reference has to be near the row's maximum,
-          // not at it, and the sum of 64 keys alone shows whether it still is. A group's first
-          // tile takes the maximum of its first 16 keys. Returns the key from which the general
-          // path below has to take over (kKeys: none).
-          auto pass = [&](auto masked) -> int {
+        const int par = ns & 1;
+        ++ns;
 #pragma unroll 1
-            for (int sg = 0; sg < 2; ++sg) {
-              float2 sum[4];
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(&sfull[2 * hf + h], par)) break;
+          tc_fence_after();
+          const uint32_t tu = ts + 64 * h;
+          const int key0 = k * kKeys + 64 * h + 2 * quad;  // this lane's first key
+          // its keys' scales: float2 index 4 * group of 8 + quad
+          const float2 *ks =
+              reinterpret_cast<const float2 *>(sm + st * kStage + 2 * kTile) + 32 * h + quad;
+          const float2 *vs = ks + kKeys / 2;
+          // One pass with the reference at hand: binary32 and bf16 keep their precision at any
+          // magnitude, so the reference has to be near the row's maximum, not at it, and the sum
+          // of these keys alone shows whether it still is. Returns whether it was (else nothing
+          // has been written).
+          auto pass = [&](auto masked) -> bool {
+            float2 sum[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
-              uint32_t v[2][2][16], pk[2][16];
-              tmem_ld_16x256_x4(ts + 64 * sg, v[0][0]);
-              tmem_ld_16x256_x4(ts + kLow + 64 * sg, v[0][1]);
+            for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
+            uint32_t v[2][2][16], pk[2][16];
+            tmem_ld_16x256_x4(tu, v[0][0]);
+            tmem_ld_16x256_x4(tu + kLow, v[0][1]);
 #pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                tmem_wait_ld();
-                if (sg == 1 && b == 1) {  // the first half's stores have ended meanwhile
-                  tmem_wait_st();
-                  tc_fence_before();
-                  __syncwarp();
-                  if (lane == 0) mbar_arrive(&pf[0]);
-                }
-                if (b == 0) {
-                  tmem_ld_16x256_x4(ts + 64 * sg + 32, v[1][0]);
-                  tmem_ld_16x256_x4(ts + kLow + 64 * sg + 32, v[1][1]);
-                }
-                const int key = k * kKeys + 64 * sg + 32 * b + 2 * quad;
+            for (int b = 0; b < 2; ++b) {
+              tmem_wait_ld();
+              if (b == 0) {
+                tmem_ld_16x256_x4(tu + 32, v[1][0]);
+                tmem_ld_16x256_x4(tu + kLow + 32, v[1][1]);
+              }
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const float2 kf = ks[32 * sg + 16 * b + 4 * q], vf = vs[32 * sg + 16 * b + 4 * q];
+              for (int q = 0; q < 4; ++q) {
+                const float2 kf = ks[16 * b + 4 * q], vf = vs[16 * b + 4 * q];
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const int *s = reinterpret_cast<const int *>(v[b][j >> 1]) + 4 * q + 2 * (j & 1);
-                    const float2 x =
-                        mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
-                    const float2 t = fma2(x, make_float2(c[j], c[j]), make_float2(-mr[j], -mr[j]));
-                    float2 e = make_float2(ex2(t.x), ex2(t.y));
-                    float2 w = mul2(e, vf);
-                    if constexpr (decltype(masked)::value) {
-                      // a hidden key's codes and scales may hold anything
-                      if (key + 8 * q >= lim[j]) e.x = w.x = 0.0f;
-                      if (key + 8 * q + 1 >= lim[j]) e.y = w.y = 0.0f;
-                    }
-                    sum[j] = add2(sum[j], e);
-                    pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(w);
+                for (int j = 0; j < 4; ++j) {
+                  const int *s = reinterpret_cast<const int *>(v[b][j >> 1]) + 4 * q + 2 * (j & 1);
+                  const float2 x =
+                      mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
+                  const float2 t = fma2(x, make_float2(c[j], c[j]), make_float2(-mr[j], -mr[j]));
+                  float2 e = make_float2(ex2(t.x), ex2(t.y));
+                  float2 w = mul2(e, vf);
+                  if constexpr (decltype(masked)::value) {
+                    // a hidden key's codes and scales may hold anything
+                    if (key0 + 32 * b + 8 * q >= lim[j]) e.x = w.x = 0.0f;
+                    if (key0 + 32 * b + 8 * q + 1 >= lim[j]) e.y = w.y = 0.0f;
                   }
+                  sum[j] = add2(sum[j], e);
+                  pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(w);
                 }
               }
-              bool fits = true;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                sum[j].x += sum[j].y;
-                fits = fits && sum[j].x < kSumMax;
-              }
-              if (!__all_sync(0xffffffffu, fits)) return 64 * sg;  // S of these keys is still there
-#pragma unroll
-              for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
-              tmem_st_16x128_x8(ts + 32 * sg, pk[0]);
-              tmem_st_16x128_x8(ts + kLow + 32 * sg, pk[1]);
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pf[1]);
-            return kKeys;
+            bool fits = true;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              sum[j].x += sum[j].y;
+              fits = fits && sum[j].x < kSumMax;
+            }
+            if (!__all_sync(0xffffffffu, fits)) return false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
+            tmem_st_16x128_x8(tu, pk[0]);
+            tmem_st_16x128_x8(tu + kLow, pk[1]);
+            return true;
           };
-          int from = 0;
           const bool masked = k >= whole_tiles;
+          bool fine = !rows;  // P of a warp without rows is whatever S was: no one reads its O
           if (rows && !(fresh && masked)) {
-            if (fresh) {
+            if (fresh) {  // the first reference: the maximum of 16 keys
               uint32_t v[2][8];
-              tmem_ld_16x256_x2(ts, v[0]);
-              tmem_ld_16x256_x2(ts + kLow, v[1]);
+              tmem_ld_16x256_x2(tu, v[0]);
+              tmem_ld_16x256_x2(tu + kLow, v[1]);
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 2 * (j & 1);
-                float m = fmaxf(fmaxf(static_cast<float>(s[0]) * ks[0].x, static_cast<float>(s[1]) * ks[0].y),
-                                fmaxf(static_cast<float>(s[4]) * ks[4].x, static_cast<float>(s[5]) * ks[4].y));
+                float m = fmaxf(
+                    fmaxf(static_cast<float>(s[0]) * ks[0].x, static_cast<float>(s[1]) * ks[0].y),
+                    fmaxf(static_cast<float>(s[4]) * ks[4].x, static_cast<float>(s[5]) * ks[4].y));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 mr[j] = c[j] * fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
               }
             }
-            from = masked ? pass(std::true_type{}) : pass(std::false_type{});
-            if (fresh && from != kKeys) {  // as if this had not been: nothing is in O or in l
+            fine = masked ? pass(std::true_type{}) : pass(std::false_type{});
+            if (fresh && !fine)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (from == 0) mr[j] = -INFINITY;
-              }
-            }
+              for (int j = 0; j < 4; ++j) mr[j] = -INFINITY;
           }
-          if (from != kKeys) {
+          if (!fine) {
             // Two passes, keys masked by row: the maximum first. The reference moves only where
             // the maximum passed it by 2^8, so that O is rarely rescaled.
-            if (rows) {
-              float mx[4];
+            float mx[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) mx[j] = -INFINITY;
+            for (int j = 0; j < 4; ++j) mx[j] = -INFINITY;
 #pragma unroll 1
-              for (int b = from; b < kKeys; b += 16) {
-                uint32_t v[2][8];
-                tmem_ld_16x256_x2(ts + b, v[0]);
-                tmem_ld_16x256_x2(ts + kLow + b, v[1]);
-                tmem_wait_ld();
-                const int key = k * kKeys + b + 2 * quad;
+            for (int b = 0; b < 64; b += 16) {
+              uint32_t v[2][8];
+              tmem_ld_16x256_x2(tu + b, v[0]);
+              tmem_ld_16x256_x2(tu + kLow + b, v[1]);
+              tmem_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const float2 kf = ks[b / 2 + 4 * q];
+              for (int q = 0; q < 2; ++q) {
+                const float2 kf = ks[b / 2 + 4 * q];
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
-                    const float x0 = static_cast<float>(s[0]) * kf.x;
-                    const float x1 = static_cast<float>(s[1]) * kf.y;
-                    if (key + 8 * q < lim[j]) mx[j] = fmaxf(mx[j], x0);
-                    if (key + 8 * q + 1 < lim[j]) mx[j] = fmaxf(mx[j], x1);
-                  }
+                for (int j = 0; j < 4; ++j) {
+                  const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
+                  const float x0 = static_cast<float>(s[0]) * kf.x;
+                  const float x1 = static_cast<float>(s[1]) * kf.y;
+                  if (key0 + b + 8 * q < lim[j]) mx[j] = fmaxf(mx[j], x0);
+                  if (key0 + b + 8 * q + 1 < lim[j]) mx[j] = fmaxf(mx[j], x1);
                 }
               }
-              float al[4];
-              bool moved = false;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
-                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
-                const float tm = mx[j] == -INFINITY ? -INFINITY : c[j] * mx[j];
-                const bool move = tm > -INFINITY && (mr[j] == -INFINITY || tm - mr[j] > 8.0f);
-                al[j] = move && mr[j] != -INFINITY ? ex2(mr[j] - tm) : 1.0f;
-                if (move) mr[j] = tm;
-                l[j] *= al[j];
-                moved = moved || move;
-              }
-              if (__any_sync(0xffffffffu, moved) && !(fresh && from == 0)) {
-                // the first half's product must be in O before O is rescaled
-                if (from != 0 && !wait(&pv0[hf], par)) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int q = 0; q < 16; ++q) {
-                  uint32_t v[8];
-                  tmem_ld_16x256_x1(to + 8 * q, v);
-                  tmem_ld_16x256_x1(to + kLow + 8 * q, v + 4);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int j = 0; j < 8; ++j)
-                    v[j] = __float_as_uint(__uint_as_float(v[j]) * al[j >> 1]);
-                  tmem_st_16x256_x1(to + 8 * q, v);
-                  tmem_st_16x256_x1(to + kLow + 8 * q, v + 4);
-                }
-              }
-#pragma unroll 1
-              for (int b = from; b < kKeys; b += 16) {  // P's columns b / 2 .. end before S's
-                uint32_t v[2][8], pk[2][4];
-                tmem_ld_16x256_x2(ts + b, v[0]);
-                tmem_ld_16x256_x2(ts + kLow + b, v[1]);
-                tmem_wait_ld();
-                const int key = k * kKeys + b + 2 * quad;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const float2 kf = ks[b / 2 + 4 * q], vf = vs[b / 2 + 4 * q];
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
-                    const float nm = mr[j] == -INFINITY ? 0.0f : -mr[j];
-                    const float x0 = static_cast<float>(s[0]) * kf.x;
-                    const float x1 = static_cast<float>(s[1]) * kf.y;
-                    // a hidden key's codes and scales may hold anything
-                    const bool s0 = key + 8 * q < lim[j], s1 = key + 8 * q + 1 < lim[j];
-                    const float e0 = s0 ? ex2(fmaf(x0, c[j], nm)) : 0.0f;
-                    const float e1 = s1 ? ex2(fmaf(x1, c[j], nm)) : 0.0f;
-                    l[j] += e0 + e1;
-                    pk[j >> 1][2 * q + (j & 1)] =
-                        pack_bf16(make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f));
-                  }
-                }
-                tmem_st_16x128_x2(ts + b / 2, pk[0]);
-                tmem_st_16x128_x2(ts + kLow + b / 2, pk[1]);
-              }
-              tmem_wait_st();
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (from == 0) mbar_arrive(&pf[0]);  // released already where the pass stopped later
-              mbar_arrive(&pf[1]);
+            float al[4];
+            bool moved = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
+              const float tm = mx[j] == -INFINITY ? -INFINITY : c[j] * mx[j];
+              const bool move = tm > -INFINITY && (mr[j] == -INFINITY || tm - mr[j] > 8.0f);
+              al[j] = move && mr[j] != -INFINITY ? ex2(mr[j] - tm) : 1.0f;
+              if (move) mr[j] = tm;
+              l[j] *= al[j];
+              moved = moved || move;
             }
+            if (__any_sync(0xffffffffu, moved) && !fresh) {
+              // the product before this half tile must be in O before O is rescaled
+              if (!wait(&pvin[2 * hf + (h ^ 1)], h ? par : par ^ 1)) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int q = 0; q < 16; ++q) {
+                uint32_t v[8];
+                tmem_ld_16x256_x1(to + 8 * q, v);
+                tmem_ld_16x256_x1(to + kLow + 8 * q, v + 4);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  v[j] = __float_as_uint(__uint_as_float(v[j]) * al[j >> 1]);
+                tmem_st_16x256_x1(to + 8 * q, v);
+                tmem_st_16x256_x1(to + kLow + 8 * q, v + 4);
+              }
+            }
+#pragma unroll 1
+            for (int b = 0; b < 64; b += 16) {  // P's columns b / 2 .. end before S's from b + 16 on
+              uint32_t v[2][8], pk[2][4];
+              tmem_ld_16x256_x2(tu + b, v[0]);
+              tmem_ld_16x256_x2(tu + kLow + b, v[1]);
+              tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const float2 kf = ks[b / 2 + 4 * q], vf = vs[b / 2 + 4 * q];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int *s = reinterpret_cast<const int *>(v[j >> 1]) + 4 * q + 2 * (j & 1);
+                  const float nm = mr[j] == -INFINITY ? 0.0f : -mr[j];
+                  const float x0 = static_cast<float>(s[0]) * kf.x;
+                  const float x1 = static_cast<float>(s[1]) * kf.y;
+                  const bool s0 = key0 + b + 8 * q < lim[j], s1 = key0 + b + 8 * q + 1 < lim[j];
+                  const float e0 = s0 ? ex2(fmaf(x0, c[j], nm)) : 0.0f;
+                  const float e1 = s1 ? ex2(fmaf(x1, c[j], nm)) : 0.0f;
+                  l[j] += e0 + e1;
+                  pk[j >> 1][2 * q + (j & 1)] =
+                      pack_bf16(make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f));
+                }
+              }
+              tmem_st_16x128_x2(tu + b / 2, pk[0]);
+              tmem_st_16x128_x2(tu + kLow + b / 2, pk[1]);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&pfull[2 * hf + h]);
+            if (h == 1) mbar_arrive_n(&empty[st], step);  // for the other group too where split
           }
           fresh = false;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_n(&empty[st], step);  // for the other group too where split
       }
       if (!ok) break;
       kt += k1 - k0;
@@ -892,9 +873,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       // ----------------------------------------------------------------- MMA issuers ----
       // All lanes walk the tiles, one elected lane issues: descriptors then stay in uniform
       // registers (in code under `lane == 0` every MMA paid for moving them there, 100 to 190
-      // cycles an MMA against its 65). P comes by 64 keys, so that the tensor pipe starts on the
-      // first half while the softmax is at the second.
-      constexpr uint32_t id_s = i8_idesc(128, 128);
+      // cycles an MMA against its 65). The group's S is two half tiles of 64 keys: while the softmax
+      // is at one, the other's P V and the next tile's S in its place run here.
+      constexpr uint32_t id_s = i8_idesc(128, 64);
       const int hf = warp - 12;
       const bool lead = elect_one();
       const uint64_t qd = sw128_desc(smem_u32(sm + kOffQ));
@@ -917,15 +898,18 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
         // a split piece's tile has one reader, which answers for two
         const int step = split ? 2 : 1;
         const uint64_t q = qd + (split ? 0 : hf) * (kTile >> 4);
-        auto scores = [&](int j) {  // by the elected lane; K of tile j is there
-          const uint64_t kd = kd0 + (j % kStages) * (kStage >> 4);
-          mma_i8(tmem_s, q, kd, id_s, 0);
+        auto scores = [&](int j, int h) {  // by the elected lane; K of tile j is there
+          const uint64_t kd = kd0 + (j % kStages) * (kStage >> 4) + h * (kTile >> 5);
+          const uint32_t d = tmem_s + 64 * h;
+          mma_i8(d, q, kd, id_s, 0);
 #pragma unroll
-          for (int x = 1; x < kHd / 32; ++x) mma_i8(tmem_s, q + 2 * x, kd + 2 * x, id_s, 1);
-          mma_commit(&sfull[hf]);
-          mbar_arrive(&sfull[hf]);  // passes on what `full` showed: the scales are there
-          mma_commit(&empty[j % kStages]);
-          if (split) mma_commit(&empty[j % kStages]);
+          for (int x = 1; x < kHd / 32; ++x) mma_i8(d, q + 2 * x, kd + 2 * x, id_s, 1);
+          mma_commit(&sfull[2 * hf + h]);
+          mbar_arrive(&sfull[2 * hf + h]);  // passes on what `full` showed: the scales are there
+          if (h == 1) {
+            mma_commit(&empty[j % kStages]);
+            if (split) mma_commit(&empty[j % kStages]);
+          }
         };
         auto keys_there = [&](int j) {
           const bool got = wait(&full[j % kStages], (j / kStages) & 1);
@@ -935,35 +919,39 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
         int i = split ? hf : 0;
         if (i < n) {
           if (!keys_there(kt + i)) break;
-          if (lead) scores(kt + i);
+          if (lead) {
+            scores(kt + i, 0);
+            scores(kt + i, 1);
+          }
           __syncwarp();
         }
 #pragma unroll 1
-        for (bool first_tile = true; i < n; i += step, first_tile = false, ++nt) {
+        for (uint32_t acc = 0; ok && i < n; i += step, ++nt) {
           const int j = kt + i, vb = j & 1;
-          const uint64_t vd = vd0 + vb * (kV16 >> 4);
-          if (!wait(&vfull[vb], (j >> 1) & 1) || !wait(&pfull[2 * hf], nt & 1)) break;
-          if (lead) {
-            mma_bf16_ts(tmem_o, tmem_s, vd, kIdescPv, !first_tile);
-#pragma unroll
-            for (int x = 1; x < 4; ++x)
-              mma_bf16_ts(tmem_o, tmem_s + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
-            mma_commit(&pv0[hf]);
-          }
-          __syncwarp();
           const bool more = i + step < n;
-          if (more && !keys_there(j + step)) break;
-          if (!wait(&pfull[2 * hf + 1], nt & 1)) break;
-          if (lead) {
+          if (!wait(&vfull[vb], (j >> 1) & 1)) break;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            if (h == 0 && more && !keys_there(j + step)) break;
+            if (!wait(&pfull[2 * hf + h], nt & 1)) break;
+            if (lead) {
+              const uint64_t vd = vd0 + vb * (kV16 >> 4) + h * (4 * 2048 >> 4);
+              const uint32_t pa = tmem_s + 64 * h;
+              mma_bf16_ts(tmem_o, pa, vd, kIdescPv, acc);  // a piece's first overwrites O
 #pragma unroll
-            for (int x = 4; x < 8; ++x)
-              mma_bf16_ts(tmem_o, tmem_s + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
-            mma_commit(&vempty[vb]);
-            if (split) mma_commit(&vempty[vb]);
-            if (more) scores(j + step);
-            else mma_commit(&ofull[hf]);
+              for (int x = 1; x < 4; ++x)
+                mma_bf16_ts(tmem_o, pa + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
+              mma_commit(&pvin[2 * hf + h]);
+              if (more) scores(j + step, h);
+              if (h == 1) {
+                mma_commit(&vempty[vb]);
+                if (split) mma_commit(&vempty[vb]);
+                if (!more) mma_commit(&ofull[hf]);
+              }
+            }
+            __syncwarp();
+            acc = 1;
           }
-          __syncwarp();
         }
         if (!ok) break;
         if (lead) mma_commit(qempty);
