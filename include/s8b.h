@@ -484,6 +484,32 @@ int s8b_moe_combine(const void *contrib, const void *topw, const int32_t *topi,
                     const int32_t *assign_pos, void *out, int T, int top_k, int H, int dtype,
                     void *stream);
 
+/* The whole sparse-MoE feed-forward for a few rows (T <= s8b_moe_layer_max_rows(H, F, top_k), 16
+ * where the codes of T rows fit in shared memory) in one launch:
+ *   p = softmax_e(y . gate[e]), the top_k largest (ties: lower expert first), w = p (over their
+ *   sum, at least 1e-9, when norm_topk_prob) * routed_scaling;
+ *   g, u = rows f and F + f of gu_w[e] . xq, times xs and gu_s; a = silu(g) u; (aq, as) =
+ *   quant_rows(a);  out[t] = sum over the row's experts, ascending, of w (aq . d_w[e]) as d_s[e].
+ * y [T,H] dtype (the router's input), xq [T,H] int8 and xs [T] (the same rows quantized, as
+ * s8b_rmsnorm_quant gives both), gate [E,H] fp32, gu_w [E,2F,H] and d_w [E,H,F] int8 with row
+ * scales gu_s [E,2F] and d_s [E,H], out [T,H] dtype. Router sums are float64; everything after
+ * the integer products is binary32, rounded to dtype once: more exact than the route / grouped
+ * GEMM / combine launches above (which round to dtype at every step) and so not equal to them.
+ * The same on every run. H % 16 == 0, F % 16 == 0, H <= 8192, E <= 256, top_k <= 16; y, xq, gate,
+ * gu_w, d_w 16-byte aligned. One cooperative launch with two grid barriers. workspace:
+ * s8b_moe_layer_workspace_size(top_k, F) bytes, 256-byte aligned, its first 256 bytes zero-filled
+ * once; workspace[0] (int32) receives S8B_ERR_TIMEOUT if a barrier gave up (the output is then
+ * invalid, and the caller zero-fills the 256 bytes again). Launches that share a workspace must
+ * be stream-ordered. Replaces SparseMoE.forward for decode rows
+ * (superl8serve/models/moe.py:88-141).                                                     */
+int s8b_moe_layer_max_rows(int H, int F, int top_k);
+size_t s8b_moe_layer_workspace_size(int top_k, int F);
+int s8b_moe_layer(const void *y, const int8_t *xq, const float *xs, const float *gate,
+                  const int8_t *gu_w, const float *gu_s, const int8_t *d_w, const float *d_s,
+                  void *out, int T, int H, int F, int E, int top_k, int norm_topk_prob,
+                  float routed_scaling, void *workspace, size_t workspace_bytes, int dtype,
+                  void *stream);
+
 /* ---- rANS entropy stage --------------------------------------------------------------
  * Static byte-level rANS in the wire format of the reference's optional entropy stage
  * (superl8serve/dist/entropy.py encode / decode, called from superl8serve/dist/__init__.py:

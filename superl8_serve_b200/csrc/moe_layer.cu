@@ -1,0 +1,467 @@
+// A whole sparse-MoE feed-forward for up to 16 rows in one launch (s8b_moe_layer): router,
+// softmax, top-k, the chosen experts' W8A8 gate_up, SwiGLU, int8 quantization, W8A8 down and
+// the weighted sum.
+//
+// With so few rows the layer is the chosen experts' weights read once (3 H F bytes each: 38 MB
+// for one row of a 2048 x 768 x 8 layer, 5.8 us at the measured copy rate), and the seven launches of
+// the general path cost more than that. Here one cooperative launch of one CTA per SM runs
+// three phases with a grid barrier between them:
+//   A  logits: expert e's gate row against every row, a warp per row (float64 sums);
+//   B  every CTA finds all rows' experts by itself (a warp per row, 8 rounds of a warp-wide
+//      maximum), and the (chosen expert, f) pairs, gate row f and up row F + f each, are cut
+//      evenly over all warps of the grid; act = silu(g) u goes to the workspace in binary32;
+//   C  every CTA quantizes the act rows and computes its slice of output columns over all
+//      chosen experts, so the weighted sum needs no third barrier and no atomics.
+// The down weights that a CTA will read are asked into L2 as soon as the experts are known, so
+// HBM streams through the barrier. Products are dp4a on CUDA cores: an expert has one or two rows
+// here, where the stream of weights, not arithmetic, sets the time, and an MMA tile would be
+// empty. Sums over experts are in ascending expert order: the result does not depend on timing.
+//
+// Numerics: logits are float64 sums rounded to binary32; integer products are exact; everything
+// else is binary32, rounded to the activation dtype once, at the end. (The general path rounds
+// to dtype after gate_up, silu, the product, down, the weighting and each addition.)
+#include <cstring>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace s8b {
+namespace {
+
+namespace ml {
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxT = 16, kMaxE = 256, kMaxK = 16, kMaxA = kMaxT * kMaxK;
+constexpr int kMaxH = 8192;
+constexpr size_t kOffBar = 64, kHeader = 256;  // workspace: status word, barrier counter
+constexpr size_t kLogits = kHeader;            // fp32 [T][E]
+constexpr size_t kAct = kLogits + sizeof(float) * kMaxT * kMaxE;  // fp32 [A][F]
+}  // namespace ml
+
+struct MoeArgs {
+  const void *y;
+  const int8_t *xq, *gu_w, *d_w;
+  const float *xs, *gate, *gu_s, *d_s;
+  void *out;
+  uint8_t *ws;
+  int T, H, F, E, k, norm;
+  int code_bytes, slice;  // shared memory: row codes, then [A][slice] contributions
+  float scaling;
+};
+
+// Every thread's writes before are seen by every thread of the grid after. Bounded: false after
+// about a second, with the status word set.
+__device__ bool grid_barrier(uint8_t *ws, int *ok) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned long long *ctr = reinterpret_cast<unsigned long long *>(ws + ml::kOffBar);
+    const unsigned long long n = gridDim.x;
+    __threadfence();
+    const unsigned long long goal = (atomicAdd(ctr, 1ull) / n + 1) * n;
+    const uint32_t t0 = static_cast<uint32_t>(clock());
+    *ok = 1;
+    while (true) {
+      unsigned long long v;
+      asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(ctr) : "memory");
+      if (v >= goal) break;
+      if (static_cast<uint32_t>(clock()) - t0 > 2000000000u) {
+        *reinterpret_cast<volatile int32_t *>(ws) = S8B_ERR_TIMEOUT;
+        *ok = 0;
+        break;
+      }
+    }
+    __threadfence();
+  }
+  __syncthreads();
+  return *ok != 0;
+}
+
+__device__ __forceinline__ int dot16(int4 a, int4 b, int acc) {
+  acc = __dp4a(a.x, b.x, acc);
+  acc = __dp4a(a.y, b.y, acc);
+  acc = __dp4a(a.z, b.z, acc);
+  return __dp4a(a.w, b.w, acc);
+}
+__device__ __forceinline__ int4 ld_stream(const int8_t *p) {  // weights: read once, not kept in L1
+  int4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+// order of logits as unsigned integers; NaN lowest
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return x != x ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+// W weight rows of `bytes` bytes at w[i] against rows x[r] (shared memory, `pitch` bytes apart):
+// sums[i][r] for R rows, complete in every lane. Chunks of 16 bytes, lane by lane, 4 at a time.
+template <int W, int R>
+__device__ __forceinline__ void dot_rows(const int8_t *const (&w)[W], const int8_t *const (&x)[R],
+                                         int bytes, int lane, int (&sums)[W][R]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int r = 0; r < R; ++r) sums[i][r] = 0;
+  for (int c0 = 16 * lane; c0 < bytes; c0 += 4 * 512) {
+    int4 v[W][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        v[i][u] = c0 + 512 * u < bytes ? ld_stream(w[i] + c0 + 512 * u) : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (c0 + 512 * u >= bytes) break;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int4 xv = *reinterpret_cast<const int4 *>(x[r] + c0 + 512 * u);
+#pragma unroll
+        for (int i = 0; i < W; ++i) sums[i][r] = dot16(v[i][u], xv, sums[i][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int r = 0; r < R; ++r) sums[i][r] = __reduce_add_sync(0xffffffffu, sums[i][r]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArgs a) {
+  using namespace ml;
+  extern __shared__ __align__(16) int8_t rows_s[];  // x codes [T][H], later act codes [A][F]
+  __shared__ float topw[kMaxA], scale_s[kMaxA];     // by assignment / by sorted row
+  __shared__ int topi[kMaxA], order[kMaxA];         // expert; sorted row -> assignment t k + j
+  __shared__ int place[kMaxA];                      // assignment -> sorted row
+  __shared__ uint32_t members[kMaxE];               // rows of each expert, a bit each
+  __shared__ int expert[kMaxA], offset[kMaxA + 1];  // chosen experts ascending; their first row
+  __shared__ int n_experts, ok_s;
+  __shared__ uint8_t slot_of[kMaxE];  // its place among the chosen experts
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int T_ = a.T, H = a.H, F = a.F, E = a.E, k = a.k, A = T_ * k;
+  float *logits = reinterpret_cast<float *>(a.ws + kLogits);
+  float *act = reinterpret_cast<float *>(a.ws + kAct);
+  float *contrib = reinterpret_cast<float *>(rows_s + a.code_bytes);  // [A][slice]
+
+  // ---- A: logits ----
+  for (int i = 16 * threadIdx.x; i < T_ * H; i += 16 * kThreads)
+    *reinterpret_cast<int4 *>(rows_s + i) = *reinterpret_cast<const int4 *>(a.xq + i);
+  if (warp < T_) {
+    const T *yr = static_cast<const T *>(a.y) + static_cast<size_t>(warp) * H;
+    for (int e = blockIdx.x; e < E; e += gridDim.x) {
+      const float *g = a.gate + static_cast<size_t>(e) * H;
+      double s0 = 0.0, s1 = 0.0;
+#pragma unroll 4
+      for (int i = 8 * lane; i < H; i += 256) {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(yr + i);
+        const float4 g0 = *reinterpret_cast<const float4 *>(g + i);
+        const float4 g1 = *reinterpret_cast<const float4 *>(g + i + 4);
+        T v[8];
+        memcpy(v, &raw, 16);
+        s0 = fma(static_cast<double>(to_f32(v[0])), static_cast<double>(g0.x), s0);
+        s1 = fma(static_cast<double>(to_f32(v[1])), static_cast<double>(g0.y), s1);
+        s0 = fma(static_cast<double>(to_f32(v[2])), static_cast<double>(g0.z), s0);
+        s1 = fma(static_cast<double>(to_f32(v[3])), static_cast<double>(g0.w), s1);
+        s0 = fma(static_cast<double>(to_f32(v[4])), static_cast<double>(g1.x), s0);
+        s1 = fma(static_cast<double>(to_f32(v[5])), static_cast<double>(g1.y), s1);
+        s0 = fma(static_cast<double>(to_f32(v[6])), static_cast<double>(g1.z), s0);
+        s1 = fma(static_cast<double>(to_f32(v[7])), static_cast<double>(g1.w), s1);
+      }
+      const double s = warp_sum_d(s0 + s1);
+      if (lane == 0) logits[warp * E + e] = static_cast<float>(s);
+    }
+  }
+  for (int i = threadIdx.x; i < E; i += kThreads) members[i] = 0u;
+  if (!grid_barrier(a.ws, &ok_s)) return;
+
+  // ---- B: each row's experts, then their gate_up and SwiGLU ----
+  if (warp < T_) {
+    constexpr int kC = kMaxE / 32;
+    uint32_t key[kC];
+    float l[kC], m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int e = lane + 32 * c;
+      l[c] = e < E ? __ldcg(logits + warp * E + e) : -INFINITY;
+      key[c] = order_key(l[c]);
+      m = fmaxf(m, l[c]);
+    }
+    m = warp_max(m);
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) s += lane + 32 * c < E ? __expf(l[c] - m) : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    uint32_t left = 0;  // this lane's experts that are still to be had
+#pragma unroll
+    for (int c = 0; c < kC; ++c) left |= (lane + 32 * c < E ? 1u : 0u) << c;
+    float total = 0.0f, mine = 0.0f;  // lane j keeps the j-th choice
+    int mine_e = 0;
+    for (int r = 0; r < k; ++r) {  // the largest logit left, the lowest index among equals
+      uint32_t bk = 0;
+      int be = 0x7fffffff;
+      float bl = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        if ((left >> c & 1u) && (key[c] > bk || be == 0x7fffffff)) {
+          bk = key[c];
+          be = lane + 32 * c;
+          bl = l[c];
+        }
+      const uint32_t best = __reduce_max_sync(0xffffffffu, be == 0x7fffffff ? 0u : bk);
+      const int e = __reduce_min_sync(0xffffffffu, bk == best ? be : 0x7fffffff);
+      if (be == e) left &= ~(1u << (e >> 5));
+      const float p = __expf(__shfl_sync(0xffffffffu, bl, e & 31) - m) / s;
+      total += p;
+      if (lane == r) {
+        mine = p;
+        mine_e = e;
+      }
+    }
+    if (lane < k) {
+      topw[warp * k + lane] = (a.norm ? mine / fmaxf(total, 1e-9f) : mine) * a.scaling;
+      topi[warp * k + lane] = mine_e;
+      atomicOr(&members[mine_e], 1u << warp);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {  // chosen experts in ascending order, and where their rows begin
+    int n = 0, rows = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const uint32_t who = e0 + lane < E ? members[e0 + lane] : 0u;
+      const uint32_t hit = __ballot_sync(0xffffffffu, who != 0u);
+      int c = __popc(who), inc = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+      }
+      if (who) {
+        const int at = n + __popc(hit & ((1u << lane) - 1u));
+        expert[at] = e0 + lane;
+        slot_of[e0 + lane] = static_cast<uint8_t>(at);
+        offset[at] = rows + inc - c;
+      }
+      n += __popc(hit);
+      rows += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) {
+      offset[n] = rows;
+      n_experts = n;
+    }
+  }
+  __syncthreads();
+  const int n_ex = n_experts;
+  for (int i = threadIdx.x; i < A; i += kThreads) {
+    const int e = topi[i], t = i / k;
+    const int p = offset[slot_of[e]] + __popc(members[e] & ((1u << t) - 1u));
+    order[p] = i;
+    place[i] = p;
+  }
+  // this CTA's output columns, and their down weights on the way to L2
+  const int h0 = static_cast<int>(static_cast<long long>(blockIdx.x) * H / gridDim.x);
+  const int nh = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * H / gridDim.x) - h0;
+  if (nh > 0)
+    for (int i = threadIdx.x; i < n_ex; i += kThreads) {
+      const int8_t *p = a.d_w + (static_cast<size_t>(expert[i]) * H + h0) * F;
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(nh * F) : "memory");
+    }
+  __syncthreads();
+  {
+    const long long units = static_cast<long long>(n_ex) * F, wg = blockIdx.x * kWarps + warp;
+    const long long nw = static_cast<long long>(gridDim.x) * kWarps;
+    const int u1 = static_cast<int>((wg + 1) * units / nw);
+    for (int u = static_cast<int>(wg * units / nw); u < u1;) {
+      const int at = u / F, f = u - at * F;
+      const int two = u + 1 < u1 && f + 1 < F;  // a second pair of the same expert
+      const size_t base = static_cast<size_t>(expert[at]) * 2 * F;
+      const int f1 = f + two;
+      const int8_t *w[4] = {a.gu_w + (base + f) * H, a.gu_w + (base + F + f) * H,
+                            a.gu_w + (base + f1) * H, a.gu_w + (base + F + f1) * H};
+      const int lo = offset[at], hi = offset[at + 1];
+      for (int p0 = lo; p0 < hi; p0 += 2) {
+        const int pl = min(p0 + 1, hi - 1);
+        const int ta = order[p0] / k, tb = order[pl] / k;
+        const int8_t *x[2] = {rows_s + ta * H, rows_s + tb * H};
+        int sum[4][2];
+        dot_rows<4, 2>(w, x, H, lane, sum);
+        // lane 2 i + r: pair i, row r
+        const int i = lane >> 1 & 1, r = lane & 1;
+        if (lane < 4 && (i == 0 || two) && (r == 0 || pl != p0)) {
+          const float sx = a.xs[r ? tb : ta];
+          const int ff = f + i;
+          const int gs = i ? (r ? sum[2][1] : sum[2][0]) : (r ? sum[0][1] : sum[0][0]);
+          const int us = i ? (r ? sum[3][1] : sum[3][0]) : (r ? sum[1][1] : sum[1][0]);
+          const float g = static_cast<float>(gs) * sx * a.gu_s[base + ff];
+          const float v = static_cast<float>(us) * sx * a.gu_s[base + F + ff];
+          act[static_cast<size_t>(p0 + r) * F + ff] = g / (1.0f + __expf(-g)) * v;
+        }
+      }
+      u += 1 + two;
+    }
+  }
+  if (!grid_barrier(a.ws, &ok_s)) return;
+
+  // ---- C: act codes, then this CTA's columns of the down products ----
+  if (nh == 0) return;
+  for (int p = warp; p < A; p += kWarps) {
+    const float *src = act + static_cast<size_t>(p) * F;
+    float4 v[4];
+    float mx = 0.0f;
+    for (int i0 = 4 * lane; i0 < F; i0 += 512) {  // 4 vectors in flight
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        v[u] = i0 + 128 * u < F ? __ldcg(reinterpret_cast<const float4 *>(src + i0 + 128 * u))
+                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
+    }
+    mx = warp_max(mx);
+    const QParams q = qparams(mx, 127.0f);
+    for (int i0 = 4 * lane; i0 < F; i0 += 512) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 128 * u;
+        if (i >= F) break;
+        if (F > 512) v[u] = __ldcg(reinterpret_cast<const float4 *>(src + i));
+        char4 c;
+        c.x = static_cast<signed char>(qcode(v[u].x, q.inv, 127));
+        c.y = static_cast<signed char>(qcode(v[u].y, q.inv, 127));
+        c.z = static_cast<signed char>(qcode(v[u].z, q.inv, 127));
+        c.w = static_cast<signed char>(qcode(v[u].w, q.inv, 127));
+        *reinterpret_cast<char4 *>(rows_s + static_cast<size_t>(p) * F + i) = c;
+      }
+    }
+    if (lane == 0) scale_s[p] = q.scale;
+  }
+  __syncthreads();
+  {
+    const int per = (nh + 3) / 4, units = n_ex * per;  // four columns of one expert at a time
+    for (int u = warp; u < units; u += kWarps) {
+      const int at = u / per, c0 = 4 * (u - at * per);
+      const size_t row = static_cast<size_t>(expert[at]) * H + h0;
+      const int8_t *w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = a.d_w + (row + min(c0 + i, nh - 1)) * F;
+      const int lo = offset[at], hi = offset[at + 1];
+      for (int p0 = lo; p0 < hi; p0 += 2) {
+        const int pl = min(p0 + 1, hi - 1);
+        const int8_t *x[2] = {rows_s + static_cast<size_t>(p0) * F,
+                              rows_s + static_cast<size_t>(pl) * F};
+        int sum[4][2];
+        dot_rows<4, 2>(w, x, F, lane, sum);
+        const int i = lane >> 1, r = lane & 1;
+        if (lane < 8 && c0 + i < nh && (r == 0 || pl != p0)) {
+          int v = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q == i) v = r ? sum[q][1] : sum[q][0];
+          contrib[(p0 + r) * a.slice + c0 + i] = static_cast<float>(v) * scale_s[p0 + r] * a.d_s[row + c0 + i];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // the rows of a token, in ascending order of their sorted rows, that is of their experts
+  T *out = static_cast<T *>(a.out);
+  for (int i = threadIdx.x; i < T_ * nh; i += kThreads) {
+    const int t = i / nh, c = i - t * nh;
+    float s = 0.0f;
+    int last = -1;
+    for (int j = 0; j < k; ++j) {
+      int next = 0x7fffffff, at = 0;
+      for (int q = 0; q < k; ++q) {
+        const int p = place[t * k + q];
+        if (p > last && p < next) next = p, at = q;
+      }
+      s = fmaf(topw[t * k + at], contrib[next * a.slice + c], s);
+      last = next;
+    }
+    out[static_cast<size_t>(t) * H + h0 + c] = from_f32<T>(s);
+  }
+}
+
+}  // namespace
+}  // namespace s8b
+
+using namespace s8b;
+
+extern "C" size_t s8b_moe_layer_workspace_size(int top_k, int F) {
+  if (top_k <= 0 || top_k > ml::kMaxK || F <= 0) return ml::kAct;
+  return ml::kAct + sizeof(float) * ml::kMaxT * static_cast<size_t>(top_k) * F;
+}
+
+extern "C" int s8b_moe_layer_max_rows(int H, int F, int top_k) {
+  using namespace ml;
+  if (H <= 0 || F <= 0 || top_k <= 0 || top_k > kMaxK || H % 16 || F % 16 || H > kMaxH) return 0;
+  const long long row = H > static_cast<long long>(top_k) * F ? H : static_cast<long long>(top_k) * F;
+  const long long n = (150ll << 10) / row;  // codes in shared memory
+  return static_cast<int>(n < kMaxT ? n : kMaxT);
+}
+
+extern "C" int s8b_moe_layer(const void *y, const int8_t *xq, const float *xs, const float *gate,
+                             const int8_t *gu_w, const float *gu_s, const int8_t *d_w,
+                             const float *d_s, void *out, int T_, int H, int F, int E, int top_k,
+                             int norm_topk_prob, float routed_scaling, void *workspace,
+                             size_t workspace_bytes, int dtype, void *stream) {
+  using namespace ml;
+  if (!y || !xq || !xs || !gate || !gu_w || !gu_s || !d_w || !d_s || !out) return S8B_ERR_ARG;
+  if (dtype != S8B_BF16 && dtype != S8B_FP16) return S8B_ERR_DTYPE;
+  if (T_ < 0 || E <= 0 || E > kMaxE || top_k <= 0 || top_k > E ||
+      T_ > s8b_moe_layer_max_rows(H, F, top_k) ||
+      static_cast<long long>(E) * 2 * F * H > (1ll << 46))
+    return S8B_ERR_SHAPE;
+  if (!aligned(y, 16) || !aligned(xq, 16) || !aligned(gate, 16) || !aligned(gu_w, 16) ||
+      !aligned(d_w, 16) || !aligned(xs, 4) || !aligned(gu_s, 4) || !aligned(d_s, 4) ||
+      !aligned(out, 2))
+    return S8B_ERR_ALIGN;
+  if (!workspace || workspace_bytes < s8b_moe_layer_workspace_size(top_k, F))
+    return S8B_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return S8B_ERR_ALIGN;
+  if (T_ == 0) return S8B_OK;
+  const int sms = tc::sm_count();
+  MoeArgs a = {};
+  a.y = y;
+  a.xq = xq;
+  a.xs = xs;
+  a.gate = gate;
+  a.gu_w = gu_w;
+  a.gu_s = gu_s;
+  a.d_w = d_w;
+  a.d_s = d_s;
+  a.out = out;
+  a.ws = static_cast<uint8_t *>(workspace);
+  a.T = T_;
+  a.H = H;
+  a.F = F;
+  a.E = E;
+  a.k = top_k;
+  a.norm = norm_topk_prob;
+  a.scaling = routed_scaling;
+  const size_t row = H > top_k * F ? H : static_cast<size_t>(top_k) * F;
+  a.code_bytes = static_cast<int>((row * T_ + 15) / 16 * 16);
+  a.slice = (H + sms - 1) / sms;
+  const size_t smem = a.code_bytes + sizeof(float) * T_ * top_k * static_cast<size_t>(a.slice);
+  if (smem > 215 * 1024) return S8B_ERR_SHAPE;
+  S8B_DISPATCH_DTYPE(dtype, TT, {
+    ensure_smem(reinterpret_cast<const void *>(moe_layer_kernel<TT>), smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr;  // the CTAs wait for one another: all must be resident
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_layer_kernel<TT>, a);
+    if (e != cudaSuccess) {
+      record_cuda_error(e);
+      return S8B_ERR_CUDA;
+    }
+  });
+  return check_launch();
+}

@@ -16,6 +16,7 @@ __all__ = [
     "paged_decode_q8", "paged_decode", "embed", "argmax", "codec_encode", "codec_decode",
     "codec_sizes", "decode_workspace_bytes", "moe_route", "moe_gemm_grouped", "moe_combine",
     "sample", "linear_w8a8", "linear_workspace", "paged_chunk_q8", "chunk_workspace",
+    "moe_layer", "moe_layer_workspace", "moe_layer_max_rows",
 ]
 
 
@@ -515,6 +516,47 @@ def moe_combine(contrib, topw, topi, assign_pos):
     out = torch.empty(T, H, dtype=contrib.dtype, device=contrib.device)
     call("s8b_moe_combine", ptr(contrib), ptr(topw), ptr(topi), ptr(assign_pos), ptr(out), T, k,
          H, dtype_code(out.dtype), stream(out.device))
+    return out
+
+
+def moe_layer_max_rows(H: int, F: int, top_k: int) -> int:
+    """Most rows that ``moe_layer`` takes at these sizes (0: none)."""
+    from ._lib import load
+
+    return int(load().s8b_moe_layer_max_rows(H, F, top_k))
+
+
+def moe_layer_workspace(top_k: int, F: int, device) -> torch.Tensor:
+    """Workspace of ``moe_layer`` for these sizes (status word and barrier zeroed)."""
+    from ._lib import load
+
+    ws = torch.empty(int(load().s8b_moe_layer_workspace_size(top_k, F)), dtype=torch.uint8,
+                     device=device)
+    ws[:256].zero_()
+    return ws
+
+
+def moe_layer(y, xq, xs, gate, gu_w, gu_s, d_w, d_s, top_k: int, *, norm_topk_prob: bool = True,
+              scaling: float = 1.0, out=None, workspace=None):
+    """The whole sparse-MoE feed-forward of a few rows in one launch (``s8b_moe_layer``): y [T, H]
+    (router), xq [T, H] int8 and xs [T] (the same rows quantized), gate [E, H] fp32, gu_w
+    [E, 2F, H], gu_s [E, 2F], d_w [E, H, F], d_s [E, H]. Returns [T, H] in y's dtype."""
+    T, H = y.shape
+    E, F = gate.shape[0], d_w.shape[-1]
+    dev, f32, i8 = y.device, torch.float32, torch.int8
+    _check("moe_layer", dev, ("y", y, y.dtype, (T, H)), ("xq", xq, i8, (T, H)), ("xs", xs, f32, (T,)),
+           ("gate", gate, f32, (E, H)), ("gu_w", gu_w, i8, (E, 2 * F, H)),
+           ("gu_s", gu_s, f32, (E, 2 * F)), ("d_w", d_w, i8, (E, H, F)), ("d_s", d_s, f32, (E, H)),
+           ("out", out, y.dtype, (T, H)))
+    code = dtype_code(y.dtype)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((T, H), dtype=y.dtype, device=dev)
+        if workspace is None:
+            workspace = moe_layer_workspace(top_k, F, dev)
+        call("s8b_moe_layer", ptr(y), ptr(xq), ptr(xs), ptr(gate), ptr(gu_w), ptr(gu_s), ptr(d_w),
+             ptr(d_s), ptr(out), T, H, F, E, int(top_k), int(norm_topk_prob), float(scaling),
+             ptr(workspace), workspace.numel(), code, stream(dev))
     return out
 
 

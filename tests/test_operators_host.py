@@ -75,3 +75,35 @@ def test_chunk_wrapper_refusals():
     bt, ctx, cu = (z(s, dtype=torch.int32) for s in ((1, 2), (1,), (2,)))
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         ops.paged_chunk_q8(q, qs, kc, ks, kc, ks, bt, ctx, cu, 0.1)
+
+
+def _moe(lib, **kw):
+    a = dict(y=OK, xq=OK, xs=OK, gate=OK, gu_w=OK, gu_s=OK, d_w=OK, d_s=OK, out=OK, T=4, H=256,
+             F=128, E=16, k=4, norm=1, scaling=1.0, space=OK, size=1 << 30, dt=0)
+    a.update(kw)
+    return lib.s8b_moe_layer(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    *[({n: None}, -8) for n in ("y", "xq", "xs", "gate", "gu_w", "gu_s", "d_w", "d_s", "out")],
+    ({"dt": 2}, -2), ({"T": -1}, -1), ({"T": 17}, -1), ({"H": 264}, -1), ({"F": 120}, -1),
+    ({"H": 0}, -1), ({"H": 8208}, -1), ({"E": 0}, -1), ({"E": 257}, -1), ({"k": 0}, -1),
+    ({"k": 17, "E": 20}, -1), ({"k": 5, "E": 4}, -1), ({"F": 16384, "k": 10}, -1),
+    ({"y": OK + 8}, -3), ({"gu_w": OK + 8}, -3), ({"d_w": OK + 4}, -3), ({"gate": OK + 4}, -3),
+    ({"xs": OK + 2}, -3), ({"out": OK + 1}, -3), ({"space": None}, -7), ({"size": 256}, -7),
+    ({"space": OK + 64}, -3), ({"T": 0}, 0),
+])
+def test_moe_layer_refusals(lib, kw, code):
+    assert _moe(lib, **kw) == code
+
+
+def test_moe_layer_rows():
+    assert ops.moe_layer_max_rows(2048, 768, 8) == 16
+    assert ops.moe_layer_max_rows(256, 16384, 8) == 1  # codes of one row of eight experts
+    assert ops.moe_layer_max_rows(256, 16384, 16) == 0
+    assert ops.moe_layer_max_rows(100, 128, 2) == 0
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        z = torch.zeros
+        ops.moe_layer(z(1, 32), z(1, 32, dtype=torch.int8), z(1), z(2, 32),
+                      z(2, 32, 32, dtype=torch.int8), z(2, 32), z(2, 32, 16, dtype=torch.int8),
+                      z(2, 32), 1)
