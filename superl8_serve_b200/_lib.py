@@ -167,8 +167,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream(device=None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle (by device index where torch offers that: building a Stream
+    object costs more than a microsecond)."""
+    index = getattr(device, "index", device)
+    if _raw_stream is None or type(index) is not int:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(index)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -4,8 +4,6 @@ layer API use the allocating forms."""
 
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
 
 from ._lib import ACTIVATION, CODEC, call, dtype_code, ptr, stream
@@ -22,26 +20,48 @@ __all__ = [
 
 def _on(dev: torch.device):
     """The context that makes ``dev`` current (a launch on a stream of another device than the
-    current one fails); nothing where it already is."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    current one fails)."""
+    return torch.cuda.device(dev)
 
 
-def _check(what: str, dev: torch.device, *tensors):
-    """Each (name, tensor or None, dtype, shape) is a contiguous CUDA tensor of that dtype and
-    shape on ``dev``."""
+def _pointers(what: str, dev: torch.device, *tensors) -> list:
+    """Addresses of (name, tensor or None, dtype, shape) entries, each a contiguous CUDA tensor
+    of that dtype and shape on ``dev``. One pass of cheap comparisons; the first that fails is
+    explained."""
+    index, out = dev.index, []
     for name, t, dt, shape in tensors:
         if t is None:
-            continue
-        if not t.is_cuda:
+            out.append(None)
+        elif (t.get_device() == index and t.dtype is dt and t.shape == shape
+              and t.is_contiguous() and index is not None):
+            out.append(t.data_ptr())
+        elif not t.is_cuda:
             raise RuntimeError(f"{what}: {name} must be a CUDA tensor (no CPU fallback)")
-        if t.device != dev:
+        elif t.get_device() != index:
             raise ValueError(f"{what}: {name} is on {t.device}, not on {dev}")
-        if t.dtype != dt:
+        elif t.dtype is not dt:
             raise ValueError(f"{what}: {name} must be {dt}, got {t.dtype}")
-        if tuple(t.shape) != tuple(shape):
+        elif t.shape != shape:
             raise ValueError(f"{what}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
-        if not t.is_contiguous():
+        else:
             raise ValueError(f"{what}: {name} must be contiguous")
+    return out
+
+
+def _workspace(what: str, dev: torch.device, ws: torch.Tensor) -> tuple[int, int]:
+    if not (ws.is_cuda and ws.get_device() == dev.index and ws.dtype is torch.uint8
+            and ws.is_contiguous()):
+        raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {dev}")
+    return ws.data_ptr(), ws.numel()
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """``call`` with ``dev`` current."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, stream(dev))
+        return
+    with _on(dev):
+        call(name, *args, stream(dev))
 
 
 def quant_rows(x: torch.Tensor):
@@ -143,26 +163,21 @@ def linear_w8a8(xq, xs, w, ws, *, bias=None, activation=None, residual=None, out
         raise ValueError(f"linear_w8a8: unknown activation {activation!r}")
     if xq.dim() < 1 or w.dim() != 2:
         raise ValueError("linear_w8a8: xq must be [..., K] and w [N, K]")
-    K, N, lead, dev = xq.shape[-1], w.shape[0], xq.shape[:-1], xq.device
-    M = 1
-    for n in lead:
-        M *= n
+    (N, K), lead, dev = w.shape, xq.shape[:-1], xq.device
+    M = lead.numel()
     dt = out_dtype if out is None else out.dtype
-    _check("linear_w8a8", dev, ("xq", xq, torch.int8, xq.shape), ("xs", xs, torch.float32, lead),
-           ("w", w, torch.int8, (N, K)), ("ws", ws, torch.float32, (N,)),
-           ("bias", bias, dt, (N,)), ("residual", residual, dt, (*lead, N)),
-           ("out", out, dt, (*lead, N)))
-    code = dtype_code(dt)
-    with _on(dev):
-        if out is None:
-            out = torch.empty((*lead, N), dtype=dt, device=dev)
-        if M == 0:
-            return out
-        if workspace is None:
-            workspace = linear_workspace(M, N, K, dev)
-        call("s8b_linear_w8a8", ptr(xq), ptr(xs), ptr(w), ptr(ws), ptr(bias),
-             ACTIVATION[activation], ptr(residual), ptr(out), M, N, K, code, ptr(workspace),
-             workspace.numel(), stream(dev))
+    code, f32, i8 = dtype_code(dt), torch.float32, torch.int8
+    if out is None:
+        out = torch.empty((*lead, N), dtype=dt, device=dev)
+    p = _pointers("linear_w8a8", dev, ("xq", xq, i8, (*lead, K)), ("xs", xs, f32, lead),
+                  ("w", w, i8, (N, K)), ("ws", ws, f32, (N,)), ("bias", bias, dt, (N,)),
+                  ("residual", residual, dt, (*lead, N)), ("out", out, dt, (*lead, N)))
+    if M == 0:
+        return out
+    if workspace is None:
+        workspace = linear_workspace(M, N, K, dev)
+    _call_on(dev, "s8b_linear_w8a8", *p[:5], ACTIVATION[activation], *p[5:], M, N, K, code,
+             *_workspace("linear_w8a8", dev, workspace))
     return out
 
 
@@ -347,9 +362,9 @@ def chunk_workspace(device) -> torch.Tensor:
     """Workspace of ``paged_chunk_q8``, for calls of any shape (its status word zeroed)."""
     from ._lib import load
 
-    dev = torch.device(device)
-    with _on(dev if dev.index is not None else torch.device(dev.type, torch.cuda.current_device())):
-        ws = torch.empty(int(load().s8b_paged_chunk_workspace_size()), dtype=torch.uint8, device=dev)
+    with _on(torch.device(device)):
+        ws = torch.empty(int(load().s8b_paged_chunk_workspace_size()), dtype=torch.uint8,
+                         device=device)
         ws[:256].zero_()
     return ws
 
@@ -366,21 +381,19 @@ def paged_chunk_q8(q_i8, q_s, kc, ks, vc, vs, block_table, context_lens, cu_q, s
     nb, Hkv, bs, _ = kc.shape
     dev = q_i8.device
     dt = dtype if out is None else out.dtype
-    f32, i32 = torch.float32, torch.int32
-    _check("paged_chunk_q8", dev, ("q_i8", q_i8, torch.int8, (T, Hq, D)), ("q_s", q_s, f32, (T, Hq)),
-           ("kc", kc, torch.int8, (nb, Hkv, bs, D)), ("ks", ks, f32, (nb, Hkv, bs)),
-           ("vc", vc, torch.int8, (nb, Hkv, bs, D)), ("vs", vs, f32, (nb, Hkv, bs)),
-           ("block_table", block_table, i32, (S, maxb)), ("context_lens", context_lens, i32, (S,)),
-           ("cu_q", cu_q, i32, (S + 1,)), ("out", out, dt, (T, Hq * D)))
-    code = dtype_code(dt)
-    with _on(dev):
-        if out is None:
-            out = torch.empty((T, Hq * D), dtype=dt, device=dev)
-        if workspace is None:
-            workspace = chunk_workspace(dev)
-        call("s8b_paged_chunk_q8", ptr(q_i8), ptr(q_s), ptr(kc), ptr(ks), ptr(vc), ptr(vs),
-             ptr(block_table), ptr(context_lens), ptr(cu_q), ptr(out), T, S, Hq, Hkv, D, bs, maxb,
-             nb, float(scale), ptr(workspace), workspace.numel(), code, stream(dev))
+    code, f32, i32, i8 = dtype_code(dt), torch.float32, torch.int32, torch.int8
+    if out is None:
+        out = torch.empty((T, Hq * D), dtype=dt, device=dev)
+    codes, scales = (nb, Hkv, bs, D), (nb, Hkv, bs)
+    p = _pointers("paged_chunk_q8", dev, ("q_i8", q_i8, i8, (T, Hq, D)), ("q_s", q_s, f32, (T, Hq)),
+                  ("kc", kc, i8, codes), ("ks", ks, f32, scales), ("vc", vc, i8, codes),
+                  ("vs", vs, f32, scales), ("block_table", block_table, i32, (S, maxb)),
+                  ("context_lens", context_lens, i32, (S,)), ("cu_q", cu_q, i32, (S + 1,)),
+                  ("out", out, dt, (T, Hq * D)))
+    if workspace is None:
+        workspace = chunk_workspace(dev)
+    _call_on(dev, "s8b_paged_chunk_q8", *p, T, S, Hq, Hkv, D, bs, maxb, nb, float(scale),
+             *_workspace("paged_chunk_q8", dev, workspace), code)
     return out
 
 
@@ -543,20 +556,17 @@ def moe_layer(y, xq, xs, gate, gu_w, gu_s, d_w, d_s, top_k: int, *, norm_topk_pr
     [E, 2F, H], gu_s [E, 2F], d_w [E, H, F], d_s [E, H]. Returns [T, H] in y's dtype."""
     T, H = y.shape
     E, F = gate.shape[0], d_w.shape[-1]
-    dev, f32, i8 = y.device, torch.float32, torch.int8
-    _check("moe_layer", dev, ("y", y, y.dtype, (T, H)), ("xq", xq, i8, (T, H)), ("xs", xs, f32, (T,)),
-           ("gate", gate, f32, (E, H)), ("gu_w", gu_w, i8, (E, 2 * F, H)),
-           ("gu_s", gu_s, f32, (E, 2 * F)), ("d_w", d_w, i8, (E, H, F)), ("d_s", d_s, f32, (E, H)),
-           ("out", out, y.dtype, (T, H)))
-    code = dtype_code(y.dtype)
-    with _on(dev):
-        if out is None:
-            out = torch.empty((T, H), dtype=y.dtype, device=dev)
-        if workspace is None:
-            workspace = moe_layer_workspace(top_k, F, dev)
-        call("s8b_moe_layer", ptr(y), ptr(xq), ptr(xs), ptr(gate), ptr(gu_w), ptr(gu_s), ptr(d_w),
-             ptr(d_s), ptr(out), T, H, F, E, int(top_k), int(norm_topk_prob), float(scaling),
-             ptr(workspace), workspace.numel(), code, stream(dev))
+    dev, f32, i8, dt = y.device, torch.float32, torch.int8, y.dtype
+    if out is None:
+        out = torch.empty((T, H), dtype=dt, device=dev)
+    p = _pointers("moe_layer", dev, ("y", y, dt, (T, H)), ("xq", xq, i8, (T, H)),
+                  ("xs", xs, f32, (T,)), ("gate", gate, f32, (E, H)),
+                  ("gu_w", gu_w, i8, (E, 2 * F, H)), ("gu_s", gu_s, f32, (E, 2 * F)),
+                  ("d_w", d_w, i8, (E, H, F)), ("d_s", d_s, f32, (E, H)), ("out", out, dt, (T, H)))
+    if workspace is None:
+        workspace = moe_layer_workspace(top_k, F, dev)
+    _call_on(dev, "s8b_moe_layer", *p, T, H, F, E, int(top_k), int(norm_topk_prob), float(scaling),
+             *_workspace("moe_layer", dev, workspace), dtype_code(dt))
     return out
 
 
