@@ -32,6 +32,8 @@ namespace ml {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxT = 16, kMaxE = 256, kMaxK = 16, kMaxA = kMaxT * kMaxK;
 constexpr int kMaxH = 8192;
+constexpr int kCols = 8;  // columns of one expert that a warp computes together
+constexpr int kSmem = 208 * 1024;  // row codes and contributions
 constexpr size_t kOffBar = 64, kHeader = 256;  // workspace: status word, barrier counter
 constexpr size_t kLogits = kHeader;            // fp32 [T][E]
 constexpr size_t kAct = kLogits + sizeof(float) * kMaxT * kMaxE;  // fp32 [A][F]
@@ -95,23 +97,23 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 
 // W weight rows of `bytes` bytes at w[i] against rows x[r] (shared memory, `pitch` bytes apart):
-// sums[i][r] for R rows, complete in every lane. Chunks of 16 bytes, lane by lane, 4 at a time.
-template <int W, int R>
+// sums[i][r] for R rows, complete in every lane. Chunks of 16 bytes, lane by lane, U at a time.
+template <int W, int R, int U>
 __device__ __forceinline__ void dot_rows(const int8_t *const (&w)[W], const int8_t *const (&x)[R],
                                          int bytes, int lane, int (&sums)[W][R]) {
 #pragma unroll
   for (int i = 0; i < W; ++i)
 #pragma unroll
     for (int r = 0; r < R; ++r) sums[i][r] = 0;
-  for (int c0 = 16 * lane; c0 < bytes; c0 += 4 * 512) {
-    int4 v[W][4];
+  for (int c0 = 16 * lane; c0 < bytes; c0 += U * 512) {
+    int4 v[W][U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < W; ++i)
         v[i][u] = c0 + 512 * u < bytes ? ld_stream(w[i] + c0 + 512 * u) : make_int4(0, 0, 0, 0);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (c0 + 512 * u >= bytes) break;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -132,8 +134,9 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   using namespace ml;
   extern __shared__ __align__(16) int8_t rows_s[];  // x codes [T][H], later act codes [A][F]
   __shared__ float topw[kMaxA], scale_s[kMaxA];     // by assignment / by sorted row
-  __shared__ int topi[kMaxA], order[kMaxA];         // expert; sorted row -> assignment t k + j
-  __shared__ int place[kMaxA];                      // assignment -> sorted row
+  __shared__ int topi[kMaxA], order[kMaxA];         // expert; sorted row -> token
+  __shared__ int place[kMaxA];                      // token's rows in ascending order
+  __shared__ float weight[kMaxA], xs_s[kMaxT];      // and their weights; rows' scales
   __shared__ uint32_t members[kMaxE];               // rows of each expert, a bit each
   __shared__ int expert[kMaxA], offset[kMaxA + 1];  // chosen experts ascending; their first row
   __shared__ int n_experts, ok_s;
@@ -173,6 +176,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
     }
   }
   for (int i = threadIdx.x; i < E; i += kThreads) members[i] = 0u;
+  if (threadIdx.x < T_) xs_s[threadIdx.x] = a.xs[threadIdx.x];
   if (!grid_barrier(a.ws, &ok_s)) return;
 
   // ---- B: each row's experts, then their gate_up and SwiGLU ----
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
     uint32_t left = 0;  // this lane's experts that are still to be had
 #pragma unroll
     for (int c = 0; c < kC; ++c) left |= (lane + 32 * c < E ? 1u : 0u) << c;
-    float total = 0.0f, mine = 0.0f;  // lane j keeps the j-th choice
+    float mine = -INFINITY;  // lane j keeps the j-th choice: its logit and expert
     int mine_e = 0;
     for (int r = 0; r < k; ++r) {  // the largest logit left, the lowest index among equals
       uint32_t bk = 0;
@@ -209,18 +213,21 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
           be = lane + 32 * c;
           bl = l[c];
         }
-      const uint32_t best = __reduce_max_sync(0xffffffffu, be == 0x7fffffff ? 0u : bk);
+      const uint32_t best = __reduce_max_sync(0xffffffffu, bk);
       const int e = __reduce_min_sync(0xffffffffu, bk == best ? be : 0x7fffffff);
       if (be == e) left &= ~(1u << (e >> 5));
-      const float p = __expf(__shfl_sync(0xffffffffu, bl, e & 31) - m) / s;
-      total += p;
+      const float pick = __shfl_sync(0xffffffffu, bl, e & 31);
       if (lane == r) {
-        mine = p;
+        mine = pick;
         mine_e = e;
       }
     }
+    const float p = lane < k ? __expf(mine - m) / s : 0.0f;
+    float total = p;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);  // k <= 16
     if (lane < k) {
-      topw[warp * k + lane] = (a.norm ? mine / fmaxf(total, 1e-9f) : mine) * a.scaling;
+      topw[warp * k + lane] = (a.norm ? p / fmaxf(total, 1e-9f) : p) * a.scaling;
       topi[warp * k + lane] = mine_e;
       atomicOr(&members[mine_e], 1u << warp);
     }
@@ -256,8 +263,11 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   for (int i = threadIdx.x; i < A; i += kThreads) {
     const int e = topi[i], t = i / k;
     const int p = offset[slot_of[e]] + __popc(members[e] & ((1u << t) - 1u));
-    order[p] = i;
-    place[i] = p;
+    order[p] = t;
+    int rank = 0;  // among the token's experts
+    for (int q = 0; q < k; ++q) rank += topi[t * k + q] < e;
+    place[t * k + rank] = p;
+    weight[t * k + rank] = topw[i];
   }
   // this CTA's output columns, and their down weights on the way to L2
   const int h0 = static_cast<int>(static_cast<long long>(blockIdx.x) * H / gridDim.x);
@@ -265,6 +275,8 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   if (nh > 0)
     for (int i = threadIdx.x; i < n_ex; i += kThreads) {
       const int8_t *p = a.d_w + (static_cast<size_t>(expert[i]) * H + h0) * F;
+      // (reading them by bulk copies into shared memory instead was slower: a copy costs an SM
+      // some 125 cycles, and a warp's share of an expert is too short for it)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(nh * F) : "memory");
     }
   __syncthreads();
@@ -280,22 +292,25 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
       const int8_t *w[4] = {a.gu_w + (base + f) * H, a.gu_w + (base + F + f) * H,
                             a.gu_w + (base + f1) * H, a.gu_w + (base + F + f1) * H};
       const int lo = offset[at], hi = offset[at + 1];
+      // lane 2 i + r finishes pair i, row r; its scales come with the weights
+      const int i = lane >> 1 & 1, r = lane & 1;
+      float sg = 0.0f, su = 0.0f;
+      if (lane < 4) {
+        sg = a.gu_s[base + (i ? f1 : f)];
+        su = a.gu_s[base + F + (i ? f1 : f)];
+      }
       for (int p0 = lo; p0 < hi; p0 += 2) {
         const int pl = min(p0 + 1, hi - 1);
-        const int ta = order[p0] / k, tb = order[pl] / k;
-        const int8_t *x[2] = {rows_s + ta * H, rows_s + tb * H};
+        const int8_t *x[2] = {rows_s + order[p0] * H, rows_s + order[pl] * H};
         int sum[4][2];
-        dot_rows<4, 2>(w, x, H, lane, sum);
-        // lane 2 i + r: pair i, row r
-        const int i = lane >> 1 & 1, r = lane & 1;
+        dot_rows<4, 2, 4>(w, x, H, lane, sum);
         if (lane < 4 && (i == 0 || two) && (r == 0 || pl != p0)) {
-          const float sx = a.xs[r ? tb : ta];
-          const int ff = f + i;
+          const float sx = xs_s[order[p0 + r]];
           const int gs = i ? (r ? sum[2][1] : sum[2][0]) : (r ? sum[0][1] : sum[0][0]);
           const int us = i ? (r ? sum[3][1] : sum[3][0]) : (r ? sum[1][1] : sum[1][0]);
-          const float g = static_cast<float>(gs) * sx * a.gu_s[base + ff];
-          const float v = static_cast<float>(us) * sx * a.gu_s[base + F + ff];
-          act[static_cast<size_t>(p0 + r) * F + ff] = g / (1.0f + __expf(-g)) * v;
+          const float g = static_cast<float>(gs) * sx * sg;
+          const float v = static_cast<float>(us) * sx * su;
+          act[static_cast<size_t>(p0 + r) * F + f + i] = g / (1.0f + __expf(-g)) * v;
         }
       }
       u += 1 + two;
@@ -307,78 +322,73 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   if (nh == 0) return;
   for (int p = warp; p < A; p += kWarps) {
     const float *src = act + static_cast<size_t>(p) * F;
-    float4 v[4];
+    constexpr int kHold = 8;  // vectors of a row that stay in registers (1024 values)
+    float4 v[kHold];
+#pragma unroll
+    for (int u = 0; u < kHold; ++u)
+      v[u] = 4 * lane + 128 * u < F
+                 ? __ldcg(reinterpret_cast<const float4 *>(src + 4 * lane + 128 * u))
+                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto top = [](float4 x) {
+      return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    };
     float mx = 0.0f;
-    for (int i0 = 4 * lane; i0 < F; i0 += 512) {  // 4 vectors in flight
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        v[u] = i0 + 128 * u < F ? __ldcg(reinterpret_cast<const float4 *>(src + i0 + 128 * u))
-                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
-    }
+    for (int u = 0; u < kHold; ++u) mx = fmaxf(mx, top(v[u]));
+    for (int i = 4 * lane + 128 * kHold; i < F; i += 128)
+      mx = fmaxf(mx, top(__ldcg(reinterpret_cast<const float4 *>(src + i))));
     mx = warp_max(mx);
     const QParams q = qparams(mx, 127.0f);
-    for (int i0 = 4 * lane; i0 < F; i0 += 512) {
+    auto put = [&](int i, float4 x) {
+      char4 c;
+      c.x = static_cast<signed char>(qcode(x.x, q.inv, 127));
+      c.y = static_cast<signed char>(qcode(x.y, q.inv, 127));
+      c.z = static_cast<signed char>(qcode(x.z, q.inv, 127));
+      c.w = static_cast<signed char>(qcode(x.w, q.inv, 127));
+      *reinterpret_cast<char4 *>(rows_s + static_cast<size_t>(p) * F + i) = c;
+    };
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + 128 * u;
-        if (i >= F) break;
-        if (F > 512) v[u] = __ldcg(reinterpret_cast<const float4 *>(src + i));
-        char4 c;
-        c.x = static_cast<signed char>(qcode(v[u].x, q.inv, 127));
-        c.y = static_cast<signed char>(qcode(v[u].y, q.inv, 127));
-        c.z = static_cast<signed char>(qcode(v[u].z, q.inv, 127));
-        c.w = static_cast<signed char>(qcode(v[u].w, q.inv, 127));
-        *reinterpret_cast<char4 *>(rows_s + static_cast<size_t>(p) * F + i) = c;
-      }
-    }
+    for (int u = 0; u < kHold; ++u)
+      if (4 * lane + 128 * u < F) put(4 * lane + 128 * u, v[u]);
+    for (int i = 4 * lane + 128 * kHold; i < F; i += 128)
+      put(i, __ldcg(reinterpret_cast<const float4 *>(src + i)));
     if (lane == 0) scale_s[p] = q.scale;
   }
   __syncthreads();
   {
-    const int per = (nh + 3) / 4, units = n_ex * per;  // four columns of one expert at a time
+    // eight columns of one expert at a time: they come from L2, whose latency needs the loads
+    const int per = (nh + kCols - 1) / kCols, units = n_ex * per;
     for (int u = warp; u < units; u += kWarps) {
-      const int at = u / per, c0 = 4 * (u - at * per);
+      const int at = u / per, c0 = kCols * (u - at * per);
       const size_t row = static_cast<size_t>(expert[at]) * H + h0;
-      const int8_t *w[4];
+      const int8_t *w[kCols];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = a.d_w + (row + min(c0 + i, nh - 1)) * F;
+      for (int i = 0; i < kCols; ++i) w[i] = a.d_w + (row + min(c0 + i, nh - 1)) * F;
+      const int i = lane >> 1, r = lane & 1;  // lane 2 i + r finishes column i, row r
+      const float sd = i < kCols && c0 + i < nh ? a.d_s[row + c0 + i] : 0.0f;
       const int lo = offset[at], hi = offset[at + 1];
       for (int p0 = lo; p0 < hi; p0 += 2) {
         const int pl = min(p0 + 1, hi - 1);
         const int8_t *x[2] = {rows_s + static_cast<size_t>(p0) * F,
                               rows_s + static_cast<size_t>(pl) * F};
-        int sum[4][2];
-        dot_rows<4, 2>(w, x, F, lane, sum);
-        const int i = lane >> 1, r = lane & 1;
-        if (lane < 8 && c0 + i < nh && (r == 0 || pl != p0)) {
-          int v = 0;
+        int sum[kCols][2];
+        dot_rows<kCols, 2, 2>(w, x, F, lane, sum);
+        int v = 0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q == i) v = r ? sum[q][1] : sum[q][0];
-          contrib[(p0 + r) * a.slice + c0 + i] = static_cast<float>(v) * scale_s[p0 + r] * a.d_s[row + c0 + i];
-        }
+        for (int q = 0; q < kCols; ++q)
+          if (q == i) v = r ? sum[q][1] : sum[q][0];
+        if (i < kCols && c0 + i < nh && (r == 0 || pl != p0))
+          contrib[(p0 + r) * a.slice + c0 + i] = static_cast<float>(v) * scale_s[p0 + r] * sd;
       }
     }
   }
   __syncthreads();
-  // the rows of a token, in ascending order of their sorted rows, that is of their experts
+  // a token's rows in ascending order, that is of their experts
   T *out = static_cast<T *>(a.out);
   for (int i = threadIdx.x; i < T_ * nh; i += kThreads) {
     const int t = i / nh, c = i - t * nh;
     float s = 0.0f;
-    int last = -1;
-    for (int j = 0; j < k; ++j) {
-      int next = 0x7fffffff, at = 0;
-      for (int q = 0; q < k; ++q) {
-        const int p = place[t * k + q];
-        if (p > last && p < next) next = p, at = q;
-      }
-      s = fmaf(topw[t * k + at], contrib[next * a.slice + c], s);
-      last = next;
-    }
+    for (int j = 0; j < k; ++j) s = fmaf(weight[t * k + j], contrib[place[t * k + j] * a.slice + c], s);
     out[static_cast<size_t>(t) * H + h0 + c] = from_f32<T>(s);
   }
 }
@@ -397,7 +407,8 @@ extern "C" int s8b_moe_layer_max_rows(int H, int F, int top_k) {
   using namespace ml;
   if (H <= 0 || F <= 0 || top_k <= 0 || top_k > kMaxK || H % 16 || F % 16 || H > kMaxH) return 0;
   const long long row = H > static_cast<long long>(top_k) * F ? H : static_cast<long long>(top_k) * F;
-  const long long n = (150ll << 10) / row;  // codes in shared memory
+  const long long per = row + 4ll * top_k * ((H + 127) / 128);  // its codes, and contributions
+  const long long n = (kSmem - 256) / per;                      // (a CTA's columns: fewer)
   return static_cast<int>(n < kMaxT ? n : kMaxT);
 }
 
@@ -444,7 +455,7 @@ extern "C" int s8b_moe_layer(const void *y, const int8_t *xq, const float *xs, c
   a.code_bytes = static_cast<int>((row * T_ + 15) / 16 * 16);
   a.slice = (H + sms - 1) / sms;
   const size_t smem = a.code_bytes + sizeof(float) * T_ * top_k * static_cast<size_t>(a.slice);
-  if (smem > 215 * 1024) return S8B_ERR_SHAPE;
+  if (smem > kSmem) return S8B_ERR_SHAPE;
   S8B_DISPATCH_DTYPE(dtype, TT, {
     ensure_smem(reinterpret_cast<const void *>(moe_layer_kernel<TT>), smem);
     cudaLaunchConfig_t cfg = {};

@@ -100,6 +100,7 @@ def test_moe_layer_refusals(lib, kw, code):
 def test_moe_layer_rows():
     assert ops.moe_layer_max_rows(2048, 768, 8) == 16
     assert ops.moe_layer_max_rows(256, 16384, 8) == 1  # codes of one row of eight experts
+    assert 0 < ops.moe_layer_max_rows(8192, 1024, 16) < 16
     assert ops.moe_layer_max_rows(256, 16384, 16) == 0
     assert ops.moe_layer_max_rows(100, 128, 2) == 0
     with pytest.raises(RuntimeError, match="CUDA tensor"):
