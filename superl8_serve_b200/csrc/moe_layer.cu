@@ -6,7 +6,7 @@
 // for one row of a 2048 x 768 x 8 layer, 5.8 us at the measured copy rate), and the seven launches of
 // the general path cost more than that. Here one cooperative launch of one CTA per SM runs
 // three phases with a grid barrier between them:
-//   A  logits: expert e's gate row against every row, a warp per row (float64 sums);
+//   A  logits: expert e's gate row against every row, all warps (float64 sums);
 //   B  every CTA finds all rows' experts by itself (a warp per row, 8 rounds of a warp-wide
 //      maximum), and the (chosen expert, f) pairs, gate row f and up row F + f each, are cut
 //      evenly over all warps of the grid; act = silu(g) u goes to the workspace in binary32;
@@ -21,6 +21,7 @@
 // else is binary32, rounded to the activation dtype once, at the end. (The general path rounds
 // to dtype after gate_up, silu, the product, down, the weighting and each addition.)
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -129,6 +130,61 @@ __device__ __forceinline__ void dot_rows(const int8_t *const (&w)[W], const int8
     for (int r = 0; r < R; ++r) sums[i][r] = __reduce_add_sync(0xffffffffu, sums[i][r]);
 }
 
+// Row `warp`'s experts and weights from its logits: lane c holds experts c, c + 32, ..
+template <int kC>
+__device__ __forceinline__ void choose(const MoeArgs &a, const float *row, int warp, int lane,
+                                       int *topi, float *topw, uint32_t *members) {
+  const int E = a.E, k = a.k;
+  uint32_t key[kC];
+  float l[kC], m = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const int e = lane + 32 * c;
+    l[c] = e < E ? __ldcg(row + e) : -INFINITY;
+    key[c] = order_key(l[c]);
+    m = fmaxf(m, l[c]);
+  }
+  m = warp_max_redux(m);
+  float s = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) s += lane + 32 * c < E ? __expf(l[c] - m) : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  uint32_t left = 0;  // this lane's experts that are still to be had
+#pragma unroll
+  for (int c = 0; c < kC; ++c) left |= (lane + 32 * c < E ? 1u : 0u) << c;
+  int mine = 0;  // lane j keeps the j-th choice
+  for (int r = 0; r < k; ++r) {  // the largest logit left, the lowest index among equals
+    uint32_t bk = 0;
+    int be = 0x7fffffff;
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      if ((left >> c & 1u) && (key[c] > bk || be == 0x7fffffff)) {
+        bk = key[c];
+        be = lane + 32 * c;
+      }
+    const uint32_t best = __reduce_max_sync(0xffffffffu, bk);
+    const int e = __reduce_min_sync(0xffffffffu, bk == best ? be : 0x7fffffff);
+    if (be == e) left &= ~(1u << (e >> 5));
+    if (lane == r) mine = e;
+  }
+  float pick = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const float v = __shfl_sync(0xffffffffu, l[c], mine & 31);
+    if (mine >> 5 == c) pick = v;
+  }
+  const float p = lane < k ? __expf(pick - m) / s : 0.0f;
+  float total = p;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);  // k <= 16
+  if (lane < k) {
+    topw[warp * k + lane] = (a.norm ? p / fmaxf(total, 1e-9f) : p) * a.scaling;
+    topi[warp * k + lane] = mine;
+    atomicOr(&members[mine], 1u << warp);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArgs a) {
   using namespace ml;
@@ -140,6 +196,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   __shared__ uint32_t members[kMaxE];               // rows of each expert, a bit each
   __shared__ int expert[kMaxA], offset[kMaxA + 1];  // chosen experts ascending; their first row
   __shared__ int n_experts, ok_s;
+  __shared__ double part_s[kWarps];
   __shared__ uint8_t slot_of[kMaxE];  // its place among the chosen experts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int T_ = a.T, H = a.H, F = a.F, E = a.E, k = a.k, A = T_ * k;
@@ -150,13 +207,15 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   // ---- A: logits ----
   for (int i = 16 * threadIdx.x; i < T_ * H; i += 16 * kThreads)
     *reinterpret_cast<int4 *>(rows_s + i) = *reinterpret_cast<const int4 *>(a.xq + i);
-  if (warp < T_) {
-    const T *yr = static_cast<const T *>(a.y) + static_cast<size_t>(warp) * H;
+  {
+    const int per = T_ > 8 ? 1 : T_ > 4 ? 2 : T_ > 2 ? 4 : T_ > 1 ? 8 : 16;  // warps of a row
+    const int row = warp / per, part = warp - row * per;
+    const T *yr = static_cast<const T *>(a.y) + static_cast<size_t>(min(row, T_ - 1)) * H;
     for (int e = blockIdx.x; e < E; e += gridDim.x) {
       const float *g = a.gate + static_cast<size_t>(e) * H;
       double s0 = 0.0, s1 = 0.0;
 #pragma unroll 4
-      for (int i = 8 * lane; i < H; i += 256) {
+      for (int i = 8 * (32 * part + lane); i < H; i += 256 * per) {
         const uint4 raw = *reinterpret_cast<const uint4 *>(yr + i);
         const float4 g0 = *reinterpret_cast<const float4 *>(g + i);
         const float4 g1 = *reinterpret_cast<const float4 *>(g + i + 4);
@@ -172,7 +231,14 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
         s1 = fma(static_cast<double>(to_f32(v[7])), static_cast<double>(g1.w), s1);
       }
       const double s = warp_sum_d(s0 + s1);
-      if (lane == 0) logits[warp * E + e] = static_cast<float>(s);
+      if (lane == 0) part_s[warp] = s;
+      __syncthreads();
+      if (threadIdx.x < T_) {
+        double sum = 0.0;
+        for (int q = 0; q < per; ++q) sum += part_s[threadIdx.x * per + q];
+        logits[threadIdx.x * E + e] = static_cast<float>(sum);
+      }
+      __syncthreads();
     }
   }
   for (int i = threadIdx.x; i < E; i += kThreads) members[i] = 0u;
@@ -181,56 +247,8 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
 
   // ---- B: each row's experts, then their gate_up and SwiGLU ----
   if (warp < T_) {
-    constexpr int kC = kMaxE / 32;
-    uint32_t key[kC];
-    float l[kC], m = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      const int e = lane + 32 * c;
-      l[c] = e < E ? __ldcg(logits + warp * E + e) : -INFINITY;
-      key[c] = order_key(l[c]);
-      m = fmaxf(m, l[c]);
-    }
-    m = warp_max(m);
-    float s = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) s += lane + 32 * c < E ? __expf(l[c] - m) : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    uint32_t left = 0;  // this lane's experts that are still to be had
-#pragma unroll
-    for (int c = 0; c < kC; ++c) left |= (lane + 32 * c < E ? 1u : 0u) << c;
-    float mine = -INFINITY;  // lane j keeps the j-th choice: its logit and expert
-    int mine_e = 0;
-    for (int r = 0; r < k; ++r) {  // the largest logit left, the lowest index among equals
-      uint32_t bk = 0;
-      int be = 0x7fffffff;
-      float bl = 0.0f;
-#pragma unroll
-      for (int c = 0; c < kC; ++c)
-        if ((left >> c & 1u) && (key[c] > bk || be == 0x7fffffff)) {
-          bk = key[c];
-          be = lane + 32 * c;
-          bl = l[c];
-        }
-      const uint32_t best = __reduce_max_sync(0xffffffffu, bk);
-      const int e = __reduce_min_sync(0xffffffffu, bk == best ? be : 0x7fffffff);
-      if (be == e) left &= ~(1u << (e >> 5));
-      const float pick = __shfl_sync(0xffffffffu, bl, e & 31);
-      if (lane == r) {
-        mine = pick;
-        mine_e = e;
-      }
-    }
-    const float p = lane < k ? __expf(mine - m) / s : 0.0f;
-    float total = p;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);  // k <= 16
-    if (lane < k) {
-      topw[warp * k + lane] = (a.norm ? p / fmaxf(total, 1e-9f) : p) * a.scaling;
-      topi[warp * k + lane] = mine_e;
-      atomicOr(&members[mine_e], 1u << warp);
-    }
+    if (E <= 128) choose<4>(a, logits + warp * E, warp, lane, topi, topw, members);
+    else choose<kMaxE / 32>(a, logits + warp * E, warp, lane, topi, topw, members);
   }
   __syncthreads();
   if (warp == 0) {  // chosen experts in ascending order, and where their rows begin
@@ -292,27 +310,38 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
       const int8_t *w[4] = {a.gu_w + (base + f) * H, a.gu_w + (base + F + f) * H,
                             a.gu_w + (base + f1) * H, a.gu_w + (base + F + f1) * H};
       const int lo = offset[at], hi = offset[at + 1];
-      // lane 2 i + r finishes pair i, row r; its scales come with the weights
-      const int i = lane >> 1 & 1, r = lane & 1;
+      // lane 4 i + r finishes pair i, row r; its scales come with the weights
+      const int i = lane >> 2 & 1, r = lane & 3;
       float sg = 0.0f, su = 0.0f;
-      if (lane < 4) {
+      if (lane < 8) {
         sg = a.gu_s[base + (i ? f1 : f)];
         su = a.gu_s[base + F + (i ? f1 : f)];
       }
-      for (int p0 = lo; p0 < hi; p0 += 2) {
-        const int pl = min(p0 + 1, hi - 1);
-        const int8_t *x[2] = {rows_s + order[p0] * H, rows_s + order[pl] * H};
-        int sum[4][2];
-        dot_rows<4, 2, 4>(w, x, H, lane, sum);
-        if (lane < 4 && (i == 0 || two) && (r == 0 || pl != p0)) {
+      auto rows = [&](auto n, int p0) {  // n of the expert's rows, from p0 on
+        constexpr int R = decltype(n)::value;
+        const int8_t *x[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) x[q] = rows_s + order[min(p0 + q, hi - 1)] * H;
+        int sum[4][R];
+        dot_rows<4, R, 4>(w, x, H, lane, sum);
+        int gs = 0, us = 0;
+#pragma unroll
+        for (int q = 0; q < R; ++q)
+          if (q == r) {
+            gs = i ? sum[2][q] : sum[0][q];
+            us = i ? sum[3][q] : sum[1][q];
+          }
+        if (r < R && p0 + r < hi && lane < 8 && (i == 0 || two)) {
           const float sx = xs_s[order[p0 + r]];
-          const int gs = i ? (r ? sum[2][1] : sum[2][0]) : (r ? sum[0][1] : sum[0][0]);
-          const int us = i ? (r ? sum[3][1] : sum[3][0]) : (r ? sum[1][1] : sum[1][0]);
           const float g = static_cast<float>(gs) * sx * sg;
           const float v = static_cast<float>(us) * sx * su;
           act[static_cast<size_t>(p0 + r) * F + f + i] = g / (1.0f + __expf(-g)) * v;
         }
-      }
+      };
+      if (hi - lo == 1) rows(std::integral_constant<int, 1>{}, lo);
+      else if (hi - lo == 2) rows(std::integral_constant<int, 2>{}, lo);
+      else
+        for (int p0 = lo; p0 < hi; p0 += 4) rows(std::integral_constant<int, 4>{}, p0);
       u += 1 + two;
     }
   }
@@ -364,22 +393,29 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
       const int8_t *w[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) w[i] = a.d_w + (row + min(c0 + i, nh - 1)) * F;
-      const int i = lane >> 1, r = lane & 1;  // lane 2 i + r finishes column i, row r
-      const float sd = i < kCols && c0 + i < nh ? a.d_s[row + c0 + i] : 0.0f;
+      const int i = lane >> 2, r = lane & 3;  // lane 4 i + r finishes column i, row r
+      const float sd = c0 + i < nh ? a.d_s[row + c0 + i] : 0.0f;
       const int lo = offset[at], hi = offset[at + 1];
-      for (int p0 = lo; p0 < hi; p0 += 2) {
-        const int pl = min(p0 + 1, hi - 1);
-        const int8_t *x[2] = {rows_s + static_cast<size_t>(p0) * F,
-                              rows_s + static_cast<size_t>(pl) * F};
-        int sum[kCols][2];
-        dot_rows<kCols, 2, 2>(w, x, F, lane, sum);
+      auto rows = [&](auto n, int p0) {
+        constexpr int R = decltype(n)::value;
+        const int8_t *x[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) x[q] = rows_s + static_cast<size_t>(min(p0 + q, hi - 1)) * F;
+        int sum[kCols][R];
+        dot_rows<kCols, R, 2>(w, x, F, lane, sum);
         int v = 0;
 #pragma unroll
-        for (int q = 0; q < kCols; ++q)
-          if (q == i) v = r ? sum[q][1] : sum[q][0];
-        if (i < kCols && c0 + i < nh && (r == 0 || pl != p0))
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int q = 0; q < R; ++q)
+            if (c == i && q == r) v = sum[c][q];
+        if (r < R && p0 + r < hi && c0 + i < nh)
           contrib[(p0 + r) * a.slice + c0 + i] = static_cast<float>(v) * scale_s[p0 + r] * sd;
-      }
+      };
+      if (hi - lo == 1) rows(std::integral_constant<int, 1>{}, lo);
+      else if (hi - lo == 2) rows(std::integral_constant<int, 2>{}, lo);
+      else
+        for (int p0 = lo; p0 < hi; p0 += 4) rows(std::integral_constant<int, 4>{}, p0);
     }
   }
   __syncthreads();
