@@ -9,11 +9,10 @@
 //   A  logits: expert e's gate row against every row, all warps (float64 sums);
 //   B  every CTA finds all rows' experts by itself (a warp per row, 8 rounds of a warp-wide
 //      maximum), and the (chosen expert, f) pairs, gate row f and up row F + f each, are cut
-//      evenly over all warps of the grid; act = silu(g) u goes to the workspace in binary32;
+//      by cost over all warps of the grid; act = silu(g) u goes to the workspace in binary32;
 //   C  every CTA quantizes the act rows and computes its slice of output columns over all
 //      chosen experts, so the weighted sum needs no third barrier and no atomics.
-// The down weights that a CTA will read are asked into L2 as soon as the experts are known, so
-// HBM streams through the barrier. Products are dp4a on CUDA cores: an expert has one or two rows
+// Products are dp4a on CUDA cores: an expert has one or two rows
 // here, where the stream of weights, not arithmetic, sets the time, and an MMA tile would be
 // empty. Sums over experts are in ascending expert order: the result does not depend on timing.
 //
@@ -91,6 +90,10 @@ __device__ __forceinline__ int4 ld_stream(const int8_t *p) {  // weights: read o
                : "l"(p));
   return v;
 }
+// What a pair of an expert with `rows` rows costs: mostly its weights, which come once, and a
+// little for each row (with equal shares a CTA whose expert had 6 of 16 rows took 15,000 cycles
+// where most took 6,400).
+__device__ __forceinline__ int pair_cost(int rows) { return 8 + rows; }
 // order of logits as unsigned integers; NaN lowest
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -196,7 +199,8 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   __shared__ uint32_t members[kMaxE];               // rows of each expert, a bit each
   __shared__ int expert[kMaxA], offset[kMaxA + 1];  // chosen experts ascending; their first row
   __shared__ int n_experts, ok_s;
-  __shared__ double part_s[kWarps];
+  __shared__ double part_s[kWarps][kMaxT];
+  __shared__ int before[kMaxA + 1];    // cost of a pair of every chosen expert before
   __shared__ uint8_t slot_of[kMaxE];  // its place among the chosen experts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int T_ = a.T, H = a.H, F = a.F, E = a.E, k = a.k, A = T_ * k;
@@ -207,39 +211,48 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   // ---- A: logits ----
   for (int i = 16 * threadIdx.x; i < T_ * H; i += 16 * kThreads)
     *reinterpret_cast<int4 *>(rows_s + i) = *reinterpret_cast<const int4 *>(a.xq + i);
-  {
-    const int per = T_ > 8 ? 1 : T_ > 4 ? 2 : T_ > 2 ? 4 : T_ > 1 ? 8 : 16;  // warps of a row
-    const int row = warp / per, part = warp - row * per;
-    const T *yr = static_cast<const T *>(a.y) + static_cast<size_t>(min(row, T_ - 1)) * H;
-    for (int e = blockIdx.x; e < E; e += gridDim.x) {
-      const float *g = a.gate + static_cast<size_t>(e) * H;
-      double s0 = 0.0, s1 = 0.0;
+  // A thread keeps 8 gate values at a time (in float64 once for all rows); a row's products add
+  // up over the warp's lanes, then over the warps.
+  // (Few experts: several CTAs share an expert's rows.)
+  const int groups = max(1, min(T_, static_cast<int>(gridDim.x) / E));
+  for (int unit = blockIdx.x; unit < E * groups; unit += gridDim.x) {
+    const int e = unit % E, grp = unit / E;
+    const int ta = grp * T_ / groups, tb = (grp + 1) * T_ / groups;
+    const float *g = a.gate + static_cast<size_t>(e) * H;
+    double mine = 0.0;  // lane t: row t's sum over this warp's columns
+    for (int i0 = 256 * warp; i0 < H; i0 += 256 * kWarps) {
+      const int i = i0 + 8 * lane;
+      double gd[8];
+      float4 g0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), g1 = g0;
+      if (i < H) {
+        g0 = *reinterpret_cast<const float4 *>(g + i);
+        g1 = *reinterpret_cast<const float4 *>(g + i + 4);
+      }
+      gd[0] = g0.x, gd[1] = g0.y, gd[2] = g0.z, gd[3] = g0.w;
+      gd[4] = g1.x, gd[5] = g1.y, gd[6] = g1.z, gd[7] = g1.w;
 #pragma unroll 4
-      for (int i = 8 * (32 * part + lane); i < H; i += 256 * per) {
-        const uint4 raw = *reinterpret_cast<const uint4 *>(yr + i);
-        const float4 g0 = *reinterpret_cast<const float4 *>(g + i);
-        const float4 g1 = *reinterpret_cast<const float4 *>(g + i + 4);
+      for (int t = ta; t < tb; ++t) {
         T v[8];
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        if (i < H)
+          raw = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.y) +
+                                                 static_cast<size_t>(t) * H + i);
         memcpy(v, &raw, 16);
-        s0 = fma(static_cast<double>(to_f32(v[0])), static_cast<double>(g0.x), s0);
-        s1 = fma(static_cast<double>(to_f32(v[1])), static_cast<double>(g0.y), s1);
-        s0 = fma(static_cast<double>(to_f32(v[2])), static_cast<double>(g0.z), s0);
-        s1 = fma(static_cast<double>(to_f32(v[3])), static_cast<double>(g0.w), s1);
-        s0 = fma(static_cast<double>(to_f32(v[4])), static_cast<double>(g1.x), s0);
-        s1 = fma(static_cast<double>(to_f32(v[5])), static_cast<double>(g1.y), s1);
-        s0 = fma(static_cast<double>(to_f32(v[6])), static_cast<double>(g1.z), s0);
-        s1 = fma(static_cast<double>(to_f32(v[7])), static_cast<double>(g1.w), s1);
+        double s = 0.0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s = fma(static_cast<double>(to_f32(v[q])), gd[q], s);
+        s = warp_sum_d(s);
+        if (lane == t) mine += s;
       }
-      const double s = warp_sum_d(s0 + s1);
-      if (lane == 0) part_s[warp] = s;
-      __syncthreads();
-      if (threadIdx.x < T_) {
-        double sum = 0.0;
-        for (int q = 0; q < per; ++q) sum += part_s[threadIdx.x * per + q];
-        logits[threadIdx.x * E + e] = static_cast<float>(sum);
-      }
-      __syncthreads();
     }
+    if (lane < T_) part_s[warp][lane] = mine;
+    __syncthreads();
+    if (threadIdx.x >= ta && threadIdx.x < tb) {
+      double sum = 0.0;
+      for (int q = 0; q < kWarps; ++q) sum += part_s[q][threadIdx.x];
+      logits[threadIdx.x * E + e] = static_cast<float>(sum);
+    }
+    __syncthreads();
   }
   for (int i = threadIdx.x; i < E; i += kThreads) members[i] = 0u;
   if (threadIdx.x < T_) xs_s[threadIdx.x] = a.xs[threadIdx.x];
@@ -252,27 +265,33 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   }
   __syncthreads();
   if (warp == 0) {  // chosen experts in ascending order, and where their rows begin
-    int n = 0, rows = 0;
+    int n = 0, rows = 0, cost = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const uint32_t who = e0 + lane < E ? members[e0 + lane] : 0u;
       const uint32_t hit = __ballot_sync(0xffffffffu, who != 0u);
-      int c = __popc(who), inc = c;
+      // rows before, and the cost of a pair before (see pair_cost), in one scan
+      const int c = __popc(who);
+      uint32_t own = who ? c | static_cast<uint32_t>(pair_cost(c)) << 16 : 0u, inc = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += u;
       }
       if (who) {
         const int at = n + __popc(hit & ((1u << lane) - 1u));
         expert[at] = e0 + lane;
         slot_of[e0 + lane] = static_cast<uint8_t>(at);
-        offset[at] = rows + inc - c;
+        offset[at] = rows + ((inc - own) & 0xffffu);
+        before[at] = cost + ((inc - own) >> 16);
       }
       n += __popc(hit);
-      rows += __shfl_sync(0xffffffffu, inc, 31);
+      const uint32_t all = __shfl_sync(0xffffffffu, inc, 31);
+      rows += all & 0xffffu;
+      cost += all >> 16;
     }
     if (lane == 0) {
       offset[n] = rows;
+      before[n] = cost;
       n_experts = n;
     }
   }
@@ -287,22 +306,27 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
     place[t * k + rank] = p;
     weight[t * k + rank] = topw[i];
   }
-  // this CTA's output columns, and their down weights on the way to L2
+  // this CTA's output columns
   const int h0 = static_cast<int>(static_cast<long long>(blockIdx.x) * H / gridDim.x);
   const int nh = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * H / gridDim.x) - h0;
-  if (nh > 0)
-    for (int i = threadIdx.x; i < n_ex; i += kThreads) {
-      const int8_t *p = a.d_w + (static_cast<size_t>(expert[i]) * H + h0) * F;
-      // (reading them by bulk copies into shared memory instead was slower: a copy costs an SM
-      // some 125 cycles, and a warp's share of an expert is too short for it)
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(nh * F) : "memory");
-    }
   __syncthreads();
   {
-    const long long units = static_cast<long long>(n_ex) * F, wg = blockIdx.x * kWarps + warp;
-    const long long nw = static_cast<long long>(gridDim.x) * kWarps;
-    const int u1 = static_cast<int>((wg + 1) * units / nw);
-    for (int u = static_cast<int>(wg * units / nw); u < u1;) {
+    // This warp's pairs: cost c of the whole lies in pair (c - before F) / cost of its expert;
+    // lane 0 looks up where the warp's share begins, lane 1 where it ends.
+    const uint32_t total = static_cast<uint32_t>(before[n_ex]) * F, nw = gridDim.x * kWarps;
+    const uint32_t wg = blockIdx.x * kWarps + warp + (lane & 1);
+    const uint32_t c = wg * (total / nw) + wg * (total % nw) / nw;
+    int lo = 0, hi = n_ex;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (static_cast<uint32_t>(before[mid]) * F <= c) lo = mid;
+      else hi = mid;
+    }
+    const uint32_t per = before[lo + 1] - before[lo];
+    const int pair =
+        c >= total ? n_ex * F : lo * F + static_cast<int>((c - before[lo] * F + per - 1) / per);
+    const int u1 = __shfl_sync(0xffffffffu, pair, 1);
+    for (int u = __shfl_sync(0xffffffffu, pair, 0); u < u1;) {
       const int at = u / F, f = u - at * F;
       const int two = u + 1 < u1 && f + 1 < F;  // a second pair of the same expert
       const size_t base = static_cast<size_t>(expert[at]) * 2 * F;
@@ -349,39 +373,47 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
 
   // ---- C: act codes, then this CTA's columns of the down products ----
   if (nh == 0) return;
-  for (int p = warp; p < A; p += kWarps) {
-    const float *src = act + static_cast<size_t>(p) * F;
+  for (int p0 = warp; p0 < A; p0 += 2 * kWarps) {  // two rows at a time
     constexpr int kHold = 8;  // vectors of a row that stay in registers (1024 values)
-    float4 v[kHold];
+    float4 v[2][kHold];
 #pragma unroll
-    for (int u = 0; u < kHold; ++u)
-      v[u] = 4 * lane + 128 * u < F
-                 ? __ldcg(reinterpret_cast<const float4 *>(src + 4 * lane + 128 * u))
-                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < kHold; ++u) {
+        const int p = p0 + h * kWarps, i = 4 * lane + 128 * u;
+        v[h][u] = p < A && i < F
+                      ? __ldcg(reinterpret_cast<const float4 *>(act + static_cast<size_t>(p) * F + i))
+                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
     auto top = [](float4 x) {
       return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
     };
-    float mx = 0.0f;
 #pragma unroll
-    for (int u = 0; u < kHold; ++u) mx = fmaxf(mx, top(v[u]));
-    for (int i = 4 * lane + 128 * kHold; i < F; i += 128)
-      mx = fmaxf(mx, top(__ldcg(reinterpret_cast<const float4 *>(src + i))));
-    mx = warp_max(mx);
-    const QParams q = qparams(mx, 127.0f);
-    auto put = [&](int i, float4 x) {
-      char4 c;
-      c.x = static_cast<signed char>(qcode(x.x, q.inv, 127));
-      c.y = static_cast<signed char>(qcode(x.y, q.inv, 127));
-      c.z = static_cast<signed char>(qcode(x.z, q.inv, 127));
-      c.w = static_cast<signed char>(qcode(x.w, q.inv, 127));
-      *reinterpret_cast<char4 *>(rows_s + static_cast<size_t>(p) * F + i) = c;
-    };
+    for (int h = 0; h < 2; ++h) {
+      const int p = p0 + h * kWarps;
+      if (p >= A) break;
+      const float *src = act + static_cast<size_t>(p) * F;
+      float mx = 0.0f;
 #pragma unroll
-    for (int u = 0; u < kHold; ++u)
-      if (4 * lane + 128 * u < F) put(4 * lane + 128 * u, v[u]);
-    for (int i = 4 * lane + 128 * kHold; i < F; i += 128)
-      put(i, __ldcg(reinterpret_cast<const float4 *>(src + i)));
-    if (lane == 0) scale_s[p] = q.scale;
+      for (int u = 0; u < kHold; ++u) mx = fmaxf(mx, top(v[h][u]));
+      for (int i = 4 * lane + 128 * kHold; i < F; i += 128)
+        mx = fmaxf(mx, top(__ldcg(reinterpret_cast<const float4 *>(src + i))));
+      const QParams q = qparams(warp_max_redux(mx), 127.0f);
+      auto put = [&](int i, float4 x) {
+        char4 c;
+        c.x = static_cast<signed char>(qcode(x.x, q.inv, 127));
+        c.y = static_cast<signed char>(qcode(x.y, q.inv, 127));
+        c.z = static_cast<signed char>(qcode(x.z, q.inv, 127));
+        c.w = static_cast<signed char>(qcode(x.w, q.inv, 127));
+        *reinterpret_cast<char4 *>(rows_s + static_cast<size_t>(p) * F + i) = c;
+      };
+#pragma unroll
+      for (int u = 0; u < kHold; ++u)
+        if (4 * lane + 128 * u < F) put(4 * lane + 128 * u, v[h][u]);
+      for (int i = 4 * lane + 128 * kHold; i < F; i += 128)
+        put(i, __ldcg(reinterpret_cast<const float4 *>(src + i)));
+      if (lane == 0) scale_s[p] = q.scale;
+    }
   }
   __syncthreads();
   {
@@ -458,7 +490,8 @@ extern "C" int s8b_moe_layer(const void *y, const int8_t *xq, const float *xs, c
   if (dtype != S8B_BF16 && dtype != S8B_FP16) return S8B_ERR_DTYPE;
   if (T_ < 0 || E <= 0 || E > kMaxE || top_k <= 0 || top_k > E ||
       T_ > s8b_moe_layer_max_rows(H, F, top_k) ||
-      static_cast<long long>(E) * 2 * F * H > (1ll << 46))
+      // pairs' costs in 32 bits: at most 24 for each of top_k T experts' F pairs
+      static_cast<long long>(F) * top_k * T_ * 24 >= (1ll << 31))
     return S8B_ERR_SHAPE;
   if (!aligned(y, 16) || !aligned(xq, 16) || !aligned(gate, 16) || !aligned(gu_w, 16) ||
       !aligned(d_w, 16) || !aligned(xs, 4) || !aligned(gu_s, 4) || !aligned(d_s, 4) ||
