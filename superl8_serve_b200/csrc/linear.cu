@@ -45,6 +45,23 @@ __device__ __forceinline__ float apply_act(float v, int act) {
   return v;
 }
 
+// The same of N values, the choice made once for all of them.
+template <int N>
+__device__ __forceinline__ void apply_act(float (&v)[N], int act) {
+#define S8B_ACT_CASE(A)                                 \
+  case A:                                               \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = apply_act(v[i], A); \
+    break;
+  switch (act) {
+    S8B_ACT_CASE(kActSilu)
+    S8B_ACT_CASE(kActGelu)
+    S8B_ACT_CASE(kActGeluTanh)
+    S8B_ACT_CASE(kActRelu)
+    default: break;
+  }
+#undef S8B_ACT_CASE
+}
+
 struct LinArgs {
   const float *xs, *ws;
   const void *bias, *res;
@@ -83,7 +100,7 @@ __device__ __forceinline__ void tile_at(int t, const LinArgs &a, int *m0, int *n
   *n0 = n * NT;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool ACT>
 __global__ void __launch_bounds__(kLinThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_w, const LinArgs a) {
@@ -197,11 +214,26 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       const float sx = mrow + lane < a.M ? a.xs[mrow + lane] : 0.0f;
       const uint32_t acc = tmem + b * NT + half * kCols + (static_cast<uint32_t>(32 * quad) << 16);
       const int nbase = n0 + half * kCols;
+      // Columns of this warp that exist. While a chunk of 16 is finished from shared memory, the
+      // next one's sums are on their way from TMEM and its residual from global memory (loaded
+      // when needed, the residual cost 12 of 89 us at 4096 x 4096 x 4096).
+      const int cols = mrow < a.M ? min(kCols, a.N - nbase) : 0;
+      uint32_t v[16];
+      uint4 rnext[2] = {};
+      auto ask = [&](int c) {  // the residual of chunk c (vector rows)
+        const int n = nbase + c + 8 * (lane & 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int m = mrow + (lane >> 1) + 16 * i;
+          if (c < cols && n < a.N && m < a.M)
+            rnext[i] = *reinterpret_cast<const uint4 *>(res + static_cast<size_t>(m) * a.N + n);
+        }
+      };
+      if (cols > 0) tmem_ld16(acc, v);
+      if (res && a.vec) ask(0);
 #pragma unroll 1
-      for (int c = 0; c < kCols; c += 16) {
-        if (nbase + c >= a.N || mrow >= a.M) break;  // uniform over the warp
-        uint32_t v[16];
-        tmem_ld16(acc + c, v);
+      for (int c = 0; c < cols; c += 16) {  // uniform over the warp
+        const uint4 rcur[2] = {rnext[0], rnext[1]};
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -212,6 +244,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           f.w = __fmul_rn(static_cast<float>(static_cast<int>(v[j + 3])), sx);
           *reinterpret_cast<float4 *>(stg + lane * kEpiPitch + j) = f;
         }
+        if (c + 16 < cols) tmem_ld16(acc + c + 16, v);
+        if (res && a.vec) ask(c + 16);
         __syncwarp();
         if (a.vec) {  // lane: 8 columns of rows lane / 2 and lane / 2 + 16
           const int n = nbase + c + 8 * (lane & 1);
@@ -219,7 +253,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             const float4 w0 = __ldg(reinterpret_cast<const float4 *>(a.ws + n));
             const float4 w1 = __ldg(reinterpret_cast<const float4 *>(a.ws + n + 4));
             const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-            T bv[8];
+            T bv[8] = {};
             if (bias) {
               const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(bias + n));
               memcpy(bv, &raw, 16);
@@ -227,43 +261,49 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int r = (lane >> 1) + 16 * i, m = mrow + r;
-              if (m >= a.M) continue;
-              const size_t at = static_cast<size_t>(m) * a.N + n;
               T rv[8], o[8];
-              if (res) {
-                const uint4 raw = *reinterpret_cast<const uint4 *>(res + at);
-                memcpy(rv, &raw, 16);
-              }
+              float z[8];
+              memcpy(rv, &rcur[i], 16);
               const float *src = stg + r * kEpiPitch + 8 * (lane & 1);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                float z = __fmul_rn(src[j], w[j]);
-                if (bias) z += to_f32(bv[j]);
-                z = apply_act(z, a.act);
-                if (res) z += to_f32(rv[j]);
-                o[j] = from_f32<T>(z);
+                z[j] = __fmul_rn(src[j], w[j]);
+                if (bias) z[j] += to_f32(bv[j]);
               }
+              if constexpr (ACT) apply_act(z, a.act);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = from_f32<T>(res ? z[j] + to_f32(rv[j]) : z[j]);
               uint4 raw;
               memcpy(&raw, o, 16);
-              *reinterpret_cast<uint4 *>(y + at) = raw;
+              if (m < a.M) *reinterpret_cast<uint4 *>(y + static_cast<size_t>(m) * a.N + n) = raw;
             }
           }
         } else {  // any N: lane = column lane % 16 of rows lane / 16 + 2 i
           const int n = nbase + c + (lane & 15);
-          if (n < a.N) {
-            const float w = a.ws[n];
-            const float bv = bias ? to_f32(bias[n]) : 0.0f;
-#pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-              const int r = (lane >> 4) + 2 * i, m = mrow + r;
-              if (m >= a.M) break;
-              const size_t at = static_cast<size_t>(m) * a.N + n;
-              float z = __fmul_rn(stg[r * kEpiPitch + (lane & 15)], w);
-              if (bias) z += bv;
-              z = apply_act(z, a.act);
-              if (res) z += to_f32(res[at]);
-              y[at] = from_f32<T>(z);
+          const bool in = n < a.N;
+          const float w = in ? a.ws[n] : 0.0f;
+          const float bv = bias && in ? to_f32(bias[n]) : 0.0f;
+          T *yp = y + static_cast<size_t>(mrow + (lane >> 4)) * a.N + n;
+          const T *rp = res + static_cast<size_t>(mrow + (lane >> 4)) * a.N + n;
+          const int left = in ? a.M - mrow - (lane >> 4) : 0;  // rows of this lane: 2 i < left
+          constexpr int kBatch = ACT ? 4 : 16;  // (an activation's code 16 times over is too long)
+#pragma unroll 1
+          for (int i0 = 0; i0 < 16; i0 += kBatch) {
+            float rv[kBatch], z[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+              rv[i] = res && 2 * (i0 + i) < left ? to_f32(rp[static_cast<size_t>(2 * (i0 + i)) * a.N])
+                                                 : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              z[i] = __fmul_rn(stg[((lane >> 4) + 2 * (i0 + i)) * kEpiPitch + (lane & 15)], w);
+              if (bias) z[i] += bv;
             }
+            if constexpr (ACT) apply_act(z, a.act);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+              if (2 * (i0 + i) < left)
+                yp[static_cast<size_t>(2 * (i0 + i)) * a.N] = from_f32<T>(res ? z[i] + rv[i] : z[i]);
           }
         }
         __syncwarp();
@@ -348,7 +388,7 @@ int launch_linear(const int8_t *xq, const int8_t *w, LinArgs a, int K, cudaStrea
   a.tiles_n = (a.N + NT - 1) / NT;
   const long tiles = static_cast<long>(a.tiles_m) * a.tiles_n;
   if (tiles > 0x7fffffffl - 4096) return S8B_ERR_SHAPE;
-  auto kern = linear_tc_kernel<T, NT>;
+  auto kern = a.act == kActNone ? linear_tc_kernel<T, NT, false> : linear_tc_kernel<T, NT, true>;
   ensure_smem(reinterpret_cast<const void *>(kern), L::kSmem);
   const int grid = static_cast<int>(tiles < sm_count() ? tiles : sm_count());
   const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kLinThreads), L::kSmem, st, mx, mw, a);
