@@ -68,6 +68,23 @@ class BlockAllocator:
         return bt
 
 
+def chunk_sequences(seq_of_row: list[int], pos_of_row: list[int], chunk: int):
+    """The sequences of each chunk of ``chunk`` packed prefill rows: per chunk (sequences, context
+    lengths after the chunk, row offsets), rows of a sequence being consecutive positions."""
+    out = []
+    for c0 in range(0, len(seq_of_row), chunk):
+        seqs, ctx, cu = [], [], [0]
+        for r in range(c0, min(len(seq_of_row), c0 + chunk)):
+            if not seqs or seqs[-1] != seq_of_row[r]:
+                seqs.append(seq_of_row[r])
+                ctx.append(0)
+                cu.append(cu[-1])
+            ctx[-1] = pos_of_row[r] + 1
+            cu[-1] += 1
+        out.append((seqs, ctx, cu))
+    return out
+
+
 def chunk_row_blocks(seq_of_row: list[int], chunk: int, block_rows: int):
     """Row blocks of packed prefill rows: chunks of ``chunk`` rows are cut into runs of at most
     ``block_rows`` consecutive rows of one sequence (``seq_of_row[i]``: row i's sequence).
@@ -97,10 +114,21 @@ class DecodePipeline:
 
     # prompt tokens per prefill launch sequence (the tensor-core GEMM's token tile limit)
     PREFILL_CHUNK = 256
+    CHUNK_SEQUENCES = 1024  # most sequences of one chunk attention
 
     def __init__(self, models: list[StageModel], *, batch: int, n_micro: int = 1,
                  max_len: int = 2048, block_size: int = 16, wire_scheme: str = "int8-had",
-                 num_blocks: int | None = None, dtype=torch.bfloat16):
+                 num_blocks: int | None = None, dtype=torch.bfloat16,
+                 prefill_attention: str = "rows", fused_moe: bool = False):
+        """``prefill_attention``: "rows" (every prompt row exactly as a decode step computes it) or
+        "chunk" (``ops.paged_chunk_q8``: each chunk's rows in 128-row tiles; within rounding of
+        "rows", not bit for bit). ``fused_moe``: MoE layers of few rows in one launch
+        (``ops.moe_layer``; likewise within rounding). ``prefill_chunk`` (attribute) sets the
+        prompt rows per launch sequence; above 256 the products are tiled for the tensor pipe,
+        with the same results."""
+        if prefill_attention not in ("rows", "chunk"):
+            raise ValueError(f"prefill_attention must be 'rows' or 'chunk', got {prefill_attention!r}")
+        self.prefill_attention, self.fused_moe = prefill_attention, fused_moe
         self.models = models
         self.cfg = models[0].cfg
         self.S = len(models)
@@ -117,6 +145,8 @@ class DecodePipeline:
                              block_size, mdl.device) for mdl in models]
         self.runners = [StageRunner(mdl, pool, self.m, max_len, dtype)
                         for mdl, pool in zip(models, self.pools)]
+        for r in self.runners:
+            r.fused_moe = fused_moe
         self.mbs: list[list[MicroBatch]] = []
         for mdl in models:
             dev = mdl.device
@@ -154,6 +184,8 @@ class DecodePipeline:
 
     def set_native(self, on: bool = True):
         """Run every stage step (decode and prefill) as one ``s8b_stage_step`` call."""
+        if on and (self.fused_moe or self.prefill_attention != "rows"):
+            raise ValueError("the native stage step has neither fused_moe nor chunk attention")
         self.native = on
         for r in self.runners + (self._pf[0] if self._pf is not None else []):
             r.native = on
@@ -375,6 +407,7 @@ class DecodePipeline:
                    for mdl, pool, r in zip(self.models, self.pools, self.runners)]
         for r in runners:
             r.native = self.native
+            r.fused_moe = self.fused_moe
             r.decode_step = False  # a chunk's rows write many positions of a sequence
         from .ops import codec_sizes
 
@@ -431,7 +464,17 @@ class DecodePipeline:
         blocks, chunk_off = chunk_row_blocks(seq.tolist(), self.prefill_chunk, R)
         rbs = torch.tensor(blocks, dtype=torch.int32).reshape(-1, 2)
         host = [x.pin_memory() for x in (ids, pos, pos + 1, bt[seq], rbs)]
-        state = []  # per stage: (ids, positions, context_lens, block_table, row blocks)
+        if self.prefill_attention == "chunk":
+            # per chunk: its sequences' tables, contexts and row offsets, packed one after another
+            parts = chunk_sequences(seq.tolist(), pos.tolist(), self.prefill_chunk)
+            i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+            host += [bt[[i for p in parts for i in p[0]]].pin_memory(),
+                     i32([c for p in parts for c in p[1]]).pin_memory(),
+                     i32([c for p in parts for c in p[2]]).pin_memory()]
+            seq_off = [0]
+            for p in parts:
+                seq_off.append(seq_off[-1] + len(p[0]))
+        state = []  # per stage: (ids, positions, context_lens, block_table, row blocks, ..)
         for s, mdl in enumerate(self.models):
             st = torch.cuda.current_stream(mdl.device) if self.single_device else self.streams[s]
             with torch.cuda.device(mdl.device), torch.cuda.stream(st):
@@ -457,12 +500,18 @@ class DecodePipeline:
                         st.wait_event(ev[s - 1])
                     if s < self.S - 1 and not self.single_device:
                         st.wait_event(ev[s + 1])  # stage s+1 has decoded the previous chunk
-                    a_ids, a_pos, a_ctx, a_bt, a_rb = state[s]
+                    a_ids, a_pos, a_ctx, a_bt, a_rb, *a_ck = state[s]
                     ci = c0 // self.prefill_chunk
+                    extra = {"row_blocks": a_rb[chunk_off[ci]:chunk_off[ci + 1]]}
+                    # (more sequences in a chunk than the chunk attention takes: row by row)
+                    if a_ck and seq_off[ci + 1] - seq_off[ci] <= self.CHUNK_SEQUENCES:
+                        lo, hi = seq_off[ci], seq_off[ci + 1]
+                        extra["chunk"] = (a_ck[0][lo:hi], a_ck[1][lo:hi],
+                                          a_ck[2][lo + ci:hi + ci + 1])
                     mb = MicroBatch(ids=(out_ids if s == self.S - 1 else a_ids)[c0:c0 + r],
                                     positions=a_pos[c0:c0 + r], context_lens=a_ctx[c0:c0 + r],
                                     block_table=a_bt[c0:c0 + r],
-                                    extra={"row_blocks": a_rb[chunk_off[ci]:chunk_off[ci + 1]]})
+                                    extra=extra)
                     runners[s].run(mb, r, boundary_in=bufs[s - 1] if s > 0 else None,
                                    boundary_out=bufs[s] if s < self.S - 1 else None,
                                    head=bool(chunk_ends))

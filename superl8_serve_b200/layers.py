@@ -41,10 +41,22 @@ class LinearW8A8(nn.Module):
         self.bias = bias
         self.out_features, self.in_features = weight.data.shape
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, *, activation: str | None = None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
+        """``activation`` (None, "silu", "gelu", "gelu_tanh", "relu") and ``residual`` (the output's
+        shape and dtype) are applied in the product's epilogue, after the bias, in binary32:
+        one rounding instead of one per step."""
         _cuda(x, "LinearW8A8")
         q, s = ops.quant_rows(x)
-        y = ops.gemm_w8a8(q, s, self.weight.data, self.weight.scale, out_dtype=x.dtype)
+        w = self.weight
+        if activation is not None or residual is not None:
+            return ops.linear_w8a8(q, s, w.data, w.scale, bias=self.bias, activation=activation,
+                                   residual=residual, out_dtype=x.dtype)
+        # one row: the dp4a product; more: the tensor cores. The same bits.
+        if s.numel() == 1:
+            y = ops.gemm_w8a8(q, s, w.data, w.scale, out_dtype=x.dtype)
+        else:
+            y = ops.linear_w8a8(q, s, w.data, w.scale, out_dtype=x.dtype)
         return y if self.bias is None else y + self.bias
 
 

@@ -383,6 +383,9 @@ class StageRunner:
         # attention may stream older partitions early (s8b_paged_decode_q8_step); prefill
         # runners set False
         self.decode_step = True
+        # True: a MoE layer of few rows whose experts are all on this GPU is one launch
+        # (s8b_moe_layer: rounds to dtype once, so not bit for bit the general path)
+        self.fused_moe = False
         # True: MoE layers run their own experts only (no handshake with partner processes):
         # the stage-time measurement of a multi-process pipeline
         self.skip_remote = False
@@ -418,6 +421,7 @@ class StageRunner:
         n_max = max([w.shape[0] for L in model.layers for w in L.matrices()]
                     + ([model.head_w.shape[0]] if model.is_last else []) + [self.H])
         self.tc_ws = ops.gemm_tc_workspace(m, n_max, dev) if m >= self.tc_min else None
+        self.chunk_ws = None  # of the chunk attention, at its first use
         # tensor-core path: every weight also kept as contiguous unit images (packed once)
         self.packed: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
         if self.tc_ws is not None and share is not None and share.model is model and share.packed:
@@ -458,7 +462,8 @@ class StageRunner:
                 "as": e(A, dt=torch.float32), "contrib": e(A, self.H),
                 # tensor-core grouped GEMM: expert input rows gathered into assignment order
                 "xg": e(A, self.H, dt=torch.int8), "xgs": e(A, dt=torch.float32),
-                "status": torch.zeros(4, dtype=torch.int32, device=dev)}
+                "status": torch.zeros(4, dtype=torch.int32, device=dev),
+                "layer_ws": ops.moe_layer_workspace(k, Fe, dev)}
             # expert-parallel partners: inputs copied in, gate_up / SwiGLU rows of their own
             self.moe_peer: dict[str, dict] = {}
             for d in sorted({str(sh.device) for mw in moes for sh in mw.shards}):
@@ -476,7 +481,15 @@ class StageRunner:
                     "ev_in": torch.cuda.Event(), "ev_out": torch.cuda.Event()}
 
     # ---------------------------------------------------------------------- pieces ----
+    # rows from which a product is tiled for the tensor pipe (s8b_linear_w8a8) instead of streaming
+    # the weights once per 256 rows; the same bits either way
+    WIDE_ROWS = 257
+
     def _gemm(self, xq, xs, w, s, out, M):
+        if self.tc_ws is not None and M >= self.WIDE_ROWS:
+            call("s8b_linear_w8a8", ptr(xq), ptr(xs), ptr(w), ptr(s), None, 0, None, ptr(out), M,
+                 w.shape[0], w.shape[1], 0, ptr(self.tc_ws), self.tc_ws.numel(), stream())
+            return
         if self.tc_ws is not None and M >= self.tc_min:
             pk = self.packed.get(id(w))
             if pk is not None and pk[0] is w:
@@ -529,6 +542,13 @@ class StageRunner:
         rows in self.xq / self.xs (expert input). Result: self.h [M, H]."""
         b, st, k = self.moe_buf, stream(), mw.top_k
         E, Fe, A, H = mw.num_experts, mw.ffn, M * mw.top_k, self.H
+        if (self.fused_moe and not mw.shards and not mw.remote
+                and M <= ops.moe_layer_max_rows(H, Fe, k)):
+            call("s8b_moe_layer", ptr(b["y"]), ptr(self.xq), ptr(self.xs), ptr(mw.router),
+                 ptr(mw.gu_w), ptr(mw.gu_s), ptr(mw.d_w), ptr(mw.d_s), ptr(self.h), M, H, Fe, E, k,
+                 int(mw.norm_topk_prob), mw.scaling, ptr(b["layer_ws"]), b["layer_ws"].numel(), 0,
+                 st)
+            return
         call("s8b_moe_route", ptr(b["y"]), 0, ptr(mw.router), M, H, E, k,
              int(mw.norm_topk_prob), mw.scaling, ptr(b["topi"]), ptr(b["topw"]),
              ptr(b["offsets"]), ptr(b["sorted_assign"]), ptr(b["sorted_token"]),
@@ -582,7 +602,7 @@ class StageRunner:
         L = self.model.layers[li]
         kc, ks, vc, vs = self.pool.layer(li)
         H, st = self.H, stream()
-        split = self.part is not None and M >= self.tc_min
+        split = self.part is not None and self.tc_min <= M < self.WIDE_ROWS
         # input_layernorm (fused residual add, except on the model's first layer)
         self._rms_quant(self.h, None if first_layer_of_model else self.res, self.res, L.in_norm,
                         M, H, src=h_src)
@@ -596,8 +616,18 @@ class StageRunner:
         else:
             self._gemm(self.xq, self.xs, L.qkv_w, L.qkv_s, self.qkv, M)
             call("s8b_qkv_post", ptr(self.qkv), *post)
-        rb = mb.extra.get("row_blocks")
-        if rb is not None:  # prefill rows: each row block's partitions staged once
+        rb, ck = mb.extra.get("row_blocks"), mb.extra.get("chunk")
+        if ck is not None:  # a chunk of rows per sequence: (block tables, contexts, row offsets)
+            bt, ctx, cu = ck
+            if self.chunk_ws is None:
+                self.chunk_ws = ops.chunk_workspace(self.dev)
+            call("s8b_paged_chunk_q8", ptr(self.q_i8), ptr(self.q_s), ptr(kc), ptr(ks), ptr(vc),
+                 ptr(vs), ptr(bt), ptr(ctx), ptr(cu), ptr(self.attn), M, bt.shape[0], self.Hq,
+                 self.Hkv, self.D, self.pool.block_size, bt.shape[1], self.pool.num_blocks,
+                 self.scale, ptr(self.chunk_ws), self.chunk_ws.numel(), 0, st)
+            call("s8b_quant_rows", ptr(self.attn), 0, ptr(self.xq), ptr(self.xs), M,
+                 self.Hq * self.D, st)
+        elif rb is not None:  # prefill rows: each row block's partitions staged once
             call("s8b_paged_prefill_q8", ptr(self.q_i8), ptr(self.q_s), ptr(kc), ptr(ks),
                  ptr(vc), ptr(vs), ptr(mb.block_table), ptr(mb.context_lens), ptr(rb),
                  rb.shape[0], ptr(self.attn), ptr(self.xq), ptr(self.xs), M, self.Hq, self.Hkv,
@@ -650,6 +680,8 @@ class StageRunner:
         M = self.m if M is None else M
         st = stream()
         if self.native:
+            if self.fused_moe or "chunk" in mb.extra:
+                raise RuntimeError("the native stage step has neither fused_moe nor chunk attention")
             from .native import stage_desc
 
             d = stage_desc(self, mb, M, boundary_in, boundary_out, head)

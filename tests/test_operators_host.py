@@ -108,3 +108,23 @@ def test_moe_layer_rows():
         ops.moe_layer(z(1, 32), z(1, 32, dtype=torch.int8), z(1), z(2, 32),
                       z(2, 32, 32, dtype=torch.int8), z(2, 32), z(2, 32, 16, dtype=torch.int8),
                       z(2, 32), 1)
+
+
+def test_chunk_sequences():
+    from superl8_serve_b200.engine import chunk_sequences
+
+    lens = [5, 1, 9]
+    seq = [i for i, n in enumerate(lens) for _ in range(n)]
+    pos = [p for n in lens for p in range(n)]
+    got = chunk_sequences(seq, pos, 4)
+    assert got == [([0], [4], [0, 4]), ([0, 1, 2], [5, 1, 2], [0, 1, 2, 4]), ([2], [6], [0, 4]),
+                   ([2], [9], [0, 3])]
+    for seqs, ctx, cu in got:
+        assert len(seqs) == len(ctx) == len(cu) - 1
+
+
+def test_pipeline_options_are_checked():
+    from superl8_serve_b200.engine import DecodePipeline
+
+    with pytest.raises(ValueError, match="prefill_attention"):
+        DecodePipeline([], batch=1, prefill_attention="tiles")

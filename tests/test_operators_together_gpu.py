@@ -1,0 +1,194 @@
+"""GPU: the linear, chunk-attention and few-row MoE operators as the layers, the stage runner
+and the pipeline use them, and one after another as a decoder layer does."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def _weight(g, n, k):
+    w = torch.randint(-127, 128, (n, k), generator=g, device=DEV, dtype=torch.int8)
+    return w, (0.5 + torch.rand(n, generator=g, device=DEV)) / (73 * math.sqrt(k))
+
+
+# ------------------------------------------------------------------------------- layers ----
+@pytest.mark.parametrize("M", [1, 2, 37, 300])
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear_layer_keeps_its_results(M, bias):
+    """Without activation and residual: the dp4a product (and the bias added after it), bit for
+    bit as before."""
+    from superl8_serve_b200 import ops
+    from superl8_serve_b200.layers import LinearW8A8
+    from superl8_serve_b200.weights import QTensor
+
+    g = _gen(M)
+    w, ws = _weight(g, 260, 272)
+    b = torch.randn(260, generator=g, device=DEV).bfloat16() if bias else None
+    lin = LinearW8A8(QTensor(w, ws, "per_row_i8"), b)
+    x = torch.randn(M, 272, generator=g, device=DEV).bfloat16()
+    q, s = ops.quant_rows(x)
+    want = ops.gemm_w8a8(q, s, w, ws)
+    assert torch.equal(lin(x), want if b is None else want + b)
+    assert torch.equal(lin(x.view(1, M, 272))[0], lin(x))
+    r = torch.randn(M, 260, generator=g, device=DEV).bfloat16()
+    assert torch.equal(lin(x, activation="gelu", residual=r),
+                       ops.linear_w8a8(q, s, w, ws, bias=b, activation="gelu", residual=r))
+
+
+# ------------------------------------------------------------- one after another ----------
+def test_a_sparse_layer_over_a_chunk_of_draft_rows():
+    """Three sequences bring 4, 1 and 7 new rows: keys and values go to the pages, the chunk
+    attends over them, the output projection adds the residual, the MoE layer follows. Each step
+    is checked against 64 bits on what the step before it gave."""
+    from superl8_serve_b200 import ops
+    from superl8_serve_b200.layers import rope_tables
+    from test_chunk_attention_gpu import Case
+    from test_linear_gpu import _exact, _near
+    from test_moe_layer_gpu import Layer
+
+    H, Hq, Hkv, bs = 512, 8, 2, 16
+    lens = [(4, 150), (1, 33), (7, 7)]
+    g = _gen(5)
+    c = Case(lens, Hq, Hkv, bs, seed=5)
+    T = c.T
+    seq = torch.tensor([i for i, (n, _) in enumerate(lens) for _ in range(n)], device=DEV)
+    pos = torch.cat([torch.arange(m - n, m) for n, m in lens]).to(torch.int32).to(DEV)
+    cos, sin = (t.to(DEV) for t in rope_tables(128, 256))
+    gain = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * 128, generator=g, device=DEV).bfloat16()
+    before = c.kc.clone()
+    c.q, c.qs, _ = ops.qkv_post(qkv, pos, cos, sin, gain, gain, 1e-6, Hq, Hkv, c.kc, c.ks, c.vc,
+                                c.vs, block_table=c.bt[seq].contiguous())
+    slot = c.bt[seq, (pos // bs).long()].long(), (pos % bs).long()
+    same = torch.ones(c.kc.shape[0], bs, dtype=torch.bool, device=DEV)
+    same[slot] = False
+    assert torch.equal(c.kc.transpose(1, 2)[same], before.transpose(1, 2)[same])
+    attn = c.run()
+    c.check(attn)
+
+    w, ws = _weight(g, H, Hq * 128)
+    res = torch.randn(T, H, generator=g, device=DEV).bfloat16()
+    aq, asc = ops.quant_rows(attn)
+    h = ops.linear_w8a8(aq, asc, w, ws, residual=res)
+    _near(h, *_exact(aq, asc, w, ws, None, res, None))
+
+    L = Layer(T, H, 128, 16, 4, seed=6)
+    _, L.xq, L.xs, L.y = ops.rmsnorm_quant(h, None, torch.ones(H, dtype=torch.bfloat16, device=DEV),
+                                           1e-6, y_out=True)
+    L.check(L.run())
+
+
+# ----------------------------------------------------------------------------- pipeline ----
+def _models(cfg, stages=1, seed=3):
+    from superl8_serve_b200.runtime import StageModel
+    from superl8_serve_b200.weights import random_state_dict
+
+    sd = random_state_dict(cfg, seed, w_std=0.1)
+    n = cfg.num_hidden_layers
+    cut = [i * n // stages for i in range(stages + 1)]
+    return [StageModel.from_state_dict(cfg, sd, cut[s], cut[s + 1], DEV, first=s == 0,
+                                       last=s == stages - 1) for s in range(stages)]
+
+
+def _prompts(lens, vocab, seed=0):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return [torch.randint(0, vocab, (n,), generator=g).tolist() for n in lens]
+
+
+@pytest.mark.parametrize("stages", [1, 2])
+def test_wide_prefill_chunks_give_the_same_bits(stages):
+    from superl8_serve_b200.config import tiny
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny()
+    models = _models(cfg, stages)
+    prompts = _prompts([300, 7, 411], cfg.vocab_size)
+    got = []
+    for chunk in (256, 700):
+        pipe = DecodePipeline(models, batch=3, max_len=512)
+        pipe.prefill_chunk = chunk
+        got.append(pipe.prefill(prompts, keep_logits=True))
+    assert got[0][0] == got[1][0]
+    for a, b in zip(got[0][1], got[1][1]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("chunk", [64, 256, 1000])
+def test_chunk_attention_in_the_prefill(chunk):
+    """One layer, so that both kinds of attention see the same queries and pages: the last chunk's
+    attention rows differ by the two forms' roundings of the weights, 2^-8 and below 2^-9 of the
+    average of |v|, itself at most the largest |v| of the pool, and the outputs' roundings."""
+    from superl8_serve_b200.config import tiny
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny(num_hidden_layers=1)
+    models = _models(cfg)
+    prompts = _prompts([300, 1, 411, 90], cfg.vocab_size)
+    rows, pools = [], []
+    for kind in ("rows", "chunk"):
+        pipe = DecodePipeline(models, batch=4, max_len=512, prefill_attention=kind)
+        pipe.prefill_chunk = chunk
+        first = pipe.prefill(prompts)
+        n = (300 + 1 + 411 + 90 - 1) % chunk + 1  # rows of the last chunk
+        rows.append(pipe._pf[0][0].attn[:n].double())
+        pools.append(pipe.pools[0])
+        assert len(first) == 4 and all(0 <= t < cfg.vocab_size for t in first)
+        ws = pipe._pf[0][0].chunk_ws
+        assert (ws is None) == (kind == "rows")
+        assert ws is None or int(ws[:4].view(torch.int32)) == 0
+    assert torch.equal(pools[0].vc, pools[1].vc) and torch.equal(pools[0].kc, pools[1].kc)
+    top = (pools[0].vc.float().abs() * pools[0].vs[..., None]).max().item()
+    assert (rows[0] - rows[1]).abs().max().item() <= (2 ** -8 + 2 ** -9 + 2 * 2 ** -8) * top
+    assert (rows[0] - rows[1]).norm() < 2 ** -7 * rows[0].norm()
+
+
+def test_generation_with_chunk_attention_and_continuation():
+    from superl8_serve_b200.config import tiny
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny()
+    pipe = DecodePipeline(_models(cfg, 2), batch=3, max_len=512, prefill_attention="chunk")
+    outs = pipe.generate(_prompts([40, 3, 130], cfg.vocab_size, 1), 5, prefill=True)
+    assert [len(o) for o in outs] == [5, 5, 5]
+    assert all(0 <= t < cfg.vocab_size for o in outs for t in o)
+    with pytest.raises(ValueError, match="native"):
+        pipe.set_native()
+
+
+@pytest.mark.parametrize("batch", [1, 5, 16])
+def test_fused_moe_in_the_decode_step(batch):
+    """One sparse layer: its output against the general path's on the same rows, within that
+    path's own roundings to dtype (16 steps of at most 2^-8 each)."""
+    from superl8_serve_b200.config import tiny_moe
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny_moe(num_hidden_layers=1)
+    models = _models(cfg)
+    h = []
+    for fused in (False, True):
+        pipe = DecodePipeline(models, batch=batch, max_len=64, fused_moe=fused)
+        pipe.add_sequences()
+        pipe.set_state([0] * batch, list(range(3, 3 + batch)), reserve=4)
+        pipe.step()
+        pipe.synchronize()
+        h.append(pipe.runners[0].h[:batch].double().clone())
+        pipe.capture()
+        for _ in range(3):
+            pipe.step()
+        pipe.synchronize()
+        assert int(pipe.runners[0].moe_buf["layer_ws"][:4].view(torch.int32)) == 0
+        toks = pipe.tokens().tolist()
+        assert all(0 <= t < cfg.vocab_size for t in toks)
+    assert ((h[0] - h[1]).norm() / h[0].norm()).item() < 16 * 2 ** -8
+    assert not torch.equal(h[0], h[1]) or batch == 1
