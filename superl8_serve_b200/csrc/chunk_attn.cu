@@ -146,11 +146,12 @@ __device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t addr, uint32_t *v) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st_16x128_x2(uint32_t addr, const uint32_t *v) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%4], {%0,%1,%2,%3};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(addr));
-}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// What packing v to two bf16 left over, packed: exact differences, rounded again.
+__device__ __forceinline__ uint32_t pack_rest(float2 v, uint32_t p) {
+  return pack_bf16(add2(v, make_float2(-__uint_as_float(p << 16), -__uint_as_float(p & 0xffff0000u))));
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -306,6 +307,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_q, const ChunkArgs a) {
   using namespace ca;
+  // fp16 results keep 11 bits, so their weights go as two bf16 terms and the second product runs
+  // twice (for bf16 results the weights' 8 bits stay below the output's own rounding)
+  constexpr bool kTwo = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~uintptr_t(1023));
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     // rows l / 4 + 8 j (j = 0..3) of its warp's 32, so that a scale read from shared memory
     // serves four rows (with a row per lane the broadcast reads alone took as long as the
     // exponentials: 512 bytes of register writes for 4 values).
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTwo ? 176 : 160));
     const int hf = warp >> 2, quad = lane & 3;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + hf * 128 + lanes, to = tmem + 256 + hf * 128 + lanes;
@@ -552,11 +556,19 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
           // magnitude, so the reference has to be near the row's maximum, not at it, and the sum
           // of these keys alone shows whether it still is. Returns whether it was (else nothing
           // has been written).
+          auto put = [&](const uint32_t (&pk)[2][16], const uint32_t (&pl)[2][16]) {
+            tmem_st_16x128_x8(tu, pk[0]);
+            tmem_st_16x128_x8(tu + kLow, pk[1]);
+            if constexpr (kTwo) {
+              tmem_st_16x128_x8(tu + 32, pl[0]);
+              tmem_st_16x128_x8(tu + 32 + kLow, pl[1]);
+            }
+          };
           auto pass = [&](auto masked) -> bool {
             float2 sum[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
-            uint32_t v[2][2][16], pk[2][16];
+            uint32_t v[2][2][16], pk[2][16], pl[2][16];
             tmem_ld_16x256_x4(tu, v[0][0]);
             tmem_ld_16x256_x4(tu + kLow, v[0][1]);
 #pragma unroll
@@ -584,6 +596,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                   }
                   sum[j] = add2(sum[j], e);
                   pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(w);
+                  if constexpr (kTwo)
+                    pl[j >> 1][8 * b + 2 * q + (j & 1)] =
+                        pack_rest(w, pk[j >> 1][8 * b + 2 * q + (j & 1)]);
                 }
               }
             }
@@ -596,8 +611,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
             if (!__all_sync(0xffffffffu, fits)) return false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
-            tmem_st_16x128_x8(tu, pk[0]);
-            tmem_st_16x128_x8(tu + kLow, pk[1]);
+            put(pk, pl);
             return true;
           };
           const bool masked = k >= whole_tiles;
@@ -678,9 +692,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                 tmem_st_16x256_x1(to + kLow + 8 * q, v + 4);
               }
             }
-#pragma unroll 1
-            for (int b = 0; b < 64; b += 16) {  // P's columns b / 2 .. end before S's from b + 16 on
-              uint32_t v[2][8], pk[2][4];
+            uint32_t pk[2][16], pl[2][16];
+#pragma unroll
+            for (int b = 0; b < 64; b += 16) {
+              uint32_t v[2][8];
               tmem_ld_16x256_x2(tu + b, v[0]);
               tmem_ld_16x256_x2(tu + kLow + b, v[1]);
               tmem_wait_ld();
@@ -697,13 +712,14 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                   const float e0 = s0 ? ex2(fmaf(x0, c[j], nm)) : 0.0f;
                   const float e1 = s1 ? ex2(fmaf(x1, c[j], nm)) : 0.0f;
                   l[j] += e0 + e1;
-                  pk[j >> 1][2 * q + (j & 1)] =
-                      pack_bf16(make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f));
+                  const float2 w = make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f);
+                  const int at = b / 4 + 2 * q + (j & 1);
+                  pk[j >> 1][at] = pack_bf16(w);
+                  if constexpr (kTwo) pl[j >> 1][at] = pack_rest(w, pk[j >> 1][at]);
                 }
               }
-              tmem_st_16x128_x2(tu + b / 2, pk[0]);
-              tmem_st_16x128_x2(tu + kLow + b / 2, pk[1]);
             }
+            put(pk, pl);
           }
           tmem_wait_st();
           tc_fence_before();
@@ -819,7 +835,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     }
   } else if (warp < 12) {
     // --------------------------------------------------------------- V codes to bf16 ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTwo ? 80 : 96));
     const int ct = threadIdx.x - 256;
     const int ch = ct & 7, key0 = ct >> 3;  // 16-byte chunk, first key; keys step by 16
     int kt = 0;
@@ -868,7 +884,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       done();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTwo ? 80 : 96));
     if (warp < 14) {
       // ----------------------------------------------------------------- MMA issuers ----
       // All lanes walk the tiles, one elected lane issues: descriptors then stay in uniform
@@ -941,6 +957,11 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
 #pragma unroll
               for (int x = 1; x < 4; ++x)
                 mma_bf16_ts(tmem_o, pa + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
+              if constexpr (kTwo) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                  mma_bf16_ts(tmem_o, pa + 32 + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
+              }
               mma_commit(&pvin[2 * hf + h]);
               if (more) scores(j + step, h);
               if (h == 1) {
