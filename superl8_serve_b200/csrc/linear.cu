@@ -72,15 +72,21 @@ struct LinArgs {
   int vec;  // out, bias and residual rows keep 16-byte alignment
 };
 
-constexpr int kLinThreads = 320;
 constexpr int kTileM = 128;
 constexpr int kSlice = 128;       // K bytes per stage
 constexpr int kEpiPitch = 20;     // floats per staged row of 16 (16-byte rows, no bank conflicts)
-constexpr int kEpiWarps = 8;
 
-template <int NT>
+template <int NT, bool ACT>
 struct LinLayout {
-  static constexpr int kStages = NT == 256 ? 4 : 6;
+  // An activation is long in instructions and a warp waits on most of them: 16 warps finish a
+  // tile sooner where its K loop does not hide it (999 x 5127 x 1040 with GELU: 39.5 -> 29.8 us;
+  // 4096 x 4096 x 4096, whose loop does: 88.6 -> 90.0). They cost a stage of the ring, so
+  // without an activation it stays at 8 (4096 cubed with bias and residual: 77.6 against 81.0),
+  // and beside 256-wide tiles' stages their staging has no room.
+  static constexpr int kEpiWarps = NT == 128 && ACT ? 16 : 8;
+  static constexpr int kStages = NT == 256 ? 4 : ACT ? 5 : 6;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kCols = 4 * NT / kEpiWarps;  // columns that an epilogue warp finishes
   static constexpr int kStageBytes = (kTileM + NT) * kSlice;
   static constexpr int kEpi = kStages * kStageBytes;                 // staging of the epilogue
   static constexpr int kHdr = kEpi + kEpiWarps * 32 * kEpiPitch * 4;  // barriers
@@ -101,10 +107,10 @@ __device__ __forceinline__ void tile_at(int t, const LinArgs &a, int *m0, int *n
 }
 
 template <typename T, int NT, bool ACT>
-__global__ void __launch_bounds__(kLinThreads, 1)
+__global__ void __launch_bounds__(LinLayout<NT, ACT>::kThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_w, const LinArgs a) {
-  using L = LinLayout<NT>;
+  using L = LinLayout<NT, ACT>;
   constexpr int kStages = L::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpiWarps);
+      mbar_init(&acc_empty[i], L::kEpiWarps);
     }
     mbar_init(drained, 1);
     *abort_flag = 0;
@@ -197,11 +203,11 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       mbar_drain(drained, 0);
     }
   } else {
-    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    const int ew = warp - 2, quad = warp & 3, part = ew >> 2;
     float *stg = reinterpret_cast<float *>(sm + L::kEpi) + ew * 32 * kEpiPitch;
     const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.res);
     T *y = static_cast<T *>(a.y);
-    constexpr int kCols = NT / 2;  // columns of this warp: one half of the tile
+    constexpr int kCols = L::kCols;
     int q = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++q) {
       const int b = q & 1;
@@ -212,8 +218,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       tc_fence_after();
       const int mrow = m0 + 32 * quad;
       const float sx = mrow + lane < a.M ? a.xs[mrow + lane] : 0.0f;
-      const uint32_t acc = tmem + b * NT + half * kCols + (static_cast<uint32_t>(32 * quad) << 16);
-      const int nbase = n0 + half * kCols;
+      const uint32_t acc = tmem + b * NT + part * kCols + (static_cast<uint32_t>(32 * quad) << 16);
+      const int nbase = n0 + part * kCols;
       // Columns of this warp that exist. While a chunk of 16 is finished from shared memory, the
       // next one's sums are on their way from TMEM and its residual from global memory (loaded
       // when needed, the residual cost 12 of 89 us at 4096 x 4096 x 4096).
@@ -229,8 +235,16 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             rnext[i] = *reinterpret_cast<const uint4 *>(res + static_cast<size_t>(m) * a.N + n);
         }
       };
+      float wnext = 0.0f, bnext = 0.0f;
+      auto ask_col = [&](int c) {  // the scale and bias of chunk c (any N)
+        const int n = nbase + c + (lane & 15);
+        const bool in = c < cols && n < a.N;
+        wnext = in ? __ldg(a.ws + n) : 0.0f;
+        bnext = bias && in ? to_f32(bias[n]) : 0.0f;
+      };
       if (cols > 0) tmem_ld16(acc, v);
-      if (res && a.vec) ask(0);
+      if (!a.vec) ask_col(0);
+      else if (res) ask(0);
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {  // uniform over the warp
         const uint4 rcur[2] = {rnext[0], rnext[1]};
@@ -245,7 +259,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           *reinterpret_cast<float4 *>(stg + lane * kEpiPitch + j) = f;
         }
         if (c + 16 < cols) tmem_ld16(acc + c + 16, v);
-        if (res && a.vec) ask(c + 16);
+        const float w1c = wnext, b1c = bnext;
+        if (!a.vec) ask_col(c + 16);
+        else if (res) ask(c + 16);
         __syncwarp();
         if (a.vec) {  // lane: 8 columns of rows lane / 2 and lane / 2 + 16
           const int n = nbase + c + 8 * (lane & 1);
@@ -281,8 +297,6 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         } else {  // any N: lane = column lane % 16 of rows lane / 16 + 2 i
           const int n = nbase + c + (lane & 15);
           const bool in = n < a.N;
-          const float w = in ? a.ws[n] : 0.0f;
-          const float bv = bias && in ? to_f32(bias[n]) : 0.0f;
           T *yp = y + static_cast<size_t>(mrow + (lane >> 4)) * a.N + n;
           const T *rp = res + static_cast<size_t>(mrow + (lane >> 4)) * a.N + n;
           const int left = in ? a.M - mrow - (lane >> 4) : 0;  // rows of this lane: 2 i < left
@@ -296,8 +310,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                                                  : 0.0f;
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-              z[i] = __fmul_rn(stg[((lane >> 4) + 2 * (i0 + i)) * kEpiPitch + (lane & 15)], w);
-              if (bias) z[i] += bv;
+              z[i] = __fmul_rn(stg[((lane >> 4) + 2 * (i0 + i)) * kEpiPitch + (lane & 15)], w1c);
+              if (bias) z[i] += b1c;
             }
             if constexpr (ACT) apply_act(z, a.act);
 #pragma unroll
@@ -376,9 +390,9 @@ inline int pick_width(int M, int N) {
   return w128 * 9 < w256 * 16 ? 128 : 256;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool ACT>
 int launch_linear(const int8_t *xq, const int8_t *w, LinArgs a, int K, cudaStream_t st) {
-  using L = LinLayout<NT>;
+  using L = LinLayout<NT, ACT>;
   CUtensorMap mx, mw;
   int rc = make_map_2d(&mx, xq, K, a.M, K, kSlice, kTileM);
   if (!rc) rc = make_map_2d(&mw, w, K, a.N, K, kSlice, NT);
@@ -388,10 +402,10 @@ int launch_linear(const int8_t *xq, const int8_t *w, LinArgs a, int K, cudaStrea
   a.tiles_n = (a.N + NT - 1) / NT;
   const long tiles = static_cast<long>(a.tiles_m) * a.tiles_n;
   if (tiles > 0x7fffffffl - 4096) return S8B_ERR_SHAPE;
-  auto kern = a.act == kActNone ? linear_tc_kernel<T, NT, false> : linear_tc_kernel<T, NT, true>;
+  auto kern = linear_tc_kernel<T, NT, ACT>;
   ensure_smem(reinterpret_cast<const void *>(kern), L::kSmem);
   const int grid = static_cast<int>(tiles < sm_count() ? tiles : sm_count());
-  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kLinThreads), L::kSmem, st, mx, mw, a);
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(L::kThreads), L::kSmem, st, mx, mw, a);
   if (e != cudaSuccess) {
     record_cuda_error(e);
     return S8B_ERR_CUDA;
@@ -464,9 +478,13 @@ extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *
           aligned(ws, 16);
   S8B_DISPATCH_DTYPE(dtype, T, {
     if (few_rows(M, K)) return launch_few<T>(xq, xs, w, a, K, workspace, dtype, stream);
-    return pick_width(M, N) == 256
-               ? launch_linear<T, 256>(xq, w, a, K, (cudaStream_t)stream)
-               : launch_linear<T, 128>(xq, w, a, K, (cudaStream_t)stream);
+    auto st = (cudaStream_t)stream;
+    const bool act = activation != kActNone;
+    if (pick_width(M, N) == 256)
+      return act ? launch_linear<T, 256, true>(xq, w, a, K, st)
+                 : launch_linear<T, 256, false>(xq, w, a, K, st);
+    return act ? launch_linear<T, 128, true>(xq, w, a, K, st)
+               : launch_linear<T, 128, false>(xq, w, a, K, st);
   });
   return S8B_OK;
 }
