@@ -400,20 +400,21 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
   for (int s = threadIdx.x; s < S; s += kThreads) {
     const int nt = tiles_of(tab, a, s);
     if (nt > kFewTiles) continue;
-    int w = 0;
+    long long w = 0;
 #pragma unroll 1
     for (int t = 0; t < nt; ++t) w += item_at(tab, a, s, t).units;
-    pre[s + 1] = static_cast<long long>(w) * a.Hkv;
+    pre[s + 1] = w * a.Hkv;
   }
 #pragma unroll 1
   for (int s = warp; s < S; s += kThreads / 32) {
     const int nt = tiles_of(tab, a, s);
     if (nt <= kFewTiles) continue;
-    int w = 0;
+    long long w = 0;
 #pragma unroll 1
     for (int t = lane; t < nt; t += 32) w += item_at(tab, a, s, t).units;
-    w = __reduce_add_sync(0xffffffffu, w);
-    if (lane == 0) pre[s + 1] = static_cast<long long>(w) * a.Hkv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (lane == 0) pre[s + 1] = w * a.Hkv;
   }
   __syncthreads();
   if (warp == 0) {
@@ -447,14 +448,15 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     const int s = first[0];
     const long long per = (pre[s + 1] - pre[s]) / a.Hkv, rem = u0 - pre[s];
     const int g = static_cast<int>(rem / per);
-    int r = static_cast<int>(rem - g * per), t0 = 0;
+    long long r = rem - g * per;  // units of this head before the run
+    int t0 = 0;
     const int nt = tiles_of(tab, a, s);
     while (true) {
       const int u = t0 + lane < nt ? item_at(tab, a, s, t0 + lane).units : 0;
-      int v = u;
+      long long v = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, v, o);
+        const long long x = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += x;
       }
       const uint32_t hit = __ballot_sync(0xffffffffu, v > r);
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
         if (lane == __ffs(hit) - 1) {
           first[1] = g;
           first[2] = t0 + lane;
-          first[3] = r - (v - u);
+          first[3] = static_cast<int>(r - (v - u));
         }
         break;
       }

@@ -50,13 +50,13 @@ class LinearW8A8(nn.Module):
         q, s = ops.quant_rows(x)
         w = self.weight
         if activation is not None or residual is not None:
-            return ops.linear_w8a8(q, s, w.data, w.scale, bias=self.bias, activation=activation,
-                                   residual=residual, out_dtype=x.dtype)
+            return ops.linear_w8a8(q, s, w.data, w.scale.reshape(-1), bias=self.bias,
+                                   activation=activation, residual=residual, out_dtype=x.dtype)
         # one row: the dp4a product; more: the tensor cores. The same bits.
         if s.numel() == 1:
             y = ops.gemm_w8a8(q, s, w.data, w.scale, out_dtype=x.dtype)
         else:
-            y = ops.linear_w8a8(q, s, w.data, w.scale, out_dtype=x.dtype)
+            y = ops.linear_w8a8(q, s, w.data, w.scale.reshape(-1), out_dtype=x.dtype)
         return y if self.bias is None else y + self.bias
 
 

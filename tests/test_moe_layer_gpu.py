@@ -182,3 +182,24 @@ def test_graph_and_out():
     torch.cuda.synchronize()
     L.check(out[1:5])
     assert (out[0] == 5).all() and (out[5] == 5).all()
+
+
+def test_two_streams_with_their_own_workspaces():
+    """Each launch needs every SM for its barriers: launches of two streams take turns."""
+    from superl8_serve_b200 import ops
+
+    Ls = [Layer(16, 1024, 512, 32, 4, seed=21), Layer(3, 512, 256, 8, 2, seed=22)]
+    want = [L.run() for L in Ls]
+    sts = [torch.cuda.Stream() for _ in Ls]
+    wss = [ops.moe_layer_workspace(L.k, L.F, DEV) for L in Ls]
+    outs = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, L in enumerate(Ls):
+            with torch.cuda.stream(sts[i]):
+                outs[i].append(ops.moe_layer(L.y, L.xq, L.xs, L.gate, L.gu_w, L.gu_s, L.d_w,
+                                             L.d_s, L.k, workspace=wss[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert int(wss[i][:4].view(torch.int32)) == 0
+        assert all(torch.equal(o, want[i]) for o in outs[i])

@@ -192,3 +192,17 @@ def test_fused_moe_in_the_decode_step(batch):
         assert all(0 <= t < cfg.vocab_size for t in toks)
     assert ((h[0] - h[1]).norm() / h[0].norm()).item() < 16 * 2 ** -8
     assert not torch.equal(h[0], h[1]) or batch == 1
+
+
+def test_linear_layer_takes_scales_as_a_column():
+    """As the dp4a product does, which took several rows before the tensor cores took over."""
+    from superl8_serve_b200 import ops
+    from superl8_serve_b200.layers import LinearW8A8
+    from superl8_serve_b200.weights import QTensor
+
+    g = _gen(3)
+    w, ws = _weight(g, 24, 272)
+    lin = LinearW8A8(QTensor(w, ws[:, None], "per_row_i8"))
+    x = torch.randn(3, 272, generator=g, device=DEV).bfloat16()
+    q, s = ops.quant_rows(x)
+    assert torch.equal(lin(x), ops.gemm_w8a8(q, s, w, ws))
