@@ -12,9 +12,10 @@
  * Citations name the superl8-serve (reference) interface each entry point replaces; the
  * reference binds its kernels through the `superl8` Python package at those call sites.
  *
- * Numerics: every entry point reproduces the CPU oracle (oracle/ in this repository) bit for
- * bit: binary32 operations in a fixed order without FMA contraction, int32 accumulation for
- * integer products, float64 accumulation for the RMSNorm sums of squares.
+ * Numerics: unless its comment says otherwise, an entry point reproduces the CPU oracle (oracle/
+ * in this repository) bit for bit: binary32 operations in a fixed order without FMA contraction,
+ * int32 accumulation for integer products, float64 accumulation for the RMSNorm sums of squares.
+ * s8b_linear_w8a8's activations, s8b_paged_chunk_q8 and s8b_moe_layer round less often instead.
  */
 #ifndef S8B_H_
 #define S8B_H_
@@ -278,10 +279,11 @@ int s8b_paged_prefill_q8(const int8_t *q_i8, const float *q_s, const int8_t *kc,
  * position gets zeros; rows of out [T, Hq*D] (dtype) behind cu_q[S] are left as they are.
  * cu_q [S+1] and context_lens [S] are read on the device, so a captured graph may replay with
  * other lengths; kc/vc [num_blocks, Hkv, bs, D], ks/vs [num_blocks, Hkv, bs].
- * Numerics: q.k exact, softmax in binary32, the weights e^(t - m) * vs rounded to bf16 before
- * the second product (binary32 sums), one rounding to dtype. Not part of the bit-exact
- * contract of the decode and prefill entry points (their weights have 15 bits relative to a
- * partition's largest); the result is the same on every run, whatever the other streams do.
+ * Numerics: q.k exact, softmax in binary32, the weights e^(t - m) * vs rounded to bf16 (for fp16
+ * results, and where max_blocks * block_size <= 256: to the sum of two bf16 numbers, 16 bits)
+ * before the second product (binary32 sums), one rounding to dtype. Not part of the bit-exact contract of the decode and prefill entry
+ * points (their weights have 15 bits relative to a partition's largest); the result is the same
+ * on every run, whatever the other streams do.
  * D = 128; block_size a power of two up to 256; Hq / Hkv <= 128; S <= 1024; scale > 0. q_i8,
  * kc, vc, out 16-byte aligned. workspace: s8b_paged_chunk_workspace_size() bytes (any shape),
  * 256-byte aligned, its first 256 bytes zero-filled once. workspace[0] (int32) receives

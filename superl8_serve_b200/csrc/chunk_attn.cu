@@ -8,7 +8,20 @@
 // rounded to bf16 for the second product (kind::f16 with binary32 sums), whose other operand,
 // the value codes, bf16 holds exactly. bf16 rather than fp16: its range is binary32's, so no
 // token's scale can overflow or vanish beside another's, and half a step of it (2^-9 to 2^-8)
-// on weights that are then averaged stays below the output's own rounding to bf16.
+// on weights that are then averaged stays below the output's own rounding to bf16. fp16 results
+// keep three bits more, so their weights go as two bf16 terms, p and what rounding to p left over,
+// and the second product runs once for each (error against 64 bits 1.7e-3 -> 2.1e-4); bf16
+// results behind short tables too (see the launch).
+//
+// Bound. Each score (row x key) costs 2 x 128 int8 and 2 x 128 bf16 operations, one exponential
+// and about 5 further instructions; a key's bytes serve 128 rows. Above some 16 rows per sequence
+// the bf16 product sets the floor (1635 TFLOP/s measured), below it the keys' 264 bytes per head.
+// What bounds the kernel is the softmax warps' instruction issue: a step of 64 keys takes its
+// group 850 cycles alone and 1270 beside the other group, against 512 of tensor work for both.
+// Measured (GPU time in a graph, beside the floor): 4096 new rows over 16K keys, 32 heads on 4,
+// 1284 us in fp16 and 1174 in bf16 (589 at the tensor rate); eight prompts of up to 2048 rows, 32
+// on 8, 364 us (102); 64 sequences x up to 4 draft rows over up to 2048 keys 108 us (27 at the
+// copy rate); 2 sequences x 16 rows over 64K keys, 40 on 8, 73 us (21); 5 rows 15 us.
 //
 // Unit of work. The G query heads of a kv head share its keys, so a tile's 128 rows are
 // 128 / G tokens x G heads, and an item is two such tiles (A and B) of one sequence and kv head:
@@ -55,6 +68,7 @@ constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4
 constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
 constexpr int kItemRows = 2 * kRows;
 constexpr float kSumMax = 0x1p60f;  // a tile's sum of e^(t - reference) above: a new reference
+constexpr int kFewKeys = 256;     // contexts up to which bf16 results' weights have two terms
 constexpr int kMaxCtas = 512;     // CTAs the workspace has room for
 // workspace: status word, per-CTA metadata, partials
 struct Meta {  // an item whose first piece is CTA c's (slot 2c + 1); pieces go on in slots 2c' + 0
@@ -131,19 +145,29 @@ __device__ __forceinline__ void tmem_ld_16x256_x1(uint32_t addr, uint32_t *v) {
                : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t addr, uint32_t *v) {
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-               : "r"(addr));
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,"
+      "%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st_16x256_x1(uint32_t addr, const uint32_t *v) {
-  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%4], {%0,%1,%2,%3};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(addr));
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%4], {%0,%1,%2,%3};" ::"r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(addr));
 }
 __device__ __forceinline__ void tmem_st_16x128_x8(uint32_t addr, const uint32_t *v) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr));
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,"
+      "%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t addr, uint32_t *v) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+                 "=r"(v[6]), "=r"(v[7])
                : "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -159,15 +183,13 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
 __device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Arrives on `bar` when all of this thread's cp.async so far have landed.
 __device__ __forceinline__ void cp_arrive(uint64_t *bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// All of this thread's cp.async have landed.
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Bounded wait, about a second. Short on purpose: instruction fetch bounds this kernel's
 // single-thread roles, because all roles' code competes for the SM's instruction caches (with
 // longer waits and every loop unrolled, 200 KB of it, a wait already satisfied took 350 cycles).
@@ -199,11 +221,13 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
-  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(p));
   return p != 0;
 }
 __device__ __forceinline__ void mbar_arrive_n(uint64_t *bar, uint32_t n) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n)
+               : "memory");
 }
 // D[128 x 128] (+)= A (bf16 in TMEM, 8 columns per 16 keys) . B (shared memory)
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
@@ -302,14 +326,12 @@ struct Walk {
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(ca::kThreads, 1) 
+// kTwo: the weights go as two bf16 terms and the second product runs twice.
+template <typename T, bool kTwo>
+__global__ void __launch_bounds__(ca::kThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_q, const ChunkArgs a) {
   using namespace ca;
-  // fp16 results keep 11 bits, so their weights go as two bf16 terms and the second product runs
-  // twice (for bf16 results the weights' 8 bits stay below the output's own rounding)
-  constexpr bool kTwo = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~uintptr_t(1023));
@@ -1128,7 +1150,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
         for (int i = max(0, kt - kStages); i < kt; ++i)
           mbar_drain(vwarp ? &vland[i % kStages] : &full[i % kStages], (i / kStages) & 1);
       if (vwarp && np > 0) mbar_drain(qfull, (np - 1) & 1);
-      cp_wait<0>();
+      cp_wait_all();
     }
   }
   tc_fence_before();
@@ -1180,7 +1202,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
       for (int x = 0; x < nb; ++x) {
         const float wx = __shfl_sync(0xffffffffu, w, x);
         if (wx == 0.0f) continue;
-        const float4 v = *reinterpret_cast<const float4 *>(a.po + slot(b + x) * slot_o + r * kHd + 4 * lane);
+        const float4 v = *reinterpret_cast<const float4 *>(a.po + slot(b + x) * slot_o + r * kHd +
+                                                            4 * lane);
         o[0] += wx * v.x;
         o[1] += wx * v.y;
         o[2] += wx * v.z;
@@ -1211,6 +1234,14 @@ int make_map_q(CUtensorMap *map, const int8_t *q, int T, int Hq, int G, int TA) 
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? S8B_OK : S8B_ERR_ALIGN;
+}
+
+template <typename T, bool kTwo>
+cudaError_t launch_attn(int ctas, cudaStream_t st, const CUtensorMap &map_k,
+                        const CUtensorMap &map_q, const ChunkArgs &a) {
+  ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T, kTwo>), ca::kSmem);
+  return launch_pdl(chunk_attn_kernel<T, kTwo>, dim3(ctas), dim3(ca::kThreads), ca::kSmem, st,
+                    map_k, map_q, a);
 }
 
 int chunk_ctas() { return min(sm_count(), ca::kMaxCtas); }
@@ -1290,14 +1321,21 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
   if (const int rc = make_map_q(&map_q, q_i8, T_, Hq, a.G, a.TA)) return rc;
   a.copies = block_size >= 8 && aligned(ks, 16) && aligned(vs, 16) && rows < (1ull << 31);
   if (a.copies) {
-    const int rc = make_map_2d(&map_k, kc, kHd, rows, kHd, kHd, block_size < kKeys ? block_size : kKeys);
+    const int rc =
+        make_map_2d(&map_k, kc, kHd, rows, kHd, kHd, block_size < kKeys ? block_size : kKeys);
     if (rc) return rc;
   }
   S8B_DISPATCH_DTYPE(dtype, T, {
-    ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T>), kSmem);
-    cudaError_t e = launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(kThreads), kSmem, st, map_k, map_q, a);
+    // Two terms for fp16 results, which keep three bits more than one term has; and where a table
+    // reaches so few keys that one weight's rounding shows in a row (5 rows over 37 keys: error
+    // against 64 bits 2.8e-3 with one term, 1.6e-3 with two, the time is latency either way;
+    // 4096 rows over 16K keys would take 1284 us for 1174).
+    cudaError_t e = std::is_same<T, __half>::value || a.cap <= kFewKeys
+                        ? launch_attn<T, true>(ctas, st, map_k, map_q, a)
+                        : launch_attn<__nv_bfloat16, false>(ctas, st, map_k, map_q, a);
     if (e == cudaSuccess)
-      e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, kMergeGroups), dim3(kMergeWarps * 32), 0, st, a);
+      e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, kMergeGroups), dim3(kMergeWarps * 32), 0,
+                     st, a);
     if (e != cudaSuccess) {
       record_cuda_error(e);
       return S8B_ERR_CUDA;

@@ -1,7 +1,7 @@
 // W8A8 linear layer with its epilogue: y = act((xq . w^T) * xs * ws + bias) + residual, for
 // any token count (s8b_linear_w8a8).
 //
-// Two forms, by the token count (see linear_rows_max below):
+// Two forms, by the token count (few_rows below):
 //  * few rows: the weights are the whole cost (1 byte read per 2 M operations), so the decode
 //    GEMM of gemm_tc.cu streams them with its K range split over CTAs, its int32 partials stay
 //    in L2, and linear_epilogue_kernel sums, scales and finishes them;
@@ -15,6 +15,13 @@
 // it. The int32 sums are exact; the scales are two rounded binary32 products in the order of
 // the framework's other GEMMs, so without bias, activation and residual the result equals
 // s8b_gemm_w8a8's bit for bit. All later steps stay in binary32 and the output is rounded once.
+//
+// Measured (GPU time in a graph, beside the floor): 8 x 4096 x 4096 with residual 7.9 us (2.6 at
+// the copy rate; two launches that overlap. One, with the sums joined over a cluster and the
+// epilogue there, took 9 to 10 us: it cannot start before the slowest CTA of a cluster);
+// 4096 x 4096 x 4096 with bias and residual 74 us, 1.86 Pop/s; 8192 x 12288 x 4096 with SiLU 345
+// us, 2.39 Pop/s; 999 x 5127 x 1040 with bias and GELU 29.8 us (6.5). The large ones are bound by
+// the operands' way from L2: 128 x 256 tiles ask it for some 94 bytes per SM and cycle.
 //
 // The epilogue turns 32 rows x 16 columns of a warp at a time through shared memory: TMEM
 // hands a lane one row, while global memory wants neighbouring lanes on neighbouring columns

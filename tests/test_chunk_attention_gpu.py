@@ -74,14 +74,14 @@ class Case:
             r0 += n
         return o, A
 
-    def check(self, out, rows=None):
+    def check(self, out, rows=None, weights=2 ** -8):
         o, A = self.exact()
         out = out[:self.T].view(self.T, self.Hq, 128)
         # below a type's normal range its steps are those of the range's lower end: 2^-24 in fp16
         # (a value that ought to be 1e-15 becomes 0), so half a step is 2^-25 there; bf16 has
         # binary32's range
         least = 2.0 ** -25 if out.dtype == torch.float16 else 1e-30
-        tol = (2 ** -8 + 2e-4) * A + torch.finfo(out.dtype).eps / 2 * o.abs() + least
+        tol = (weights + 2e-4) * A + torch.finfo(out.dtype).eps / 2 * o.abs() + least
         bad = ~((out.double() - o).abs() <= tol)
         if rows is not None:
             bad = bad[rows]
@@ -317,3 +317,23 @@ def test_bad_pages_and_lengths_are_reported():
     assert status(cu=i32(8, 4, 16))[0] == -8
     assert status()[0] == 0
     assert _lib.strerror(-8) == "null pointer or invalid argument"
+
+
+@pytest.mark.parametrize("lens,dtype", [
+    ([(5, 37)], torch.bfloat16), ([(1, 1), (256, 256), (7, 200)], torch.bfloat16),
+    ([(40, 129), (3, 3)], torch.float16), ([(130, 700)], torch.float16),
+])
+def test_weights_of_two_terms(lens, dtype):
+    """Tables of up to 256 keys, and fp16 results at any length: a weight is p1 + p2 in bf16, p2 what
+    rounding to p1 left over (at most 2^-8 of it), itself off by at most 2^-8: 2^-16 in all."""
+    c = Case(lens, 8, 2, 16)
+    assert dtype == torch.float16 or c.bt.shape[1] * c.bs <= 256
+    c.check(c.run(dtype=dtype), weights=2 ** -16)
+
+
+def test_tables_on_both_sides_of_256_keys():
+    """The same context behind a table of 256 and of 272 positions."""
+    for extra in (0, 1):
+        c = Case([(33, 250)], 4, 2, 16, seed=9, extra=extra)
+        assert c.bt.shape[1] == 16 + extra
+        c.check(c.run())
