@@ -67,6 +67,10 @@ constexpr int kMaxSeqs = 1024;
 constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4;
 constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
 constexpr int kItemRows = 2 * kRows;
+// What an item costs beside its key tiles (queries, the softmax's start, its result), in tiles:
+// it counts so many units more, before its first key tile. Eight prompts' CTAs with 6 and 18
+// items took 500,000 and 660,000 cycles for as many key tiles.
+constexpr int kItemUnits = 3;
 constexpr float kSumMax = 0x1p60f;  // a tile's sum of e^(t - reference) above: a new reference
 constexpr int kFewKeys = 256;     // contexts up to which bf16 results' weights have two terms
 constexpr int kMaxCtas = 512;     // CTAs the workspace has room for
@@ -89,7 +93,7 @@ struct ChunkArgs {
   void *out;
   uint8_t *ws;
   float *ml, *po;
-  int T, S, Hq, Hkv, G, TA, bs_log2, max_blocks, num_blocks;
+  int T, S, Hq, Hkv, G, TA, TN, bs_log2, max_blocks, num_blocks;
   int cap;     // positions that a block-table row reaches
   int copies;  // pages go by bulk copies
   float c;     // scale * log2(e)
@@ -262,7 +266,8 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t x) {
 }
 
 // ---------------------------------------------------------------------- the work list ----
-// Item (sequence, kv head, tile of 2 TA tokens). units = its key tiles, at least one.
+// Item (sequence, kv head, tile of 2 TA tokens). units = kItemUnits and its key tiles, at least
+// one. A cut among an item's first units is moved to its start, so that no piece is without keys.
 struct SeqTab {
   const long long *pre;  // [S + 1] units before each sequence
   const int *cu, *ctx;
@@ -279,8 +284,18 @@ __device__ __forceinline__ Item item_at(const SeqTab &q, const ChunkArgs &a, int
   it.base = q.ctx[s] - n + i0;
   it.keys = min(max(it.base + it.ntok, 0), cap);
   it.nk = (it.keys + ca::kKeys - 1) / ca::kKeys;
-  it.units = max(it.nk, 1);
+  it.units = ca::kItemUnits + max(it.nk, 1);
   return it;
+}
+// Row rr of a 128-row tile -> its token (of the tile) and head (of the kv head's); false: none.
+// Usually token by token. An item of up to 32 / G tokens is narrow: each softmax warp gets up to
+// 8 rows of it, its first ones, a quarter of a warp's work (see the softmax).
+__device__ __forceinline__ bool place(const ChunkArgs &a, int ntok, int rr, int *tok, int *head) {
+  const bool narrow = ntok <= 4 * a.TN;
+  const int i = narrow ? rr & 31 : rr, t = i / a.G;
+  *head = i - t * a.G;
+  *tok = narrow ? (rr >> 5) * a.TN + t : t;
+  return t < (narrow ? a.TN : a.TA);
 }
 // Tiles of sequence s (none if it brings no row, or its range is no range).
 __device__ __forceinline__ int tiles_of(const SeqTab &q, const ChunkArgs &a, int s) {
@@ -309,8 +324,8 @@ struct Walk {
     p->ntok = it.ntok;
     p->base = it.base;
     p->keys = it.keys;
-    p->k0 = off;
-    p->k1 = min(off + take, it.nk);
+    p->k0 = max(off - ca::kItemUnits, 0);
+    p->k1 = min(off + take - ca::kItemUnits, it.nk);
     p->starts = off == 0;
     p->ends = off + take == it.units;
     p->behind = it.units - (off + take);
@@ -330,7 +345,8 @@ struct Walk {
 template <typename T, bool kTwo>
 __global__ void __launch_bounds__(ca::kThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_q, const ChunkArgs a) {
+                      const __grid_constant__ CUtensorMap map_q,
+                      const __grid_constant__ CUtensorMap map_qn, const ChunkArgs a) {
   using namespace ca;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -352,6 +368,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
   uint32_t *tmem_base = reinterpret_cast<uint32_t *>(drained + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base + 1);
   int *first = reinterpret_cast<int *>(tmem_base + 2);  // s, g, t, off of this CTA's run
+  long long *run = reinterpret_cast<long long *>(sm + kOffBar + 448);  // its units: begin, end
+  int *in_seq = reinterpret_cast<int *>(run + 2);                       // their sequences
   Piece *pieces = reinterpret_cast<Piece *>(sm + kOffBar + 512);
   static_assert(kPieces * sizeof(Piece) <= 512, "the ring of pieces fits its 512 bytes");
   float *bsum = reinterpret_cast<float *>(sm + kOffSums);  // [128] reference, sum of B's rows
@@ -460,22 +478,25 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
   const long long ctas = min(static_cast<long long>(gridDim.x), W);  // CTAs with work
   const long long u0 = blockIdx.x < ctas ? blockIdx.x * W / ctas : 0;
   const long long u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * W / ctas : 0;
-  if (u1 > u0) {
+  if (threadIdx.x < 2) run[threadIdx.x] = threadIdx.x ? u1 : u0;
 #pragma unroll 1
-    for (int s = threadIdx.x; s < S; s += kThreads)
-      if (pre[s] <= u0 && u0 < pre[s + 1]) first[0] = s;
+  for (int s = threadIdx.x; s < S; s += kThreads) {
+    if (pre[s] <= u0 && u0 < pre[s + 1]) in_seq[0] = s;
+    if (pre[s] <= u1 && u1 < pre[s + 1]) in_seq[1] = s;
   }
   __syncthreads();
-  if (warp == 0 && u1 > u0) {
-    const int s = first[0];
-    const long long per = (pre[s + 1] - pre[s]) / a.Hkv, rem = u0 - pre[s];
+  // Warp 0 finds the item of unit u0, warp 1 that of u1 (none behind the last unit).
+  if (warp < 2 && u1 > u0 && (warp ? u1 : u0) < W) {
+    const long long u = warp ? u1 : u0;
+    const int s = in_seq[warp];
+    const long long per = (pre[s + 1] - pre[s]) / a.Hkv, rem = u - pre[s];
     const int g = static_cast<int>(rem / per);
-    long long r = rem - g * per;  // units of this head before the run
+    long long r = rem - g * per;  // units of this head before u
     int t0 = 0;
     const int nt = tiles_of(tab, a, s);
     while (true) {
-      const int u = t0 + lane < nt ? item_at(tab, a, s, t0 + lane).units : 0;
-      long long v = u;
+      const int n = t0 + lane < nt ? item_at(tab, a, s, t0 + lane).units : 0;
+      long long v = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long x = __shfl_up_sync(0xffffffffu, v, o);
@@ -484,15 +505,23 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       const uint32_t hit = __ballot_sync(0xffffffffu, v > r);
       if (hit) {
         if (lane == __ffs(hit) - 1) {
-          first[1] = g;
-          first[2] = t0 + lane;
-          first[3] = static_cast<int>(r - (v - u));
+          int off = static_cast<int>(r - (v - n));
+          if (off <= kItemUnits) {
+            run[warp] = u - off;
+            off = 0;
+          }
+          if (warp == 0) {
+            first[0] = s;
+            first[1] = g;
+            first[2] = t0 + lane;
+            first[3] = off;
+          }
         }
         break;
       }
       r -= __shfl_sync(0xffffffffu, v, 31);
       t0 += 32;
-      if (t0 >= nt) break;  // not reached: the units of the sequence hold u0
+      if (t0 >= nt) break;  // not reached: the units of the sequence hold u
     }
   }
   if (threadIdx.x == 0) meta[blockIdx.x].valid = 0;
@@ -534,13 +563,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     while (const Piece *pc = next()) {
       const bool split = pc->ntok <= a.TA;  // one tile of rows: the groups share its key tiles
       const int tok0 = split ? 0 : hf * a.TA;
-      auto q_row = [&](int rr) {  // tile row -> row of q (valid rows)
-        const int tok = rr / a.G;
-        return static_cast<size_t>(pc->t0 + tok0 + tok) * a.Hq + pc->g * a.G + (rr - tok * a.G);
-      };
-      auto is_row = [&](int rr) {
-        const int tok = rr / a.G;
-        return tok < a.TA && tok0 + tok < pc->ntok;
+      const bool narrow = pc->ntok <= 4 * a.TN;
+      auto q_row = [&](int tok, int head) {
+        return static_cast<size_t>(pc->t0 + tok0 + tok) * a.Hq + pc->g * a.G + head;
       };
       float c[4], mr[4], l[4];  // log2(e) scale q_s, reference (a power of 2), sum of own keys
       int lim[4];               // keys the row sees (rows of no token: all, they mask no tile)
@@ -549,9 +574,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int rr = 32 * (warp & 3) + (lane >> 2) + 8 * j;
-        const bool valid = is_row(rr);
-        c[j] = valid ? a.qs[q_row(rr)] * a.c : 0.0f;
-        lim[j] = valid ? min(max(pc->base + tok0 + rr / a.G + 1, 0), pc->keys) : pc->keys;
+        int tok, head;
+        const bool valid = place(a, pc->ntok, rr, &tok, &head) && tok0 + tok < pc->ntok;
+        c[j] = valid ? a.qs[q_row(tok, head)] * a.c : 0.0f;
+        lim[j] = valid ? min(max(pc->base + tok0 + tok + 1, 0), pc->keys) : pc->keys;
         mr[j] = -INFINITY;
         l[j] = 0.0f;
         least = min(least, lim[j]);
@@ -580,33 +606,35 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
           // magnitude, so the reference has to be near the row's maximum, not at it, and the sum
           // of these keys alone shows whether it still is. Returns whether it was (else nothing
           // has been written).
-          auto put = [&](const uint32_t (&pk)[2][16], const uint32_t (&pl)[2][16]) {
+          auto put = [&](const uint32_t (&pk)[2][16], const uint32_t (&pl)[2][16], auto low) {
             tmem_st_16x128_x8(tu, pk[0]);
-            tmem_st_16x128_x8(tu + kLow, pk[1]);
+            if constexpr (decltype(low)::value) tmem_st_16x128_x8(tu + kLow, pk[1]);
             if constexpr (kTwo) {
               tmem_st_16x128_x8(tu + 32, pl[0]);
-              tmem_st_16x128_x8(tu + 32 + kLow, pl[1]);
+              if constexpr (decltype(low)::value) tmem_st_16x128_x8(tu + 32 + kLow, pl[1]);
             }
           };
-          auto pass = [&](auto masked) -> bool {
-            float2 sum[4];
+          auto pass = [&](auto masked, auto all) -> bool {
+            constexpr bool kAll = decltype(all)::value;
+            constexpr int J = kAll ? 4 : 1;  // rows of a lane (narrow: the warp's first 8 rows)
+            float2 sum[J];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
-            uint32_t v[2][2][16], pk[2][16], pl[2][16];
+            for (int j = 0; j < J; ++j) sum[j] = make_float2(0.0f, 0.0f);
+            uint32_t v[2][2][16], pk[2][16] = {}, pl[2][16] = {};
             tmem_ld_16x256_x4(tu, v[0][0]);
-            tmem_ld_16x256_x4(tu + kLow, v[0][1]);
+            if constexpr (kAll) tmem_ld_16x256_x4(tu + kLow, v[0][1]);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               tmem_wait_ld();
               if (b == 0) {
                 tmem_ld_16x256_x4(tu + 32, v[1][0]);
-                tmem_ld_16x256_x4(tu + kLow + 32, v[1][1]);
+                if constexpr (kAll) tmem_ld_16x256_x4(tu + kLow + 32, v[1][1]);
               }
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 const float2 kf = ks[16 * b + 4 * q], vf = vs[16 * b + 4 * q];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < J; ++j) {
                   const int *s = reinterpret_cast<const int *>(v[b][j >> 1]) + 4 * q + 2 * (j & 1);
                   const float2 x =
                       mul2(make_float2(static_cast<float>(s[0]), static_cast<float>(s[1])), kf);
@@ -628,14 +656,14 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
             }
             bool fits = true;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < J; ++j) {
               sum[j].x += sum[j].y;
               fits = fits && sum[j].x < kSumMax;
             }
             if (!__all_sync(0xffffffffu, fits)) return false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) l[j] += sum[j].x;
-            put(pk, pl);
+            for (int j = 0; j < J; ++j) l[j] += sum[j].x;
+            put(pk, pl, all);
             return true;
           };
           const bool masked = k >= whole_tiles;
@@ -656,7 +684,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                 mr[j] = c[j] * fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
               }
             }
-            fine = masked ? pass(std::true_type{}) : pass(std::false_type{});
+            const std::true_type yes{};
+            const std::false_type no{};
+            fine = narrow ? (masked ? pass(yes, no) : pass(no, no))
+                          : (masked ? pass(yes, yes) : pass(no, yes));
             if (fresh && !fine)
 #pragma unroll
               for (int j = 0; j < 4; ++j) mr[j] = -INFINITY;
@@ -743,7 +774,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                 }
               }
             }
-            put(pk, pl);
+            put(pk, pl, std::true_type{});
           }
           tmem_wait_st();
           tc_fence_before();
@@ -802,10 +833,12 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       }
       if (split ? hf == 0 : pc->ntok > hf * a.TA) {
         const bool whole = pc->starts && pc->ends;
-        const bool valid = is_row(row), join = split && k1 > k0 + 1;
+        int tok, head;
+        const bool valid = place(a, pc->ntok, row, &tok, &head) && tok0 + tok < pc->ntok;
+        const bool join = split && k1 > k0 + 1;
         const int slot = 2 * blockIdx.x + (pc->starts ? 1 : 0);
         const float inv = 1.0f / lr;  // not used where lr is 0
-        T *orow = static_cast<T *>(a.out) + (valid ? q_row(row) : 0) * kHd;
+        T *orow = static_cast<T *>(a.out) + (valid ? q_row(tok, head) : 0) * kHd;
         float *prow = a.po + slot * slot_o + ((tok0 ? kRows : 0) + row) * kHd;
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
@@ -1018,7 +1051,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       w.g = first[1];
       w.t = first[2];
       w.off = first[3];
-      w.left = static_cast<int>(u1 - u0);
+      w.left = static_cast<int>(run[1] - run[0]);
       int kt = 0, np = 0;
       bool ok = true;
       while (true) {
@@ -1038,7 +1071,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
               me.t0 = p->t0;
               me.ntok = p->ntok;
               me.g = p->g;
-              me.last = static_cast<int>(((u1 + p->behind) * ctas - 1) / W);
+              me.last = static_cast<int>(((run[1] + p->behind) * ctas - 1) / W);
               me.valid = 1;
             }
             mbar_arrive(&afull[na % kPieces]);
@@ -1051,13 +1084,20 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
         const int32_t *bt = a.bt + static_cast<size_t>(pc->s) * a.max_blocks;
         const int keys = pc->keys, g = pc->g, k0 = pc->k0, k1 = pc->k1;
         if (vwarp) {
-          const int t0 = pc->t0, both = pc->ntok > a.TA;
+          const int t0 = pc->t0, ntok = pc->ntok, both = ntok > a.TA;
           done();
           if (k1 > k0) {
             // a tile's rows are TA tokens x G heads, which one box of the queries holds in order
             ok = bar_wait(qempty, (np & 1) ^ 1, abort_flag, status);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
-            if (lane == 0) {
+            if (ntok <= 4 * a.TN) {  // narrow: TN tokens at the first rows of each softmax warp
+              if (lane == 0) {
+                const int warps = (ntok + a.TN - 1) / a.TN;
+                mbar_expect_tx(qfull, warps * a.TN * a.G * kHd);
+                for (int i = 0; i < warps; ++i)
+                  tma_load_3d(sm + kOffQ + i * 32 * kHd, &map_qn, 0, g * a.G, t0 + i * a.TN, qfull);
+              }
+            } else if (lane == 0) {
               mbar_expect_tx(qfull, (1 + both) * a.TA * a.G * kHd);
               tma_load_3d(sm + kOffQ, &map_q, 0, g * a.G, t0, qfull);
               if (both) tma_load_3d(sm + kOffQ + kTile, &map_q, 0, g * a.G, t0 + a.TA, qfull);
@@ -1177,8 +1217,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
   const int c0 = blockIdx.x, n = me.last - c0 + 1;
   auto slot = [&](int i) { return static_cast<size_t>(2 * (c0 + i) + (i == 0)); };
   for (int r = blockIdx.y * kMergeWarps + warp; r < kItemRows; r += gridDim.y * kMergeWarps) {
-    const int hf = r >> 7, rr = r & 127, tok = rr / a.G, i = hf * a.TA + tok;
-    if (tok >= a.TA || i >= me.ntok) continue;
+    int tok, head;
+    const bool is = place(a, me.ntok, r & 127, &tok, &head);
+    const int i = (r >> 7) * a.TA + tok;
+    if (!is || i >= me.ntok) continue;
     float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int b = 0; b < n; b += 32) {
       float mi = -INFINITY, li = 0.0f;
@@ -1216,7 +1258,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
     for (int x = 0; x < 4; ++x) t[x] = from_f32<T>(l == 0.0f ? 0.0f : o[x] * inv);
     uint2 raw;
     memcpy(&raw, t, 8);
-    const size_t qrow = static_cast<size_t>(me.t0 + i) * a.Hq + me.g * a.G + (rr - tok * a.G);
+    const size_t qrow = static_cast<size_t>(me.t0 + i) * a.Hq + me.g * a.G + head;
     *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + qrow * kHd + 4 * lane) = raw;
   }
 }
@@ -1238,10 +1280,11 @@ int make_map_q(CUtensorMap *map, const int8_t *q, int T, int Hq, int G, int TA) 
 
 template <typename T, bool kTwo>
 cudaError_t launch_attn(int ctas, cudaStream_t st, const CUtensorMap &map_k,
-                        const CUtensorMap &map_q, const ChunkArgs &a) {
+                        const CUtensorMap &map_q, const CUtensorMap &map_qn,
+                        const ChunkArgs &a) {
   ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T, kTwo>), ca::kSmem);
   return launch_pdl(chunk_attn_kernel<T, kTwo>, dim3(ctas), dim3(ca::kThreads), ca::kSmem, st,
-                    map_k, map_q, a);
+                    map_k, map_q, map_qn, a);
 }
 
 int chunk_ctas() { return min(sm_count(), ca::kMaxCtas); }
@@ -1306,6 +1349,7 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
   a.Hkv = Hkv;
   a.G = Hq / Hkv;
   a.TA = kRows / a.G;
+  a.TN = a.G <= 8 ? 8 / a.G : 0;
   a.bs_log2 = bs_log2;
   a.max_blocks = max_blocks;
   a.num_blocks = num_blocks;
@@ -1316,9 +1360,12 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
   // bulk copies want 16-byte boundaries, the tensor copy whole 8-row swizzle atoms and row
   // numbers below 2^31
   const unsigned long long rows = static_cast<unsigned long long>(num_blocks) * Hkv * block_size;
-  CUtensorMap map_k, map_q;
+  CUtensorMap map_k, map_q, map_qn;
   memset(&map_k, 0, sizeof(map_k));
   if (const int rc = make_map_q(&map_q, q_i8, T_, Hq, a.G, a.TA)) return rc;
+  map_qn = map_q;
+  if (a.TN > 0)
+    if (const int rc = make_map_q(&map_qn, q_i8, T_, Hq, a.G, a.TN)) return rc;
   a.copies = block_size >= 8 && aligned(ks, 16) && aligned(vs, 16) && rows < (1ull << 31);
   if (a.copies) {
     const int rc =
@@ -1331,8 +1378,8 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
     // against 64 bits 2.8e-3 with one term, 1.6e-3 with two, the time is latency either way;
     // 4096 rows over 16K keys would take 1284 us for 1174).
     cudaError_t e = std::is_same<T, __half>::value || a.cap <= kFewKeys
-                        ? launch_attn<T, true>(ctas, st, map_k, map_q, a)
-                        : launch_attn<__nv_bfloat16, false>(ctas, st, map_k, map_q, a);
+                        ? launch_attn<T, true>(ctas, st, map_k, map_q, map_qn, a)
+                        : launch_attn<__nv_bfloat16, false>(ctas, st, map_k, map_q, map_qn, a);
     if (e == cudaSuccess)
       e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, kMergeGroups), dim3(kMergeWarps * 32), 0,
                      st, a);
