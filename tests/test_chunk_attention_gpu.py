@@ -337,3 +337,23 @@ def test_tables_on_both_sides_of_256_keys():
         c = Case([(33, 250)], 4, 2, 16, seed=9, extra=extra)
         assert c.bt.shape[1] == 16 + extra
         c.check(c.run())
+
+
+@pytest.mark.parametrize("Hq,Hkv,edge", [(4, 4, 32), (8, 4, 16), (6, 2, 8), (8, 2, 8), (10, 2, 4),
+                                         (8, 1, 4), (9, 1, 0)])
+def test_items_of_few_tokens(Hq, Hkv, edge):
+    """On both sides of 32 / G tokens (each softmax warp has 8 rows, 8 / G whole tokens), alone and
+    as a long sequence's rest, in one piece and cut over CTAs."""
+    G = Hq // Hkv
+    whole = 2 * (128 // G)
+    lens = [(max(edge, 1), 70), (edge + 1, 300), (max(edge - 1, 1), 2000), (1, 1),
+            (whole + max(edge, 1), whole + 150), (whole + edge + 1, whole + 400), (2, 5000)]
+    c = Case(lens, Hq, Hkv, 16, seed=Hq)
+    c.check(c.run())
+    c.check(c.run(dtype=torch.float16), weights=2 ** -16)
+
+
+def test_cuts_next_to_an_items_start():
+    """Many items of one and two key tiles: cuts fall before, among and behind their first units."""
+    c = Case([(1 + i % 5, 1 + 37 * i % 260 + 5) for i in range(70)], 8, 4, 16, seed=4)
+    c.check(c.run())
