@@ -16,12 +16,14 @@
 // Bound. Each score (row x key) costs 2 x 128 int8 and 2 x 128 bf16 operations, one exponential
 // and about 5 further instructions; a key's bytes serve 128 rows. Above some 16 rows per sequence
 // the bf16 product sets the floor (1635 TFLOP/s measured), below it the keys' 264 bytes per head.
-// What bounds the kernel is the softmax warps' instruction issue: a step of 64 keys takes its
-// group 850 cycles alone and 1270 beside the other group, against 512 of tensor work for both.
-// Measured (GPU time in a graph, beside the floor): 4096 new rows over 16K keys, 32 heads on 4,
-// 1284 us in fp16 and 1174 in bf16 (589 at the tensor rate); eight prompts of up to 2048 rows, 32
-// on 8, 364 us (102); 64 sequences x up to 4 draft rows over up to 2048 keys 108 us (27 at the
-// copy rate); 2 sequences x 16 rows over 64K keys, 40 on 8, 73 us (21); 5 rows 15 us.
+// What bounds the kernel is the chain from S to P: a step of 64 keys takes a softmax group 850
+// cycles alone, 1270 beside the other group and about 1900 beside the converters too, against
+// 512 of tensor work for both groups (issue slots 44%, tensor pipe 20% busy); with few rows the
+// conversion of V, 2000 of the 2500 cycles of a tile of 128 keys. An item costs 12,000 to 15,000
+// cycles beside its tiles. Measured (GPU time in a graph, beside the floor): 4096 new rows over
+// 16K keys, 32 heads on 4, 1310 us in fp16 (589 at the tensor rate); eight prompts of up to 2048
+// rows, 32 on 8, 355 us (102); 64 sequences x up to 4 draft rows over up to 2048 keys 98 us (27
+// at the copy rate); 2 sequences x 16 rows over 64K keys, 40 on 8, 70 us (21); 5 rows 15 us.
 //
 // Unit of work. The G query heads of a kv head share its keys, so a tile's 128 rows are
 // 128 / G tokens x G heads, and an item is two such tiles (A and B) of one sequence and kv head:
@@ -68,8 +70,9 @@ constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4
 constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
 constexpr int kItemRows = 2 * kRows;
 // What an item costs beside its key tiles (queries, the softmax's start, its result), in tiles:
-// it counts so many units more, before its first key tile. Eight prompts' CTAs with 6 and 18
-// items took 500,000 and 660,000 cycles for as many key tiles.
+// it counts so many units more, before its first key tile. Uncounted, eight prompts' CTAs with 6
+// and 18 items took 500,000 and 660,000 cycles for as many key tiles: 380 us, with 3 units 355,
+// with 5 374 (64 sequences of 4 draft rows: 101, 98, 97).
 constexpr int kItemUnits = 3;
 constexpr float kSumMax = 0x1p60f;  // a tile's sum of e^(t - reference) above: a new reference
 constexpr int kFewKeys = 256;     // contexts up to which bf16 results' weights have two terms
