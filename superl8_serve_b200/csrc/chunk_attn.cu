@@ -19,10 +19,9 @@
 // What bounds the kernel is the chain from S to P: a step of 64 keys takes a softmax group 850
 // cycles alone, 1270 beside the other group and about 1900 beside the converters too, against
 // 512 of tensor work for both groups (issue slots 44%, tensor pipe 20% busy); with few rows the
-// conversion of V, 2000 of the 2500 cycles of a tile of 128 keys. An item costs 12,000 to 15,000
-// cycles beside its tiles. Measured (GPU time in a graph, beside the floor): 4096 new rows over
+// conversion of V, 2000 of the 2500 cycles of a tile of 128 keys. Measured (GPU time in a graph, beside the floor): 4096 new rows over
 // 16K keys, 32 heads on 4, 1310 us in fp16 (589 at the tensor rate); eight prompts of up to 2048
-// rows, 32 on 8, 355 us (102); 64 sequences x up to 4 draft rows over up to 2048 keys 98 us (27
+// rows, 32 on 8, 353 us (102); 64 sequences x up to 4 draft rows over up to 2048 keys 84 us (27
 // at the copy rate); 2 sequences x 16 rows over 64K keys, 40 on 8, 70 us (21); 5 rows 15 us.
 //
 // Unit of work. The G query heads of a kv head share its keys, so a tile's 128 rows are
@@ -368,7 +367,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
   uint64_t *afull = btaken + 1;        // [4] piece announced
   uint64_t *aempty = afull + kPieces;  // [4] piece done by every other role's warp
   uint64_t *qfull = aempty + kPieces, *qempty = qfull + 1, *drained = qempty + 1;
-  uint32_t *tmem_base = reinterpret_cast<uint32_t *>(drained + 2);
+  uint64_t *pdone = drained + 2;  // a piece's products done by both groups
+  uint32_t *tmem_base = reinterpret_cast<uint32_t *>(pdone + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base + 1);
   int *first = reinterpret_cast<int *>(tmem_base + 2);  // s, g, t, off of this CTA's run
   long long *run = reinterpret_cast<long long *>(sm + kOffBar + 448);  // its units: begin, end
@@ -413,6 +413,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     }
     mbar_init(qfull, 1);
     mbar_init(qempty, 2);
+    mbar_init(pdone, 2);
     mbar_init(&drained[0], 1);
     mbar_init(&drained[1], 1);
     *abort_flag = 0;
@@ -1001,6 +1002,14 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
           }
           __syncwarp();
         }
+        // After this group's last scores the next piece's queries may come (released after the
+        // products, they held up V's pages too: 98 us, not 84, for 64 sequences of 4 draft rows
+        // over 2K keys). The products begin when
+        // both groups' of the piece before have ended: a group that had no tile there would
+        // otherwise wait for a bf16 V buffer two fills ahead, and a parity tells only one.
+        if (lead && i + step >= n) mma_commit(qempty);
+        __syncwarp();
+        if (np > 1 && !wait(pdone, np & 1)) break;
 #pragma unroll 1
         for (uint32_t acc = 0; ok && i < n; i += step, ++nt) {
           const int j = kt + i, vb = j & 1;
@@ -1025,6 +1034,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
               mma_commit(&pvin[2 * hf + h]);
               if (more) scores(j + step, h);
               if (h == 1) {
+                if (more && i + 2 * step >= n) mma_commit(qempty);
                 mma_commit(&vempty[vb]);
                 if (split) mma_commit(&vempty[vb]);
                 if (!more) mma_commit(&ofull[hf]);
@@ -1035,7 +1045,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
           }
         }
         if (!ok) break;
-        if (lead) mma_commit(qempty);
+        if (lead) mma_commit(pdone);
         __syncwarp();
         kt += n;
       }
