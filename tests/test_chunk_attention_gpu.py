@@ -357,3 +357,17 @@ def test_cuts_next_to_an_items_start():
     """Many items of one and two key tiles: cuts fall before, among and behind their first units."""
     c = Case([(1 + i % 5, 1 + 37 * i % 260 + 5) for i in range(70)], 8, 4, 16, seed=4)
     c.check(c.run())
+
+
+def test_pieces_of_one_tile_between_longer_ones():
+    """The groups of a piece of one key tile do not both work: the order between pieces has to hold
+    however the runs fall in time."""
+    from superl8_serve_b200 import ops
+
+    c = Case([(1 + (i * 7) % 40, 41 + 97 * i % 900) for i in range(60)], 8, 2, 16, seed=5)
+    ws = ops.chunk_workspace(DEV)
+    want = c.run(workspace=ws)
+    c.check(want)
+    for _ in range(50):
+        assert torch.equal(ops.paged_chunk_q8(c.q, c.qs, c.kc, c.ks, c.vc, c.vs, c.bt, c.ctx,
+                                              c.cu, c.scale, workspace=ws), want)
