@@ -55,6 +55,14 @@ constexpr int kThreads = 512;
 constexpr int kKeys = 128;        // keys per tile
 constexpr int kRows = 128;        // rows per tile
 constexpr int kStages = 3;
+// Barriers that tell of a stage's K. A parity tells only one phase from the next, so a wait for
+// tile j is right only if the barrier's last use before is known to have landed, and none after j
+// can. Where the groups share a piece's key tiles, a group waits for every second tile alone: with a
+// barrier per stage the use before tile j is tile j - 3, which the other group waited for. Six
+// barriers keep the groups apart: the use before is tile j - 6, the group's own (or of an
+// earlier piece, all of whose K has landed when the next piece's queries come), and the use
+// after waits for this group's reads of tile j.
+constexpr int kFull = 2 * kStages;
 constexpr int kTile = kKeys * kHd;                 // one int8 tile (16 KB)
 constexpr int kStage = 2 * kTile + 2 * kKeys * 4;  // K | V | ks | vs
 constexpr int kOffVs = kStages * kStage;           // V in bf16: 2 buffers of 2 panels of 64 dims
@@ -353,10 +361,10 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~uintptr_t(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(sm + kOffBar);  // [3] K and scales loaded
-  uint64_t *vland = full + 3;    // [3] V codes loaded
-  uint64_t *empty = vland + 3;   // [3] K read, V converted, scales read by both softmax groups
-  uint64_t *vfull = empty + 3;   // [2] bf16 V written
+  uint64_t *full = reinterpret_cast<uint64_t *>(sm + kOffBar);  // [6] K and scales loaded
+  uint64_t *vland = full + kFull;     // [3] V codes loaded
+  uint64_t *empty = vland + kStages;  // [3] K read, V converted, scales read by both softmax groups
+  uint64_t *vfull = empty + kStages;   // [2] bf16 V written
   uint64_t *vempty = vfull + 2;  // [2] bf16 V read
   uint64_t *sfull = vempty + 2;  // [group][half tile] S ready
   uint64_t *pfull = sfull + 4;   // [group][half tile] P written (S read, O rescaled)
@@ -390,8 +398,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 0) {
+    for (int i = 0; i < kFull; ++i) mbar_init(&full[i], a.copies ? 1 + 32 : 32);
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], a.copies ? 1 + 32 : 32);
       mbar_init(&vland[i], a.copies ? 1 : 32);
       mbar_init(&empty[i], 2 + 4 + 4 + 4);
     }
@@ -989,7 +997,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
           }
         };
         auto keys_there = [&](int j) {
-          const bool got = wait(&full[j % kStages], (j / kStages) & 1);
+          const bool got = wait(&full[j % kFull], (j / kFull) & 1);
           if (!a.copies) fence_async();  // K was written by plain copies
           return got;
         };
@@ -1145,7 +1153,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
             ok = bar_wait(&empty[st], ((kt / kStages) & 1) ^ 1, abort_flag, status);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             uint8_t *base = sm + st * kStage;
-            uint64_t *bar = vwarp ? &vland[st] : &full[st];
+            uint64_t *bar = vwarp ? &vland[st] : &full[kt % kFull];
             const int n = __popc(__ballot_sync(0xffffffffu, at >= 0));
             if (lane == 0) mbar_expect_tx(bar, n * rows * kHd);
             __syncwarp();
@@ -1193,7 +1201,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                 if (src >= 0) cp16(dst, (vwarp ? a.vc : a.kc) + src * kHd + ch * 16);
               }
             }
-            cp_arrive(vwarp ? &vland[st] : &full[st]);  // the MMA's warps fence for their proxy
+            cp_arrive(vwarp ? &vland[st] : &full[kt % kFull]);  // the MMA's warps fence for their proxy
           }
         }
         if (!ok) break;
@@ -1201,7 +1209,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       // nothing may still be on its way when the shared memory goes
       if (a.copies)
         for (int i = max(0, kt - kStages); i < kt; ++i)
-          mbar_drain(vwarp ? &vland[i % kStages] : &full[i % kStages], (i / kStages) & 1);
+          if (vwarp) mbar_drain(&vland[i % kStages], (i / kStages) & 1);
+          else mbar_drain(&full[i % kFull], (i / kFull) & 1);
       if (vwarp && np > 0) mbar_drain(qfull, (np - 1) & 1);
       cp_wait_all();
     }
