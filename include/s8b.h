@@ -279,11 +279,11 @@ int s8b_paged_prefill_q8(const int8_t *q_i8, const float *q_s, const int8_t *kc,
  * position gets zeros; rows of out [T, Hq*D] (dtype) behind cu_q[S] are left as they are.
  * cu_q [S+1] and context_lens [S] are read on the device, so a captured graph may replay with
  * other lengths; kc/vc [num_blocks, Hkv, bs, D], ks/vs [num_blocks, Hkv, bs].
- * Numerics: q.k exact, softmax in binary32, the weights e^(t - m) * vs rounded to bf16 (for fp16
- * results, and where max_blocks * block_size <= 256: to the sum of two bf16 numbers, 16 bits)
- * before the second product (binary32 sums), one rounding to dtype. Not part of the bit-exact contract of the decode and prefill entry
- * points (their weights have 15 bits relative to a partition's largest); the result is the same
- * on every run, whatever the other streams do.
+ * Numerics: q.k exact, softmax in binary32, the weights e^(t - m) * vs as the sum of two bf16
+ * numbers (16 bits) in the second product (binary32 sums), one rounding to dtype. Not part of the
+ * bit-exact contract of the decode and prefill entry points (their weights have 15 bits relative
+ * to a partition's largest); the result is the same on every run, whatever the other streams
+ * do.
  * D = 128; block_size a power of two up to 256; Hq / Hkv <= 128; S <= 1024; scale > 0. q_i8,
  * kc, vc, out 16-byte aligned. workspace: s8b_paged_chunk_workspace_size() bytes (any shape),
  * 256-byte aligned, its first 256 bytes zero-filled once. workspace[0] (int32) receives

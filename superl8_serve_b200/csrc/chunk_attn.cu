@@ -4,14 +4,16 @@
 // Sequence s brings n new rows (cu_q[s] .. cu_q[s+1]) at the end of a context of c keys; row i
 // sees keys 0 .. c - n + i. With int8 queries, keys and values,
 //   x_j = (q . k_j) ks_j,   t_j = qs scale x_j,   o = sum_j e^(t_j - m) vs_j v_j / sum_j e^(t_j - m)
-// q . k is exact (kind::i8, int32); the softmax is binary32; the products e^(..) vs_j are
-// rounded to bf16 for the second product (kind::f16 with binary32 sums), whose other operand,
-// the value codes, bf16 holds exactly. bf16 rather than fp16: its range is binary32's, so no
-// token's scale can overflow or vanish beside another's, and half a step of it (2^-9 to 2^-8)
-// on weights that are then averaged stays below the output's own rounding to bf16. fp16 results
-// keep three bits more, so their weights go as two bf16 terms, p and what rounding to p left over,
-// and the second product runs once for each (error against 64 bits 1.7e-3 -> 2.1e-4); bf16
-// results behind short tables too (see the launch).
+// q . k is exact (kind::i8, int32); the softmax is binary32; the products w_j = e^(..) vs_j go
+// into the second product (kind::f16 with binary32 sums) as the sum of two bf16 numbers, p and
+// what rounding to p left over (2^-16 of w_j at most in all), and that product runs once for
+// each; its other operand, the value codes, bf16 holds exactly. bf16 rather than fp16: its
+// range is binary32's, so no token's scale can overflow or vanish beside another's. One term alone
+// (2^-8 at most) shows beside the output's own rounding: the root of the mean square error
+// against 64 bits was 2.3e-3 for bf16 results (2.8e-3 behind 37 keys) where that rounding makes
+// 1.7e-3, and 1.7e-3 for fp16 results where it makes 2.1e-4. The second term costs 3
+// to 8 % (by the call: eight prompts of up to 2048 rows 354 -> 382 us, 64 sequences of up to 4
+// draft rows 82 -> 86, 5 rows over 37 keys nothing).
 //
 // Bound. Each score (row x key) costs 2 x 128 int8 and 2 x 128 bf16 operations, one exponential
 // and about 5 further instructions; a key's bytes serve 128 rows. Above some 16 rows per sequence
@@ -82,7 +84,6 @@ constexpr int kItemRows = 2 * kRows;
 // with 5 374 (64 sequences of 4 draft rows: 101, 98, 97).
 constexpr int kItemUnits = 3;
 constexpr float kSumMax = 0x1p60f;  // a tile's sum of e^(t - reference) above: a new reference
-constexpr int kFewKeys = 256;     // contexts up to which bf16 results' weights have two terms
 constexpr int kMaxCtas = 512;     // CTAs the workspace has room for
 // workspace: status word, per-CTA metadata, partials
 struct Meta {  // an item whose first piece is CTA c's (slot 2c + 1); pieces go on in slots 2c' + 0
@@ -351,8 +352,7 @@ struct Walk {
   }
 };
 
-// kTwo: the weights go as two bf16 terms and the second product runs twice.
-template <typename T, bool kTwo>
+template <typename T>
 __global__ void __launch_bounds__(ca::kThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_q,
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     // rows l / 4 + 8 j (j = 0..3) of its warp's 32, so that a scale read from shared memory
     // serves four rows (with a row per lane the broadcast reads alone took as long as the
     // exponentials: 512 bytes of register writes for 4 values).
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTwo ? 176 : 160));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(176));
     const int hf = warp >> 2, quad = lane & 3;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + hf * 128 + lanes, to = tmem + 256 + hf * 128 + lanes;
@@ -621,10 +621,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
           auto put = [&](const uint32_t (&pk)[2][16], const uint32_t (&pl)[2][16], auto low) {
             tmem_st_16x128_x8(tu, pk[0]);
             if constexpr (decltype(low)::value) tmem_st_16x128_x8(tu + kLow, pk[1]);
-            if constexpr (kTwo) {
-              tmem_st_16x128_x8(tu + 32, pl[0]);
-              if constexpr (decltype(low)::value) tmem_st_16x128_x8(tu + 32 + kLow, pl[1]);
-            }
+            tmem_st_16x128_x8(tu + 32, pl[0]);
+            if constexpr (decltype(low)::value) tmem_st_16x128_x8(tu + 32 + kLow, pl[1]);
           };
           auto pass = [&](auto masked, auto all) -> bool {
             constexpr bool kAll = decltype(all)::value;
@@ -660,9 +658,8 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                   }
                   sum[j] = add2(sum[j], e);
                   pk[j >> 1][8 * b + 2 * q + (j & 1)] = pack_bf16(w);
-                  if constexpr (kTwo)
-                    pl[j >> 1][8 * b + 2 * q + (j & 1)] =
-                        pack_rest(w, pk[j >> 1][8 * b + 2 * q + (j & 1)]);
+                  pl[j >> 1][8 * b + 2 * q + (j & 1)] =
+                      pack_rest(w, pk[j >> 1][8 * b + 2 * q + (j & 1)]);
                 }
               }
             }
@@ -782,7 +779,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
                   const float2 w = make_float2(s0 ? e0 * vf.x : 0.0f, s1 ? e1 * vf.y : 0.0f);
                   const int at = b / 4 + 2 * q + (j & 1);
                   pk[j >> 1][at] = pack_bf16(w);
-                  if constexpr (kTwo) pl[j >> 1][at] = pack_rest(w, pk[j >> 1][at]);
+                  pl[j >> 1][at] = pack_rest(w, pk[j >> 1][at]);
                 }
               }
             }
@@ -904,7 +901,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
     }
   } else if (warp < 12) {
     // --------------------------------------------------------------- V codes to bf16 ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTwo ? 80 : 96));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(80));
     const int ct = threadIdx.x - 256;
     const int ch = ct & 7, key0 = ct >> 3;  // 16-byte chunk, first key; keys step by 16
     int kt = 0;
@@ -953,7 +950,7 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
       done();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTwo ? 80 : 96));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(80));
     if (warp < 14) {
       // ----------------------------------------------------------------- MMA issuers ----
       // All lanes walk the tiles, one elected lane issues: descriptors then stay in uniform
@@ -1034,11 +1031,9 @@ __global__ void __launch_bounds__(ca::kThreads, 1)
 #pragma unroll
               for (int x = 1; x < 4; ++x)
                 mma_bf16_ts(tmem_o, pa + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
-              if constexpr (kTwo) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  mma_bf16_ts(tmem_o, pa + 32 + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
-              }
+              for (int x = 0; x < 4; ++x)  // the weights' second terms
+                mma_bf16_ts(tmem_o, pa + 32 + 8 * x, vd + x * (2048 >> 4), kIdescPv, 1);
               mma_commit(&pvin[2 * hf + h]);
               if (more) scores(j + step, h);
               if (h == 1) {
@@ -1300,12 +1295,12 @@ int make_map_q(CUtensorMap *map, const int8_t *q, int T, int Hq, int G, int TA) 
   return r == CUDA_SUCCESS ? S8B_OK : S8B_ERR_ALIGN;
 }
 
-template <typename T, bool kTwo>
+template <typename T>
 cudaError_t launch_attn(int ctas, cudaStream_t st, const CUtensorMap &map_k,
                         const CUtensorMap &map_q, const CUtensorMap &map_qn,
                         const ChunkArgs &a) {
-  ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T, kTwo>), ca::kSmem);
-  return launch_pdl(chunk_attn_kernel<T, kTwo>, dim3(ctas), dim3(ca::kThreads), ca::kSmem, st,
+  ensure_smem(reinterpret_cast<const void *>(chunk_attn_kernel<T>), ca::kSmem);
+  return launch_pdl(chunk_attn_kernel<T>, dim3(ctas), dim3(ca::kThreads), ca::kSmem, st,
                     map_k, map_q, map_qn, a);
 }
 
@@ -1395,13 +1390,7 @@ extern "C" int s8b_paged_chunk_q8(const int8_t *q_i8, const float *q_s, const in
     if (rc) return rc;
   }
   S8B_DISPATCH_DTYPE(dtype, T, {
-    // Two terms for fp16 results, which keep three bits more than one term has; and where a table
-    // reaches so few keys that one weight's rounding shows in a row (5 rows over 37 keys: error
-    // against 64 bits 2.8e-3 with one term, 1.6e-3 with two, the time is latency either way;
-    // 4096 rows over 16K keys would take 1284 us for 1174).
-    cudaError_t e = std::is_same<T, __half>::value || a.cap <= kFewKeys
-                        ? launch_attn<T, true>(ctas, st, map_k, map_q, map_qn, a)
-                        : launch_attn<__nv_bfloat16, false>(ctas, st, map_k, map_q, map_qn, a);
+    cudaError_t e = launch_attn<T>(ctas, st, map_k, map_q, map_qn, a);
     if (e == cudaSuccess)
       e = launch_pdl(chunk_merge_kernel<T>, dim3(ctas, kMergeGroups), dim3(kMergeWarps * 32), 0,
                      st, a);

@@ -371,3 +371,19 @@ def test_pieces_of_one_tile_between_longer_ones():
     for _ in range(50):
         assert torch.equal(ops.paged_chunk_q8(c.q, c.qs, c.kc, c.ks, c.vc, c.vs, c.bt, c.ctx,
                                               c.cu, c.scale, workspace=ws), want)
+
+
+@pytest.mark.parametrize("lens", [[(5, 37)], [(1, 1), (3, 3), (40, 41)], [(33, 250)], [(70, 2100)]])
+def test_weights_keep_16_bits_behind_any_table(lens):
+    """bf16 results too, and where rows see few of the keys that the table reaches: a weight is p1 + p2
+    in bf16, off by at most 2^-16 of it, so that the output's own rounding is what remains."""
+    for extra in (0, 1, 200):
+        c = Case(lens, 8, 2, 16, seed=71, extra=extra)
+        c.check(c.run(), weights=2 ** -16)
+
+
+def test_the_tables_width_does_not_show():
+    """The same sequences behind tables of other widths: the same bits."""
+    want = Case([(33, 250), (5, 37)], 8, 2, 16, seed=72).run()
+    for extra in (1, 2, 113):
+        assert torch.equal(Case([(33, 250), (5, 37)], 8, 2, 16, seed=72, extra=extra).run(), want)
