@@ -105,9 +105,12 @@ int s8b_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *w, const floa
  * (s8b_gemm_tc_workspace_size bytes, 256-byte aligned, zero-filled once by the caller) only
  * holds a status word: workspace[0] (int32) receives S8B_ERR_TIMEOUT if a bounded wait
  * inside the kernel gave up, after which the caller must re-zero it. The launch carries a
- * programmatic dependency on the preceding kernel in the stream (weights prefetch early;
- * activations, scales and outputs are touched only after that kernel has completed).
+ * programmatic dependency on the preceding kernel in the stream (weights prefetch early, so no
+ * kernel that may still run when it starts may write them; activations, scales and outputs are
+ * touched only after the preceding kernel has completed). S8B_GEMM_ORDERED added to out_kind
+ * (s8b_gemm_w8a8_tc only) reads the weights after that, too.
  * Replaces superl8.linear / gemm_w8a8 (superl8serve/layers/linear.py:122).               */
+#define S8B_GEMM_ORDERED 8
 size_t s8b_gemm_tc_workspace_size(int M, int N);
 /* out_kind 2 of the tensor-core GEMM: no dequantization and no reduction of the split-K
  * partial sums; y is int32 [C][M][N] with C = s8b_gemm_tc_split_count(M, N, K), and
@@ -140,7 +143,8 @@ int s8b_gemm_w8a8_tc_packed(const int8_t *xq, const float *xs, const int8_t *wpa
  * K % 16 == 0, K < 131072; xq, w 16-byte aligned, bias, residual, y 2-byte aligned (16 bytes and
  * N % 8 == 0 store vectors). workspace: s8b_linear_workspace_size bytes, 256-byte aligned, its
  * first 256 bytes zero-filled once; workspace[0] (int32) receives S8B_ERR_TIMEOUT if a bounded
- * wait gave up. Launches that share a workspace must be stream-ordered.
+ * wait gave up. Launches that share a workspace must be stream-ordered. Any argument may come
+ * from the kernel just before on the stream, the weights among them.
  * Replaces superl8.linear and the bias and residual additions around it
  * (superl8serve/layers/linear.py:122).                                                     */
 #define S8B_ACT_NONE 0

@@ -98,6 +98,7 @@ struct TcArgs {
   const float *ws;
   void *y;
   int32_t *status;  // workspace status word
+  int ordered;      // nothing is read before the preceding kernel has ended
   int out_kind, M, N, K, m0, n_tiles, kc;
   int csplit;     // CTAs sharing each tile's K range (1: no split)
   int nclusters;  // CTA groups in the grid (launched as clusters unless out_kind == 2)
@@ -251,7 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto load_b = [&](const UnitPos &u, uint8_t *sa, uint64_t *bar) {
         tma_load_2d(sa + kABytes, &tmap_x, u.kk * kBK, a.m0, bar);
       };
-      // weights of the first stages before the previous kernel has finished
+      // weights of the first stages before the previous kernel has finished (unless it, or one
+      // before it that may still be running, writes them)
+      if (a.ordered) griddep_wait();
       const int pre = n_units < S ? static_cast<int>(n_units) : S;
       UnitPos u{cid, k_lo};
       for (int i = 0; i < pre; ++i, advance(u)) {
@@ -624,7 +627,8 @@ int launch_tc(const int8_t *xq, const float *xs, const int8_t *w, const float *w
   args.ws = ws;
   args.y = y;
   args.status = static_cast<int32_t *>(workspace);
-  args.out_kind = out_kind;
+  args.out_kind = out_kind & ~S8B_GEMM_ORDERED;
+  args.ordered = (out_kind & S8B_GEMM_ORDERED) != 0;
   args.M = M;
   args.N = N;
   args.K = K;
@@ -671,8 +675,9 @@ extern "C" size_t s8b_gemm_tc_workspace_size(int M, int N) {
 extern "C" int s8b_gemm_w8a8_tc(const int8_t *xq, const float *xs, const int8_t *w,
                                 const float *ws, void *y, int out_kind, int M, int N, int K,
                                 int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  if (!xq || !w || !y || (out_kind == 0 && (!xs || !ws))) return S8B_ERR_ARG;
-  if (out_kind < 0 || out_kind > 2) return S8B_ERR_ARG;
+  const int kind = out_kind & ~S8B_GEMM_ORDERED;
+  if (!xq || !w || !y || (kind == 0 && (!xs || !ws))) return S8B_ERR_ARG;
+  if (kind < 0 || kind > 2) return S8B_ERR_ARG;
   if (M < 0 || N <= 0 || K <= 0 || K % kBK != 0) return S8B_ERR_SHAPE;
   if (!aligned(xq, 16) || !aligned(w, 16)) return S8B_ERR_ALIGN;
   if (!workspace || workspace_bytes < s8b_gemm_tc_workspace_size(M, N)) return S8B_ERR_WORKSPACE;

@@ -426,8 +426,9 @@ int launch_few(const int8_t *xq, const float *xs, const int8_t *w, const LinArgs
   const int C = s8b_gemm_tc_split_count(a.M, a.N, K);
   if (C < 1) return C;
   int32_t *part = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) + kLinHeader);
-  const int rc = s8b_gemm_w8a8_tc(xq, xs, w, nullptr, part, 2, a.M, a.N, K, dtype, workspace,
-                                  kLinHeader, stream);
+  // Ordered: the caller's weights may come from a kernel just before (quantized on this stream).
+  const int rc = s8b_gemm_w8a8_tc(xq, xs, w, nullptr, part, 2 | S8B_GEMM_ORDERED, a.M, a.N, K,
+                                  dtype, workspace, kLinHeader, stream);
   if (rc) return rc;
   const bool v4 = a.N % 4 == 0;
   const int cols = 256 * (v4 ? 4 : 1);

@@ -172,3 +172,40 @@ def test_linear_graph_and_side_stream(M):
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, ops.linear_w8a8(xq, xs, w, ws, bias=b, activation="gelu", residual=r))
+
+
+@pytest.mark.parametrize("M", [1, 8, 64, 256, 300])
+@pytest.mark.parametrize("epilogue", [False, True])
+def test_linear_weights_quantized_just_before(M, epilogue):
+    """The weights come from kernels that the launch may overlap with, directly before or before the
+    activations' own quantization: the product is that of the new weights."""
+    from superl8_serve_b200 import _lib, ops
+
+    N, K = 1184, 4096
+    g = torch.Generator(device=DEV)
+    g.manual_seed(M)
+    ws_in = [torch.randn(N, K, generator=g, device=DEV).bfloat16() for _ in range(2)]
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    r = torch.randn(M, N, generator=g, device=DEV).bfloat16() if epilogue else None
+    space = ops.linear_workspace(M, N, K, DEV)
+    w, ws = ops.quant_rows(ws_in[0])
+    xq, xs = ops.quant_rows(x)
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    want = []
+    for t in ws_in:
+        qw, qs = ops.quant_rows(t)
+        torch.cuda.synchronize()
+        want.append(ops.linear_w8a8(xq, xs, qw, qs, residual=r))
+    torch.cuda.synchronize()
+
+    def quantize(src, q, s):
+        _lib.call("s8b_quant_rows", src.data_ptr(), 0, q.data_ptr(), s.data_ptr(), src.shape[0], K,
+                  _lib.stream(src.device))
+
+    for i in range(40):
+        for both in (False, True):
+            quantize(ws_in[i % 2], w, ws)
+            if both:
+                quantize(x, xq, xs)
+            ops.linear_w8a8(xq, xs, w, ws, residual=r, out=out, workspace=space)
+            assert torch.equal(out, want[i % 2])
