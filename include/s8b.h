@@ -505,7 +505,8 @@ int s8b_moe_combine(const void *contrib, const void *topw, const int32_t *topi,
  * gu_w, d_w 16-byte aligned. One cooperative launch with two grid barriers. workspace:
  * s8b_moe_layer_workspace_size(top_k, F) bytes, 256-byte aligned, its first 256 bytes zero-filled
  * once; workspace[0] (int32) receives S8B_ERR_TIMEOUT if a barrier gave up (the output is then
- * invalid, and the caller zero-fills the 256 bytes again). Launches that share a workspace must
+ * invalid). Until the caller has zero-filled the 256 bytes again, launches on that workspace write
+ * nothing. Launches that share a workspace must
  * be stream-ordered. Replaces SparseMoE.forward for decode rows
  * (superl8serve/models/moe.py:88-141).                                                     */
 int s8b_moe_layer_max_rows(int H, int F, int top_k);

@@ -56,10 +56,13 @@ struct MoeArgs {
 };
 
 // Every thread's writes before are seen by every thread of the grid after. Bounded: false after
-// about a second, with the status word set.
-__device__ bool grid_barrier(uint8_t *ws, int *ok) {
+// about a second, with the status word set. `status` (thread 0) is that word as the kernel found it:
+// where an earlier launch gave up, its arrivals may be missing from the counter, and a barrier would
+// open before all CTAs came. Then no CTA arrives or goes on, until the caller has zeroed both.
+__device__ bool grid_barrier(uint8_t *ws, int *ok, int32_t status) {
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && status != 0) *ok = 0;
+  if (threadIdx.x == 0 && status == 0) {
     unsigned long long *ctr = reinterpret_cast<unsigned long long *>(ws + ml::kOffBar);
     const unsigned long long n = gridDim.x;
     __threadfence();
@@ -208,6 +211,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   __shared__ int before[kMaxA + 1];    // cost of a pair of every chosen expert before
   __shared__ uint8_t slot_of[kMaxE];  // its place among the chosen experts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t status = threadIdx.x == 0 ? *reinterpret_cast<volatile int32_t *>(a.ws) : 0;
   const int T_ = a.T, H = a.H, F = a.F, E = a.E, k = a.k, A = T_ * k;
   float *logits = reinterpret_cast<float *>(a.ws + kLogits);
   float *act = reinterpret_cast<float *>(a.ws + kAct);
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   }
   for (int i = threadIdx.x; i < E; i += kThreads) members[i] = 0u;
   if (threadIdx.x < T_) xs_s[threadIdx.x] = a.xs[threadIdx.x];
-  if (!grid_barrier(a.ws, &ok_s)) return;
+  if (!grid_barrier(a.ws, &ok_s, status)) return;
 
   // ---- B: each row's experts, then their gate_up and SwiGLU ----
   if (warp < T_) {
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
       u += 1 + two;
     }
   }
-  if (!grid_barrier(a.ws, &ok_s)) return;
+  if (!grid_barrier(a.ws, &ok_s, status)) return;
 
   // ---- C: act codes, then this CTA's columns of the down products ----
   if (nh == 0) return;
