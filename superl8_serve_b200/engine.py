@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import ops
-from ._lib import call, ptr, stream
+from ._lib import S8BError, call, ptr, stream
 from .runtime import KVPool, MicroBatch, StageModel, StageRunner
 
 
@@ -353,8 +353,23 @@ class DecodePipeline:
         return g
 
     def synchronize(self):
+        """Wait for every stage; raises where a kernel reported an error (``check_status``)."""
         for mdl in self.models:
             torch.cuda.synchronize(mdl.device)
+        self.check_status(self.runners)
+
+    def check_status(self, runners: list[StageRunner]):
+        """Raise if a launch of ``runners`` left its workspace's status word set (a bounded wait that
+        gave up, a bad block id or length): the tokens since the last check are invalid. The
+        headers are zeroed, so that the workspaces can be used again. Reads nothing where none of
+        the runners' launches has such a word."""
+        found = [(name, ws) for r in runners for name, ws in r.status_workspaces()]
+        codes = [int(ws[:4].view(torch.int32)) for _, ws in found]
+        if any(codes):
+            for _, ws in found:
+                ws[:256].zero_()
+            name, code = next((n, c) for (n, _), c in zip(found, codes) if c)
+            raise S8BError(name, code, ", reported on the device: the results are invalid")
 
     # --------------------------------------------------------------------- sampling ----
     def set_sampling(self, params: list[dict] | None, prompts: list[list[int]] | None = None,
@@ -523,6 +538,7 @@ class DecodePipeline:
                     if not self.single_device:
                         ev[s].record(st)
         self.synchronize()
+        self.check_status(runners)
         first = out_ids[ends.to(out_ids.device)].cpu().tolist()
         if keep_logits:
             return first, list(lg_rows.float().cpu())

@@ -480,6 +480,18 @@ class StageRunner:
                     "stream": torch.cuda.Stream(device=pd),
                     "ev_in": torch.cuda.Event(), "ev_out": torch.cuda.Event()}
 
+    def status_workspaces(self) -> list[tuple[str, torch.Tensor]]:
+        """(entry point, workspace) of this runner's launches whose workspace begins with a status
+        word: non-zero once a bounded wait gave up or an argument on the device was bad."""
+        out = []
+        if self.chunk_ws is not None:
+            out.append(("s8b_paged_chunk_q8", self.chunk_ws))
+        if self.fused_moe and self.moe_buf is not None:
+            out.append(("s8b_moe_layer", self.moe_buf["layer_ws"]))
+        if self.tc_ws is not None and self.m >= self.WIDE_ROWS:
+            out.append(("s8b_linear_w8a8", self.tc_ws))
+        return out
+
     # ---------------------------------------------------------------------- pieces ----
     # rows from which a product is tiled for the tensor pipe (s8b_linear_w8a8) instead of streaming
     # the weights once per 256 rows; the same bits either way

@@ -206,3 +206,22 @@ def test_linear_layer_takes_scales_as_a_column():
     x = torch.randn(3, 272, generator=g, device=DEV).bfloat16()
     q, s = ops.quant_rows(x)
     assert torch.equal(lin(x), ops.gemm_w8a8(q, s, w, ws))
+
+
+def test_status_words_end_a_step_and_a_prefill():
+    """A word left in a workspace, as by a wait that gave up, raises at the next synchronisation;
+    afterwards the pipeline gives what it gave before."""
+    from superl8_serve_b200._lib import ERR_TIMEOUT, S8BError
+    from superl8_serve_b200.config import tiny_moe
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny_moe()
+    prompts = _prompts([20, 3], cfg.vocab_size, 2)
+    pipe = DecodePipeline(_models(cfg), batch=2, max_len=64, prefill_attention="chunk",
+                          fused_moe=True)
+    want = pipe.generate(prompts, 4, prefill=True)
+    for ws in (pipe._pf[0][0].chunk_ws, pipe.runners[0].moe_buf["layer_ws"]):
+        ws[:4].view(torch.int32).fill_(ERR_TIMEOUT)
+        with pytest.raises(S8BError, match="invalid"):
+            pipe.generate(prompts, 4, prefill=True)
+        assert pipe.generate(prompts, 4, prefill=True) == want
