@@ -136,8 +136,9 @@ int s8b_gemm_w8a8_tc_packed(const int8_t *xq, const float *xs, const int8_t *wpa
  *   v = (f32(sum_k xq[m,k]*w[n,k]) * xs[m]) * ws[n] + bias[n];  y[m,n] = act(v) + residual[m,n],
  * int32 sums, binary32 epilogue, one rounding to dtype. bias [N] and residual [M,N] are in dtype
  * and nullable; y may be residual itself. With neither and S8B_ACT_NONE the result equals
- * s8b_gemm_w8a8 bit for bit; the activations use the device's binary32 exp and erf (relative
- * error below 1e-5), so they are not part of the bit-exact contract. Up to 256 rows (and
+ * s8b_gemm_w8a8 bit for bit; the activations use the device's binary32 exp (error below 1e-4 of the
+ * activation's value, in its tails too, down to 2^-118), so they are not part of the bit-exact
+ * contract. Up to 256 rows (and
  * K % 128 == 0) the weights stream through the split-K GEMM above and a second launch finishes
  * the rows; beyond, one launch tiles the product 128 x 128 or 128 x 256 on tcgen05 kind::i8.
  * K % 16 == 0, K < 131072; xq, w 16-byte aligned, bias, residual, y 2-byte aligned (16 bytes and

@@ -38,13 +38,33 @@ using namespace tc;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActGeluTanh = 3, kActRelu = 4 };
 
-// v * sigmoid(z): exp overflows to +inf for z below -88, where the quotient is the limit 0.
+// v * sigmoid(z): exp overflows to +inf for z below -88.7, where the product, 2.7e-37 there, is given
+// as the limit 0 (1 / (1 + e) or e / (1 + e) of e = exp(-|z|) would hold it down to binary32's
+// end, for 1 us of 30 at 999 x 5127 x 1040).
 __device__ __forceinline__ float times_sigmoid(float v, float z) {
   return __fdiv_rn(v, 1.0f + __expf(-z));
 }
+// v Phi(v), Phi the normal distribution. Its lower half is h(|v|) = e^(x^2) erfc(x) e^(-x^2) / 2 with
+// x = |v| / sqrt 2, whose relative precision holds to binary32's end, where (1 + erf) / 2 cancels (ten
+// bits are left of it at v = -4, none at -5.6). e^(x^2) erfc(x) falls smoothly from 1 like 1 / x:
+// in t = 1 / (1 + 0.37 x) it is t times a polynomial, here of degree 6, fitted to it over x in
+// [0, 9.6] for the least largest relative error, 7.6e-7. With erfcf instead the ragged product
+// (999 x 5127 x 1040) takes 34.8 us, with this 29.8.
+__device__ __forceinline__ float times_phi(float v) {
+  const float t = __fdividef(1.0f, fmaf(0.26162952184677124f, fabsf(v), 1.0f));
+  float q = -0.07118100672960281f;
+  q = fmaf(q, t, 0.2174852341413498f);
+  q = fmaf(q, t, -0.09271273016929626f);
+  q = fmaf(q, t, 0.158327117562294f);
+  q = fmaf(q, t, 0.07647876441478729f);
+  q = fmaf(q, t, 0.10741057991981506f);
+  q = fmaf(q, t, 0.10419242829084396f);
+  const float lower = q * t * __expf(-0.5f * v * v);
+  return v * (v < 0.0f ? lower : 1.0f - lower);
+}
 __device__ __forceinline__ float apply_act(float v, int act) {
   if (act == kActSilu) return times_sigmoid(v, v);
-  if (act == kActGelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+  if (act == kActGelu) return times_phi(v);
   // (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2/pi) (v + 0.044715 v^3)
   if (act == kActGeluTanh)
     return times_sigmoid(v, 1.5957691216057308f * v * (1.0f + 0.044715f * v * v));

@@ -209,3 +209,36 @@ def test_linear_weights_quantized_just_before(M, epilogue):
                 quantize(x, xq, xs)
             ops.linear_w8a8(xq, xs, w, ws, residual=r, out=out, workspace=space)
             assert torch.equal(out, want[i % 2])
+
+
+@pytest.mark.parametrize("M", [9, 257])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_activation_tails(M, act, dtype):
+    """Relative to the activation's own value, however small. v has two roundings (2^-23 relative), which
+    the tails multiply by |v f'(v) / f(v)|: below v^2 + 1 <= 200 for GELU down to binary32's smallest
+    values, 100 for SiLU: 2.4e-5. The argument's own rounding counts the same again, exp, erfc and the
+    division below 2e-5. Together below 1e-4, then half a step of the output. Below binary32's normal
+    range (2^-126, times |v| < 2^7) steps are coarser; fp16's own end at 2^-24."""
+    from superl8_serve_b200 import ops
+
+    K, N = 128, 254
+    xq = torch.zeros(M, K, dtype=torch.int8, device=DEV)
+    w = torch.zeros(N, K, dtype=torch.int8, device=DEV)
+    xq[:, 5] = 1 + torch.arange(M, device=DEV) % 9
+    w[:, 5] = torch.cat([torch.arange(-127, 0), torch.arange(1, 128)]).to(DEV)
+    xs = 0.25 + torch.rand(M, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    ws = torch.full((N,), 0.1, device=DEV)
+    v = (xq.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+    assert v.min() < -100 and v.max() > 100 and v.abs().min() < 0.1
+    if act == "silu":
+        want = v * torch.sigmoid(v)
+    elif act == "gelu":
+        want = v * 0.5 * torch.erfc(-v / math.sqrt(2))
+    else:
+        want = v * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3))
+    y = ops.linear_w8a8(xq, xs, w, ws, activation=act, out_dtype=dtype).double()
+    least = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -118
+    tol = (torch.finfo(dtype).eps / 2 + 1e-4) * want.abs() + least
+    bad = (y - want).abs() > tol
+    assert not bad.any(), (v[bad][:4].tolist(), y[bad][:4].tolist(), want[bad][:4].tolist())
