@@ -138,12 +138,12 @@ int s8b_gemm_w8a8_tc_packed(const int8_t *xq, const float *xs, const int8_t *wpa
  * and nullable; y may be residual itself. With neither and S8B_ACT_NONE the result equals
  * s8b_gemm_w8a8 bit for bit; the activations use the device's binary32 exp (error below 1e-4 of the
  * activation's value, in its tails too, down to 2^-118), so they are not part of the bit-exact
- * contract. Up to 256 rows (and
- * K % 128 == 0) the weights stream through the split-K GEMM above and a second launch finishes
- * the rows; beyond, one launch tiles the product 128 x 128 or 128 x 256 on tcgen05 kind::i8.
+ * contract. Few rows (up to 16, and up to 256 where the partial sums cost less than tiles; K % 128
+ * == 0) stream the weights through the split-K GEMM above and a second launch finishes them; else
+ * one launch tiles the product 128 x 128 or 128 x 256 on tcgen05 kind::i8.
  * K % 16 == 0, K < 131072; xq, w 16-byte aligned, bias, residual, y 2-byte aligned (16 bytes and
- * N % 8 == 0 store vectors). workspace: s8b_linear_workspace_size bytes, 256-byte aligned, its
- * first 256 bytes zero-filled once; workspace[0] (int32) receives S8B_ERR_TIMEOUT if a bounded
+ * N % 8 == 0 store vectors). workspace: s8b_linear_workspace_size bytes (enough for calls of fewer
+ * rows too where M <= 256), 256-byte aligned, its first 256 bytes zero-filled once; workspace[0] (int32) receives S8B_ERR_TIMEOUT if a bounded
  * wait gave up. Launches that share a workspace must be stream-ordered. Any argument may come
  * from the kernel just before on the stream, the weights among them.
  * Replaces superl8.linear and the bias and residual additions around it

@@ -1,8 +1,8 @@
 // W8A8 linear layer with its epilogue: y = act((xq . w^T) * xs * ws + bias) + residual, for
 // any token count (s8b_linear_w8a8).
 //
-// Two forms, by the token count (few_rows below):
-//  * few rows: the weights are the whole cost (1 byte read per 2 M operations), so the decode
+// Two forms, by their cost (few_rows below):
+//  * few rows: the weights are most of the cost (1 byte read per 2 M operations), so the decode
 //    GEMM of gemm_tc.cu streams them with its K range split over CTAs, its int32 partials stay
 //    in L2, and linear_epilogue_kernel sums, scales and finishes them;
 //  * many rows: the product is bound by the int8 tensor pipe. linear_tc_kernel below tiles it
@@ -404,10 +404,6 @@ __global__ void __launch_bounds__(256)
 // ----------------------------------------------------------------------------- host ----
 constexpr size_t kLinHeader = 256;  // the status word
 
-// Rows up to which the weights' stream decides (and K fits the decode GEMM's 128-byte slices).
-constexpr int kFewRows = 256;
-inline bool few_rows(int M, int K) { return M <= kFewRows && K % 128 == 0; }
-
 // Weight rows per tile: the width whose last wave wastes less. A 128-wide tile moves a third
 // more operand bytes per product than a 256-wide one, counted as 1/8 more time.
 inline int pick_width(int M, int N) {
@@ -415,6 +411,24 @@ inline int pick_width(int M, int N) {
   const long w256 = (tm * ((N + 255) / 256) + sms - 1) / sms;
   const long w128 = (tm * ((N + 127) / 128) + sms - 1) / sms;
   return w128 * 9 < w256 * 16 ? 128 : 256;
+}
+
+// Whether the split-K stream takes the call: at most one pass of it, and K in its 128-byte slices.
+// Up to 16 rows always. Beyond, by cost in microseconds: the stream reads the weights at some 4.5
+// TB/s and its partials go out and come back at 1 TB/s of their size, a tile's CTA takes 0.4 for
+// each 128 columns of each K slice. Measured (stream / tiles, with residual, us): 4096 x 4096 (N x K)
+// 64 rows 11.5 / 14.3, 256 rows 17.8 / 14.8; 12288 x 4096 32 rows 15.7 / 16.1, 64 rows 19.7 / 16.0; 1024 x
+// 4096 256 rows 12.2 / 14.3; 151936 x 4096 8 rows 108 / 124, 64 rows 182 / 118, 256 rows 427 / 166
+// (622 MB of partials). Over N of 256 to 151936, K of 1024 to 12288 and 1 to 256 rows the choice costs 0.5
+// % on average and at worst 1.4 times (256 x 1024, 256 rows: 10.0 / 7.1).
+inline bool few_rows(int M, int N, int K) {
+  if (M > 256 || K % 128 != 0) return false;
+  if (M <= 16) return true;
+  const int C = s8b_gemm_tc_split_count(M, N, K), NT = pick_width(M, N);
+  if (C < 1) return false;
+  const long sms = sm_count(), tiles = (M + kTileM - 1l) / kTileM * ((N + NT - 1l) / NT);
+  const double stream = static_cast<double>(N) * K / 4.5e6 + 4.0 * C * M * N / 1e6;
+  return stream <= 0.4 * (NT / 128) * (K / kSlice) * ((tiles + sms - 1) / sms);
 }
 
 template <typename T, int NT, bool ACT>
@@ -470,10 +484,17 @@ int launch_few(const int8_t *xq, const float *xs, const int8_t *w, const LinArgs
 
 using namespace s8b;
 
+// What this call needs.
+static size_t workspace_need(int M, int N, int K) {
+  if (!few_rows(M, N, K)) return kLinHeader;
+  return kLinHeader + sizeof(int32_t) * s8b_gemm_tc_split_count(M, N, K) * M * N;
+}
+
+// What every call of up to M rows needs, for M <= 256.
 extern "C" size_t s8b_linear_workspace_size(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || !few_rows(M, K)) return kLinHeader;
-  const int C = s8b_gemm_tc_split_count(M, N, K);
-  return kLinHeader + static_cast<size_t>(C < 1 ? 0 : C) * M * N * sizeof(int32_t);
+  if (M <= 0 || N <= 0 || K <= 0 || M > 256 || K % 128 != 0) return kLinHeader;
+  while (M > 1 && !few_rows(M, N, K)) --M;
+  return workspace_need(M, N, K);
 }
 
 extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *w,
@@ -488,7 +509,7 @@ extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *
   if (!aligned(xq, 16) || !aligned(w, 16) || !aligned(xs, 4) || !aligned(ws, 4) ||
       !aligned(y, 2) || !aligned(bias, 2) || !aligned(residual, 2))
     return S8B_ERR_ALIGN;
-  if (!workspace || workspace_bytes < s8b_linear_workspace_size(M, N, K))
+  if (!workspace || workspace_bytes < (M ? workspace_need(M, N, K) : kLinHeader))
     return S8B_ERR_WORKSPACE;
   if (!aligned(workspace, 256)) return S8B_ERR_ALIGN;
   if (M == 0) return S8B_OK;
@@ -505,7 +526,7 @@ extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *
   a.vec = N % 8 == 0 && aligned(y, 16) && aligned(bias, 16) && aligned(residual, 16) &&
           aligned(ws, 16);
   S8B_DISPATCH_DTYPE(dtype, T, {
-    if (few_rows(M, K)) return launch_few<T>(xq, xs, w, a, K, workspace, dtype, stream);
+    if (few_rows(M, N, K)) return launch_few<T>(xq, xs, w, a, K, workspace, dtype, stream);
     auto st = (cudaStream_t)stream;
     const bool act = activation != kActNone;
     if (pick_width(M, N) == 256)

@@ -242,3 +242,33 @@ def test_activation_tails(M, act, dtype):
     tol = (torch.finfo(dtype).eps / 2 + 1e-4) * want.abs() + least
     bad = (y - want).abs() > tol
     assert not bad.any(), (v[bad][:4].tolist(), y[bad][:4].tolist(), want[bad][:4].tolist())
+
+
+@pytest.mark.parametrize("M", [16, 17, 40, 96, 128, 129, 200, 256])
+@pytest.mark.parametrize("N,K", [(264, 256), (1025, 1024), (20000, 256), (4096, 512)])
+def test_both_forms_with_one_workspace(M, N, K):
+    """A workspace made for 256 rows serves every smaller call, whichever form it takes."""
+    from superl8_serve_b200 import ops
+
+    xq, xs, w, ws, b, r = _case(M, N, K, torch.bfloat16, True, True, seed=M + N)
+    space = ops.linear_workspace(256, N, K, DEV)
+    y = ops.linear_w8a8(xq, xs, w, ws, bias=b, activation="silu", residual=r, workspace=space)
+    _near(y, *_exact(xq, xs, w, ws, b, r, "silu"))
+    y = ops.linear_w8a8(xq, xs, w, ws, workspace=space)
+    assert torch.equal(y, ops.gemm_w8a8(xq, xs, w, ws))
+    assert int(space[:4].view(torch.int32)) == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 7, 128), (5, 261, 256), (16, 1001, 384), (3, 129, 4096),
+                                   (60, 515, 512)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows_of_odd_width(M, N, K, dtype):
+    """The streamed form's scalar epilogue (N not a multiple of 4)."""
+    from superl8_serve_b200 import ops
+
+    xq, xs, w, ws, b, r = _case(M, N, K, dtype, True, True, seed=M + N)
+    assert ops.linear_workspace(M, N, K, DEV).numel() > 256
+    y = ops.linear_w8a8(xq, xs, w, ws, bias=b, activation="gelu", residual=r, out_dtype=dtype)
+    _near(y, *_exact(xq, xs, w, ws, b, r, "gelu"))
+    assert torch.equal(ops.linear_w8a8(xq, xs, w, ws, out_dtype=dtype),
+                       ops.gemm_w8a8(xq, xs, w, ws, out_dtype=dtype))
