@@ -47,14 +47,23 @@ class LinearW8A8(nn.Module):
         shape and dtype) are applied in the product's epilogue, after the bias, in binary32:
         one rounding instead of one per step."""
         _cuda(x, "LinearW8A8")
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"LinearW8A8: rows of {x.shape[-1]} values, weights of {self.in_features}")
         q, s = ops.quant_rows(x)
         w = self.weight
         if activation is not None or residual is not None:
             return ops.linear_w8a8(q, s, w.data, w.scale.reshape(-1), bias=self.bias,
                                    activation=activation, residual=residual, out_dtype=x.dtype)
-        # one row: the dp4a product; more: the tensor cores. The same bits.
-        if s.numel() == 1:
+        # The dp4a product or the tensor cores: the same bits. GPU time (dp4a / tensor cores, us): K a
+        # multiple of 128, 24576 x 4096 (N x K) 2 rows 22 / 24, 8 rows 42 / 24; other K, where the
+        # streamed form does not serve, 4096 x 4112 4 rows 11 / 14, 8 rows 16 / 14, 260 x 272 8 rows
+        # 6.3 / 7.5, 16 rows 12 / 7.6 (and 7 us less host time by dp4a).
+        rows, streams = s.numel(), self.in_features % 128 == 0
+        if rows <= (2 if streams else 8):
             y = ops.gemm_w8a8(q, s, w.data, w.scale, out_dtype=x.dtype)
+        elif streams and rows <= 256:
+            y = ops.gemm_w8a8_tc(q, s, w.data, w.scale, out_dtype=x.dtype, ordered=True,
+                                 workspace=ops._status_word(x.device))
         else:
             y = ops.linear_w8a8(q, s, w.data, w.scale.reshape(-1), out_dtype=x.dtype)
         return y if self.bias is None else y + self.bias

@@ -13,7 +13,7 @@ __all__ = [
     "silu_mul_quant", "qkv_post", "kv_write_paged",
     "paged_decode_q8", "paged_decode", "embed", "argmax", "codec_encode", "codec_decode",
     "codec_sizes", "decode_workspace_bytes", "moe_route", "moe_gemm_grouped", "moe_combine",
-    "sample", "linear_w8a8", "linear_workspace", "paged_chunk_q8", "chunk_workspace",
+    "sample", "linear_w8a8", "linear_workspace", "linear_status", "paged_chunk_q8", "chunk_workspace",
     "moe_layer", "moe_layer_workspace", "moe_layer_max_rows",
 ]
 
@@ -103,6 +103,9 @@ def gemm_w8a8(xq, xs, w, ws, *, out=None, out_dtype=torch.bfloat16, raw=False):
     return out
 
 
+_GEMM_ORDERED = 8  # out_kind flag: the weights are read after the preceding kernel has ended
+
+
 def gemm_tc_workspace(M: int, N: int, device) -> torch.Tensor:
     """Zero-filled workspace for s8b_gemm_w8a8_tc (kept zero by every completed launch)."""
     from ._lib import load
@@ -122,9 +125,11 @@ def pack_weights_tc(w: torch.Tensor) -> torch.Tensor:
 
 
 def gemm_w8a8_tc(xq, xs, w, ws, *, out=None, out_dtype=torch.bfloat16, raw=False, workspace=None,
-                 packed: torch.Tensor | None = None):
+                 packed: torch.Tensor | None = None, ordered: bool = False):
     """Tensor-core (tcgen05 kind::i8) form of gemm_w8a8; identical results. With `packed`
-    (from pack_weights_tc(w)) the weight stream is read as contiguous unit images."""
+    (from pack_weights_tc(w)) the weight stream is read as contiguous unit images. The weights'
+    first reads may overlap with the kernel before; with `ordered` (not for `packed`) that kernel
+    may write them."""
     K = xq.shape[-1]
     M = xq.numel() // K
     N = w.shape[0]
@@ -138,13 +143,43 @@ def gemm_w8a8_tc(xq, xs, w, ws, *, out=None, out_dtype=torch.bfloat16, raw=False
         call("s8b_gemm_w8a8_tc_packed", ptr(xq), ptr(xs), ptr(packed), ptr(ws), ptr(out),
              1 if raw else 0, M, N, K, dt, ptr(workspace), workspace.numel(), stream(xq.device))
     else:
-        call("s8b_gemm_w8a8_tc", ptr(xq), ptr(xs), ptr(w), ptr(ws), ptr(out), 1 if raw else 0, M,
-             N, K, dt, ptr(workspace), workspace.numel(), stream(xq.device))
+        call("s8b_gemm_w8a8_tc", ptr(xq), ptr(xs), ptr(w), ptr(ws), ptr(out),
+             (1 if raw else 0) | (_GEMM_ORDERED if ordered else 0), M, N, K, dt, ptr(workspace),
+             workspace.numel(), stream(xq.device))
     return out
 
 
+_status: dict[int, torch.Tensor] = {}
+
+
+def _status_word(dev: torch.device) -> torch.Tensor:
+    """The workspace of products that need a status word only: one per device, shared by all streams
+    (it is written only where a bounded wait gave up). During a graph capture that comes before
+    any other call, one of the graph's own."""
+    ws = _status.get(dev.index)
+    if ws is None:
+        with _on(dev):
+            ws = torch.zeros(256, dtype=torch.uint8, device=dev)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(dev).synchronize()  # other streams may use it at once
+                _status[dev.index] = ws
+    return ws
+
+
+def linear_status(device) -> int:
+    """0, or the error that a ``linear_w8a8`` call without ``workspace`` left on this device since the
+    last ask (``_lib.ERR_TIMEOUT``: a bounded wait gave up). Waits for the current stream."""
+    index = torch.device(device).index
+    ws = _status_word(torch.device("cuda", torch.cuda.current_device() if index is None else index))
+    code = int(ws[:4].view(torch.int32))
+    if code:
+        ws.zero_()
+    return code
+
+
 def linear_workspace(M: int, N: int, K: int, device) -> torch.Tensor:
-    """Workspace of ``linear_w8a8`` for these sizes (its status word zeroed)."""
+    """Workspace of ``linear_w8a8`` for these sizes (its status word zeroed); up to 256 rows it serves
+    calls of fewer rows too."""
     from ._lib import load
 
     ws = torch.empty(int(load().s8b_linear_workspace_size(M, N, K)), dtype=torch.uint8,
@@ -158,7 +193,9 @@ def linear_w8a8(xq, xs, w, ws, *, bias=None, activation=None, residual=None, out
     """``act(dequant(xq @ w^T) + bias) + residual`` rounded once to ``out_dtype``
     (``s8b_linear_w8a8``): xq [..., K] int8, xs [...] fp32, w [N, K] int8, ws [N] fp32, bias [N]
     and residual [..., N] in the output dtype; activation None, "silu", "gelu", "gelu_tanh" or
-    "relu". ``out`` may be ``residual``."""
+    "relu". ``out`` may be ``residual``. Without ``workspace`` (``linear_workspace``) a call that only
+    needs a status word uses the device's (``linear_status``): tiled products, and all that have
+    no bias, activation or residual, which then take one launch; the bits are the same."""
     if activation not in ACTIVATION:
         raise ValueError(f"linear_w8a8: unknown activation {activation!r}")
     if xq.dim() < 1 or w.dim() != 2:
@@ -175,7 +212,13 @@ def linear_w8a8(xq, xs, w, ws, *, bias=None, activation=None, residual=None, out
     if M == 0:
         return out
     if workspace is None:
-        workspace = linear_workspace(M, N, K, dev)
+        if activation is None and bias is None and residual is None and M <= 256 and K % 128 == 0:
+            ws1 = _status_word(dev)
+            _call_on(dev, "s8b_gemm_w8a8_tc", *p[:4], p[6], _GEMM_ORDERED, M, N, K, code,
+                     ws1.data_ptr(), ws1.numel())
+            return out
+        workspace = (_status_word(dev) if M > 256 or K % 128 != 0 else
+                     linear_workspace(M, N, K, dev))
     _call_on(dev, "s8b_linear_w8a8", *p[:5], ACTIVATION[activation], *p[5:], M, N, K, code,
              *_workspace("linear_w8a8", dev, workspace))
     return out

@@ -225,3 +225,68 @@ def test_status_words_end_a_step_and_a_prefill():
         with pytest.raises(S8BError, match="invalid"):
             pipe.generate(prompts, 4, prefill=True)
         assert pipe.generate(prompts, 4, prefill=True) == want
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 260, 256), (3, 260, 256), (8, 24, 272), (9, 24, 272),
+                                   (64, 1000, 512), (256, 264, 1024), (257, 264, 1024)])
+def test_linear_layer_keeps_its_bits_in_every_form(M, N, K):
+    from superl8_serve_b200 import ops
+    from superl8_serve_b200.layers import LinearW8A8
+    from superl8_serve_b200.weights import QTensor
+
+    g = _gen(M + K)
+    w, ws = _weight(g, N, K)
+    lin = LinearW8A8(QTensor(w, ws, "per_row_i8"))
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    q, s = ops.quant_rows(x)
+    want = ops.gemm_w8a8(q, s, w, ws)
+    assert torch.equal(lin(x), want)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        y = lin(x)
+    y.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and ops.linear_status(DEV) == 0
+
+
+def test_linear_layer_needs_no_more_than_its_output():
+    """256 rows of a head with 40,000 columns: no partial sums in memory beside the result."""
+    from superl8_serve_b200.layers import LMHead
+    from superl8_serve_b200.weights import QTensor
+
+    g = _gen(8)
+    w, ws = _weight(g, 40000, 1024)
+    head = LMHead(QTensor(w, ws, "per_row_i8"))
+    x = torch.randn(256, 1024, generator=g, device=DEV).bfloat16()
+    y = head(x)
+    out = y.numel() * 2
+    del y
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = head(x)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before <= out + (1 << 20)
+
+
+def test_status_word_of_calls_without_a_workspace():
+    from superl8_serve_b200 import _lib, ops
+
+    assert ops.linear_status(DEV) == 0
+    ops._status[0][:4].view(torch.int32).fill_(_lib.ERR_TIMEOUT)
+    assert ops.linear_status("cuda") == _lib.ERR_TIMEOUT
+    assert ops.linear_status(torch.device(DEV)) == 0
+
+
+def test_linear_layer_refuses_rows_of_another_length():
+    from superl8_serve_b200.layers import LinearW8A8
+    from superl8_serve_b200.weights import QTensor
+
+    g = _gen(4)
+    w, ws = _weight(g, 24, 256)
+    for M in (1, 3, 300):
+        with pytest.raises(ValueError, match="rows of 272"):
+            LinearW8A8(QTensor(w, ws, "per_row_i8"))(torch.zeros(M, 272, device=DEV).bfloat16())
