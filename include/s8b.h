@@ -573,7 +573,9 @@ int s8b_sample(const void *logits, int dtype, int M, int V, const float *tempera
  *   [else]  s8b_codec_encode(h, res) into out_payload (may be a peer's memory)
  * GEMMs run on the tensor cores (packed weight images) when tc_min > 0, M >= tc_min and a
  * packed image is given, with split-K partials in `part` between a GEMM and the row kernel
- * that follows it; otherwise on the dp4a path. Buffers are sized for M rows as the Python
+ * that follows it; otherwise on the dp4a path. Above 256 rows they are tiled (s8b_linear_w8a8, the
+ * same bits; qkv and gu then hold what `part` held, which needs 256 rows only) unless qkv, a
+ * dense layer's gu or a layer's plain weights are NULL. Buffers are sized for M rows as the Python
  * runtime sizes them (StageRunner). Expert shards on other GPUs are not handled here.   */
 typedef struct S8bLayerDesc {
   const int8_t *qkv_w, *qkv_packed; const float *qkv_s;

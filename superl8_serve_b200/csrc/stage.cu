@@ -16,11 +16,16 @@ struct Step {
   const S8bStageDesc &d;
   void *st;
   int M;
-  bool tc;  // tensor-core GEMMs (and split-K partials) for this launch size
+  bool tc;    // tensor-core GEMMs for this launch size
+  bool wide;  // more rows than a pass of the streamed GEMM takes: products tiled (the same bits)
+  bool split() const { return tc && !wide; }  // products leave split-K partials in d.part
 
   // y = dequant(xq @ w^T) in the activation dtype (out_kind 0)
   int gemm(const int8_t *xq, const float *xs, const int8_t *w, const int8_t *packed,
            const float *s, void *y, int N, int K) const {
+    if (wide)
+      return s8b_linear_w8a8(xq, xs, w, s, nullptr, S8B_ACT_NONE, nullptr, y, M, N, K, d.dtype,
+                             d.tc_ws, d.tc_ws_bytes, st);
     if (tc && packed)
       return s8b_gemm_w8a8_tc_packed(xq, xs, packed, s, y, 0, M, N, K, d.dtype, d.tc_ws,
                                      d.tc_ws_bytes, st);
@@ -72,7 +77,7 @@ struct Step {
                                       d.eps, d.xq, d.xs, M, H, d.dtype, st));
     else
       S8B_TRY(rms(d.h, first_of_model ? nullptr : d.res, L.in_norm, in_C, in_ws, nullptr));
-    if (tc) {
+    if (split()) {
       const int C = gemm_split(L.qkv_packed, Nqkv, H);
       if (C < 0) return C;
       S8B_TRY(s8b_qkv_post_split(d.part, C, d.xs, L.qkv_s, d.positions, d.cos_tab, d.sin_tab,
@@ -92,7 +97,7 @@ struct Step {
                                 d.attn_ws_bytes, d.dtype, st));
     const int Kattn = d.Hq * d.D;
     if (L.moe_experts > 0) {
-      if (tc) {
+      if (split()) {
         const int C = gemm_split(L.o_packed, H, Kattn);
         if (C < 0) return C;
         S8B_TRY(rms(nullptr, d.res, L.post_norm, C, L.o_s, d.moe_y));
@@ -102,7 +107,7 @@ struct Step {
       }
       return moe(L);
     }
-    if (tc) {
+    if (split()) {
       int C = gemm_split(L.o_packed, H, Kattn);
       if (C < 0) return C;
       S8B_TRY(rms(nullptr, d.res, L.post_norm, C, L.o_s, nullptr));
@@ -155,7 +160,12 @@ extern "C" int s8b_stage_step(const S8bStageDesc *desc, void *stream) {
         return S8B_ERR_ARG;
     }
   }
-  Step s{d, stream, d.M, tc};
+  bool wide = tc && d.M > 256 && d.qkv;
+  for (int li = 0; li < d.n_layers; ++li) {
+    const S8bLayerDesc &L = d.layers[li];
+    wide = wide && L.qkv_w && L.o_w && (L.moe_experts > 0 || d.gu);
+  }
+  Step s{d, stream, d.M, tc, wide};
   // stage prologue: the first RMSNorm decodes the received [hidden | residual] on load
   if (d.embed)
     S8B_TRY(s8b_embed(d.ids, d.embed, d.M, d.H, d.h, d.dtype, stream));

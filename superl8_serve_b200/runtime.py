@@ -444,7 +444,7 @@ class StageRunner:
                     N, K = w.shape
                     c = int(lib.s8b_gemm_tc_split_count(m, N, K))
                     self.splits[(N, K)] = c
-                    need = max(need, c * m * N)
+                    need = max(need, c * min(m, self.WIDE_ROWS - 1) * N)
             self.part = torch.empty(need, dtype=torch.int32, device=dev)
         # sparse-MoE layers: router input, routing / grouping state and per-assignment rows
         moes = [L.moe for L in model.layers if L.moe is not None]
@@ -494,7 +494,10 @@ class StageRunner:
 
     # ---------------------------------------------------------------------- pieces ----
     # rows from which a product is tiled for the tensor pipe (s8b_linear_w8a8) instead of streaming
-    # the weights once per 256 rows; the same bits either way
+    # the weights once per 256 rows; the same bits either way. Tiles / packed streams, us: 257 rows
+    # 14.1 / 28.6 (N x K 4096 x 4096), 36.7 / 57.5 (24576 x 4096), 13.7 / 26.2 (2048 x 4096); 1024 rows
+    # 18.4 / 77.5, 84.9 / 153, 14.0 / 76.8. (At 256 rows 14.8 / 20.4 and 37.7 / 38.5, but there the
+    # streams' partials are summed by the next row kernel, which saves a pass.)
     WIDE_ROWS = 257
 
     def _gemm(self, xq, xs, w, s, out, M):

@@ -290,3 +290,32 @@ def test_linear_layer_refuses_rows_of_another_length():
     for M in (1, 3, 300):
         with pytest.raises(ValueError, match="rows of 272"):
             LinearW8A8(QTensor(w, ws, "per_row_i8"))(torch.zeros(M, 272, device=DEV).bfloat16())
+
+
+@pytest.mark.parametrize("moe", [False, True])
+@pytest.mark.parametrize("stages", [1, 2])
+def test_wide_chunks_in_every_kind_of_stage_step(moe, stages):
+    """Prefill chunks above 256 rows, launch by launch and as native stage steps, dense and sparse: the
+    bits of 256-row chunks, without partial sums for more than 256 rows in memory."""
+    from superl8_serve_b200 import _lib
+    from superl8_serve_b200.config import tiny, tiny_moe
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny_moe() if moe else tiny()
+    models = _models(cfg, stages)
+    prompts = _prompts([300, 7, 411], cfg.vocab_size)
+    got = []
+    for native, chunk in ((False, 256), (False, 700), (True, 256), (True, 700)):
+        pipe = DecodePipeline(models, batch=3, max_len=512)
+        pipe.prefill_chunk = chunk
+        if native:
+            pipe.set_native()
+        got.append(pipe.prefill(prompts, keep_logits=True))
+        for r in pipe._pf[0]:
+            most = max(_lib.load().s8b_gemm_tc_split_count(256, *w.shape) * w.shape[0]
+                       for L in r.model.layers for w in L.matrices())
+            assert r.m == chunk and r.part.numel() == 256 * most
+    for toks, logits in got[1:]:
+        assert toks == got[0][0]
+        for a, b in zip(logits, got[0][1]):
+            assert torch.equal(a, b)
