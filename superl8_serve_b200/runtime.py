@@ -361,6 +361,17 @@ def moe_expert_buffers(M: int, k: int, H: int, Fe: int, E: int, device, dtype=to
             "status": z(4, dt=torch.int32)}
 
 
+def fused_moe_pays(M: int, H: int, F: int, E: int, k: int) -> bool:
+    """Whether the one-launch MoE layer is the faster one for M rows that it takes. Its dp4a products
+    cost time for every row beyond the two or three that an expert's weights hide, where the
+    grouped tensor-core products do not. GPU time (route + grouped products + combine / one launch, us): 2048 x
+    768, 8 of 128 experts, 1 row 81 / 20, 8 rows 123 / 65, 16 rows 141 / 97; 1040 x 272, 3 of 20, 16
+    rows 31 / 25; 2048 x 768, 4 of 16, 16 rows 44 / 40; 8 of 32, 12 rows 63 / 59, 16 rows 64 / 65;
+    4096 x 2048, 2 of 8, 10 rows 62 / 59, 14 rows 63 / 66; 4096 x 4096, 2 of 8, 8 rows 96 / 89, 12 rows
+    95 / 107; 4 of 8, 12 rows 98 / 151."""
+    return M * k < 3 * E or M * k * 3 * H * F < 500_000_000
+
+
 class StageRunner:
     """Launches one stage's decode kernels for a micro-batch of up to ``m`` rows."""
 
@@ -383,8 +394,8 @@ class StageRunner:
         # attention may stream older partitions early (s8b_paged_decode_q8_step); prefill
         # runners set False
         self.decode_step = True
-        # True: a MoE layer of few rows whose experts are all on this GPU is one launch
-        # (s8b_moe_layer: rounds to dtype once, so not bit for bit the general path)
+        # True: a MoE layer of few rows whose experts are all on this GPU is one launch where that
+        # is faster (s8b_moe_layer: rounds to dtype once, so not bit for bit the general path)
         self.fused_moe = False
         # True: MoE layers run their own experts only (no handshake with partner processes):
         # the stage-time measurement of a multi-process pipeline
@@ -558,7 +569,7 @@ class StageRunner:
         b, st, k = self.moe_buf, stream(), mw.top_k
         E, Fe, A, H = mw.num_experts, mw.ffn, M * mw.top_k, self.H
         if (self.fused_moe and not mw.shards and not mw.remote
-                and M <= ops.moe_layer_max_rows(H, Fe, k)):
+                and M <= ops.moe_layer_max_rows(H, Fe, k) and fused_moe_pays(M, H, Fe, E, k)):
             call("s8b_moe_layer", ptr(b["y"]), ptr(self.xq), ptr(self.xs), ptr(mw.router),
                  ptr(mw.gu_w), ptr(mw.gu_s), ptr(mw.d_w), ptr(mw.d_s), ptr(self.h), M, H, Fe, E, k,
                  int(mw.norm_topk_prob), mw.scaling, ptr(b["layer_ws"]), b["layer_ws"].numel(), 0,
