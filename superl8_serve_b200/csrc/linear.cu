@@ -403,6 +403,7 @@ __global__ void __launch_bounds__(256)
 
 // ----------------------------------------------------------------------------- host ----
 constexpr size_t kLinHeader = 256;  // the status word
+constexpr int kMaxSide = 0x7fffffff - 4096;
 
 // Weight rows per tile: the width whose last wave wastes less. A 128-wide tile moves a third
 // more operand bytes per product than a 256-wide one, counted as 1/8 more time.
@@ -492,7 +493,7 @@ static size_t workspace_need(int M, int N, int K) {
 
 // What every call of up to M rows needs, for M <= 256.
 extern "C" size_t s8b_linear_workspace_size(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || M > 256 || K % 128 != 0) return kLinHeader;
+  if (M <= 0 || N <= 0 || K <= 0 || M > 256 || K % 128 != 0 || N > kMaxSide) return kLinHeader;
   while (M > 1 && !few_rows(M, N, K)) --M;
   return workspace_need(M, N, K);
 }
@@ -504,8 +505,10 @@ extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *
   if (!xq || !xs || !w || !ws || !y) return S8B_ERR_ARG;
   if (activation < kActNone || activation > kActRelu) return S8B_ERR_ARG;
   if (dtype != S8B_BF16 && dtype != S8B_FP16) return S8B_ERR_DTYPE;
-  // |sum| <= K * 128 * 128 stays below 2^31 for K < 2^17
-  if (M < 0 || N <= 0 || K <= 0 || K % 16 != 0 || K >= 131072) return S8B_ERR_SHAPE;
+  // |sum| <= K * 128 * 128 stays below 2^31 for K < 2^17; rows and columns are counted in 32 bits, up
+  // to a tile (or a block of the few rows' second launch) beyond the last
+  if (M < 0 || N <= 0 || K <= 0 || K % 16 != 0 || K >= 131072 || M > kMaxSide || N > kMaxSide)
+    return S8B_ERR_SHAPE;
   if (!aligned(xq, 16) || !aligned(w, 16) || !aligned(xs, 4) || !aligned(ws, 4) ||
       !aligned(y, 2) || !aligned(bias, 2) || !aligned(residual, 2))
     return S8B_ERR_ALIGN;

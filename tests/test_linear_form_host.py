@@ -30,3 +30,10 @@ def test_what_a_call_needs(lib):
     assert call(16, 151936, 4096, n - 1) == -7
     assert call(256, 151936, 4096, 255) == -7
     assert call(300, 4096, 4096, 255) == -7
+
+
+@pytest.mark.parametrize("M,N,K", [(2 ** 31 - 1, 64, 16), (2 ** 31 - 100, 64, 128), (300, 2 ** 31 - 1, 16),
+                                   (1, 2 ** 31 - 1, 128), (4, 2 ** 31 - 500, 128)])
+def test_sides_whose_last_tile_passes_32_bits_are_refused(lib, M, N, K):
+    assert lib.s8b_linear_w8a8(OK, OK, OK, OK, None, 0, None, OK, M, N, K, 0, OK, 2 ** 62, None) == -1
+    assert lib.s8b_linear_workspace_size(M, N, K) == 256
