@@ -128,6 +128,15 @@ class DecodePipeline:
         with the same results."""
         if prefill_attention not in ("rows", "chunk"):
             raise ValueError(f"prefill_attention must be 'rows' or 'chunk', got {prefill_attention!r}")
+        if prefill_attention == "chunk":
+            cfg = models[0].cfg
+            if not (0 < block_size <= 256 and block_size & (block_size - 1) == 0):
+                raise ValueError("prefill_attention='chunk' takes a block_size that is a power of two up "
+                                 f"to 256, got {block_size}")
+            if (cfg.resolved_head_dim() != 128
+                    or cfg.num_attention_heads > 128 * cfg.num_key_value_heads):
+                raise ValueError("prefill_attention='chunk' takes a head_dim of 128 and at most 128 "
+                                 "query heads to a kv head")
         self.prefill_attention, self.fused_moe = prefill_attention, fused_moe
         self.models = models
         self.cfg = models[0].cfg
@@ -444,7 +453,9 @@ class DecodePipeline:
         Row (sequence i, position t) writes its K/V at t and attends over positions [0, t]
         of the paged cache (context length t + 1), after the same layer's KV write of the
         whole chunk, so it computes exactly what a decode step of that token computes: the
-        result is bit-identical to feeding the prompt one token per step. The final norm,
+        result is bit-identical to feeding the prompt one token per step (unless the pipeline
+        was made with ``prefill_attention="chunk"`` or ``fused_moe``: then within rounding of
+        it). The final norm,
         LM head and argmax run only in chunks where some sequence ends; the argmax of each
         sequence's last row is its first generated token (returned, one per sequence; with
         ``keep_logits`` also that row's logits). Block capacity is reserved for
@@ -550,7 +561,9 @@ class DecodePipeline:
         """Greedy generation. Without ``prefill`` every row advances one token per step and
         prompt tokens are fed teacher-forced, exactly as ``oracle.model.OraclePipeline
         .generate``; with ``prefill`` the prompts go through ``prefill()`` first and every
-        row then decodes from its own prompt length. Both give identical tokens and logits."""
+        row then decodes from its own prompt length. Both give identical tokens and logits
+        (with ``prefill_attention="chunk"`` or ``fused_moe`` within rounding, so a close choice
+        may fall otherwise)."""
         n = len(prompts)
         if n != self.batch:
             raise ValueError("generate() expects exactly `batch` prompts")
