@@ -387,3 +387,17 @@ def test_the_tables_width_does_not_show():
     want = Case([(33, 250), (5, 37)], 8, 2, 16, seed=72).run()
     for extra in (1, 2, 113):
         assert torch.equal(Case([(33, 250), (5, 37)], 8, 2, 16, seed=72, extra=extra).run(), want)
+
+
+def test_no_sequence_brings_a_row():
+    """All chunks empty: nothing is written, and the workspace serves the next call."""
+    from superl8_serve_b200 import ops
+
+    c = Case([(9, 300), (4, 70)], 8, 2, 16, seed=81)
+    ws = ops.chunk_workspace(DEV)
+    want = c.run(workspace=ws)
+    out = torch.full_like(want, 7.0)
+    ops.paged_chunk_q8(c.q, c.qs, c.kc, c.ks, c.vc, c.vs, c.bt, c.ctx, torch.zeros_like(c.cu), c.scale,
+                       out=out, workspace=ws)
+    assert (out == 7.0).all() and int(ws[:4].view(torch.int32)) == 0
+    assert torch.equal(c.run(workspace=ws), want)

@@ -319,3 +319,25 @@ def test_wide_chunks_in_every_kind_of_stage_step(moe, stages):
         assert toks == got[0][0]
         for a, b in zip(logits, got[0][1]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("batch", [1, 5, 16])
+def test_the_pipelines_fused_layer_is_the_operator(batch):
+    """What the stage leaves is, bit for bit, ``ops.moe_layer`` of the layer's normalised rows."""
+    from superl8_serve_b200 import ops
+    from superl8_serve_b200.config import tiny_moe
+    from superl8_serve_b200.engine import DecodePipeline
+
+    cfg = tiny_moe(num_hidden_layers=1)
+    models = _models(cfg)
+    pipe = DecodePipeline(models, batch=batch, max_len=64, fused_moe=True)
+    pipe.add_sequences()
+    pipe.set_state([0] * batch, list(range(3, 3 + batch)), reserve=4)
+    pipe.step()
+    pipe.synchronize()
+    r, mw = pipe.runners[0], models[0].layers[0].moe
+    y = r.moe_buf["y"][:batch].clone()
+    q, s = ops.quant_rows(y)
+    want = ops.moe_layer(y, q, s, mw.router, mw.gu_w, mw.gu_s, mw.d_w, mw.d_s, mw.top_k,
+                         norm_topk_prob=mw.norm_topk_prob, scaling=mw.scaling)
+    assert torch.equal(r.h[:batch], want)
