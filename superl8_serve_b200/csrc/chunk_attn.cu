@@ -17,14 +17,19 @@
 //
 // Bound. Each score (row x key) costs 2 x 128 int8 and 2 x 128 bf16 operations, one exponential
 // and about 5 further instructions; a key's bytes serve 128 rows. Above some 16 rows per sequence
-// the bf16 product sets the floor (1635 TFLOP/s measured), below it the keys' 264 bytes per head.
-// What bounds the kernel is the chain from S to P: a step of 64 keys takes a softmax group 850
-// cycles alone, 1270 beside the other group and about 1900 beside the converters too, against
-// 512 of tensor work for both groups (issue slots 44%, tensor pipe 20% busy); with few rows the
-// conversion of V, 2000 of the 2500 cycles of a tile of 128 keys. Measured (GPU time in a graph, beside the floor): 4096 new rows over
-// 16K keys, 32 heads on 4, 1310 us in fp16 (589 at the tensor rate); eight prompts of up to 2048
-// rows, 32 on 8, 353 us (102); 64 sequences x up to 4 draft rows over up to 2048 keys 84 us (27
-// at the copy rate); 2 sequences x 16 rows over 64K keys, 40 on 8, 70 us (21); 5 rows 15 us.
+// the products set the floor (1635 TFLOP/s measured for bf16, twice that counted for int8), below it
+// the keys' 264 bytes per head. What bounds the kernel is the chain from S to P: a step of 64 keys
+// took a softmax group 850 cycles alone, 1270 beside the other group and about 1900 beside the
+// converters too, against 512 of tensor work for both groups; with few rows the conversion of V,
+// 2000 of the 2500 cycles of a tile of 128 keys (counted with one weight term; with two, the issue
+// slots are 46 % and the tensor pipe 31 % busy over eight prompts). The kernel has 128 registers a
+// thread at its launch, shared out as 176 and 80, and spills 28 bytes.
+//
+// Measured (us, in a graph / by the call, beside the floor): 4096 new rows over 16K keys, 32 heads
+// on 4, fp16, 1312 / 1375 (442); eight prompts of up to 2048 rows, 32 on 8, 376 / 382 (77), where the
+// row-by-row prefill attention takes 8673; 64 sequences x up to 4 draft rows over up to 2048 keys 87 /
+// 87 (27 at the copy rate; 156); 2 sequences x 16 rows over 64K keys, 40 on 8, 73 / 72 (21); 5 rows
+// over 37 keys 15 / 18 (14).
 //
 // Unit of work. The G query heads of a kv head share its keys, so a tile's 128 rows are
 // 128 / G tokens x G heads, and an item is two such tiles (A and B) of one sequence and kv head:
@@ -79,9 +84,10 @@ constexpr int kSeqBytes = (kMaxSeqs + 1) * 8 + (kMaxSeqs + 1) * 4 + kMaxSeqs * 4
 constexpr int kSmem = 1024 + kOffSeq + kSeqBytes;
 constexpr int kItemRows = 2 * kRows;
 // What an item costs beside its key tiles (queries, the softmax's start, its result), in tiles:
-// it counts so many units more, before its first key tile. Uncounted, eight prompts' CTAs with 6
-// and 18 items took 500,000 and 660,000 cycles for as many key tiles: 380 us, with 3 units 355,
-// with 5 374 (64 sequences of 4 draft rows: 101, 98, 97).
+// it counts so many units more, before its first key tile. Times (us) with 0, 1, 3 and 5 units: eight
+// prompts of up to 2048 rows 406, 381, 376, 395; 32 of up to 700 rows 300, 282, 279, 278; 64 sequences of
+// 4 draft rows over 2K keys 92, 90, 87, 86; 24 of 16 rows over 4K keys 72, 67, 66, 66; 2 x 16 rows over
+// 64K keys 77, 75, 73, 73; 500 rows over 30K keys 761, 756, 757, 759.
 constexpr int kItemUnits = 3;
 constexpr float kSumMax = 0x1p60f;  // a tile's sum of e^(t - reference) above: a new reference
 constexpr int kMaxCtas = 512;     // CTAs the workspace has room for
@@ -313,7 +319,7 @@ __device__ __forceinline__ int tiles_of(const SeqTab &q, const ChunkArgs &a, int
   const int n = q.cu[s + 1] - q.cu[s];
   return n <= 0 ? 0 : n <= 2 * a.TA ? 1 : (n + 2 * a.TA - 1) / (2 * a.TA);
 }
-// One piece of a CTA's run: key tiles [k0, k1) of one item. Warp 15 walks the run and announces
+// One piece of a CTA's run: key tiles [k0, k1) of one item. Warp 14 walks the run and announces
 // the pieces to the other roles through a small ring in shared memory (a walk in every role's
 // registers made the softmax spill).
 struct Piece {

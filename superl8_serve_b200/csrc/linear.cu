@@ -16,12 +16,14 @@
 // the framework's other GEMMs, so without bias, activation and residual the result equals
 // s8b_gemm_w8a8's bit for bit. All later steps stay in binary32 and the output is rounded once.
 //
-// Measured (GPU time in a graph, beside the floor): 8 x 4096 x 4096 with residual 7.9 us (2.6 at
-// the copy rate; two launches that overlap. One, with the sums joined over a cluster and the
+// Measured (us, in a graph that repeats the call / by the call, beside the floor: bytes at 6.53 TB/s,
+// int8 operations at twice the measured bf16 rate, 3.27 Pop/s): 8 x 4096 x 4096 with residual 8.4 /
+// 15.8 (2.6; two launches that overlap. One, with the sums joined over a cluster and the
 // epilogue there, took 9 to 10 us: it cannot start before the slowest CTA of a cluster);
-// 4096 x 4096 x 4096 with bias and residual 74 us, 1.86 Pop/s; 8192 x 12288 x 4096 with SiLU 345
-// us, 2.39 Pop/s; 999 x 5127 x 1040 with bias and GELU 29.8 us (6.5). The large ones are bound by
-// the operands' way from L2: 128 x 256 tiles ask it for some 94 bytes per SM and cycle.
+// 4096 x 4096 x 4096 with bias and residual 77 / 88 (42; 1.8 / 1.6 Pop/s); 8192 x 12288 x 4096 with
+// SiLU 361 / 429 (252; 2.3 / 1.9 Pop/s, the latter under the power cap); 999 x 5127 x 1040 with bias
+// and GELU 29.6 / 28.9 (3.3). The large ones are bound by the operands' way from L2: 128 x 256
+// tiles ask it for some 94 bytes per SM and cycle.
 //
 // The epilogue turns 32 rows x 16 columns of a warp at a time through shared memory: TMEM
 // hands a lane one row, while global memory wants neighbouring lanes on neighbouring columns
@@ -107,7 +109,7 @@ template <int NT, bool ACT>
 struct LinLayout {
   // An activation is long in instructions and a warp waits on most of them: 16 warps finish a
   // tile sooner where its K loop does not hide it (999 x 5127 x 1040 with GELU: 39.5 -> 29.8 us;
-  // 4096 x 4096 x 4096, whose loop does: 88.6 -> 90.0). They cost a stage of the ring, so
+  // 4096 x 4096 x 4096 with SiLU, whose loop does: 88.6 -> 90.0). They cost a stage of the ring, so
   // without an activation it stays at 8 (4096 cubed with bias and residual: 77.6 against 81.0),
   // and beside 256-wide tiles' stages their staging has no room.
   static constexpr int kEpiWarps = NT == 128 && ACT ? 16 : 8;

@@ -13,10 +13,13 @@
 //   C  every CTA quantizes the act rows and computes its slice of output columns over all
 //      chosen experts, so the weighted sum needs no third barrier and no atomics.
 // Products are dp4a on CUDA cores: an expert has one or two rows here, where the stream of
-// weights, not arithmetic, sets the time, and an MMA tile would be empty. Sums over experts are in ascending expert order: the result does not depend on timing.
+// weights, not arithmetic, sets the time, and an MMA tile would be empty. Sums over experts are in
+// ascending expert order: the result does not depend on timing.
 //
-// Measured (2048 x 768, 8 of 128 experts, GPU time in a graph, bytes over the copy rate): one row
-// 19.4 us (6.0), eight rows 63 us (37.6; 3.9 TB/s); 16 rows of 1040 x 272, 3 of 20, 23.5 us (2.4).
+// Measured (2048 x 768, 8 of 128 experts; us, in a graph / by the call, beside the bytes at the copy
+// rate): one row 18.1 / 22.5 (6.0), eight rows 60 / 62 (37.6; 4.1 TB/s); 16 rows of 1040 x 272, 3 of
+// 20, 22.9 / 25.2 (2.4). The seven launches on the same rows, with every layer's weights from HBM:
+// 81, 123 and 31 beside 20, 65 and 25. The kernel spills 124 bytes a thread of its 128 registers.
 // One row's time is latency: the phases wait for one another, each with its own cold loads; eight
 // rows' is the stream of weights. Rings of bulk copies per warp were slower (about 125 cycles of
 // issue per copy and SM), and fetching the down weights into L2 during phase B gained nothing.
