@@ -424,14 +424,16 @@ inline int pick_width(int M, int N) {
 // 4096 256 rows 12.2 / 14.3; 151936 x 4096 8 rows 108 / 124, 64 rows 182 / 118, 256 rows 427 / 166
 // (622 MB of partials). Over N of 256 to 151936, K of 1024 to 12288 and 1 to 256 rows the choice costs 0.5
 // % on average and at worst 1.4 times (256 x 1024, 256 rows: 10.0 / 7.1).
-inline bool few_rows(int M, int N, int K) {
-  if (M > 256 || K % 128 != 0) return false;
-  if (M <= 16) return true;
+inline int few_rows_limit(int M, int N, int K) {  // most rows that stream among those of M's token tiles
+  if (M > 256 || K % 128 != 0) return 0;
   const int C = s8b_gemm_tc_split_count(M, N, K), NT = pick_width(M, N);
-  if (C < 1) return false;
   const long sms = sm_count(), tiles = (M + kTileM - 1l) / kTileM * ((N + NT - 1l) / NT);
-  const double stream = static_cast<double>(N) * K / 4.5e6 + 4.0 * C * M * N / 1e6;
-  return stream <= 0.4 * (NT / 128) * (K / kSlice) * ((tiles + sms - 1) / sms);
+  const double tiled = 0.4 * (NT / 128) * (K / kSlice) * ((tiles + sms - 1) / sms);
+  const double rows = (tiled - static_cast<double>(N) * K / 4.5e6) / (4.0 * C * N / 1e6);
+  return rows < 16 ? 16 : rows < 256 ? static_cast<int>(rows) : 256;
+}
+inline bool few_rows(int M, int N, int K) {
+  return M <= 16 ? K % 128 == 0 : M <= few_rows_limit(M, N, K);
 }
 
 template <typename T, int NT, bool ACT>
@@ -487,17 +489,17 @@ int launch_few(const int8_t *xq, const float *xs, const int8_t *w, const LinArgs
 
 using namespace s8b;
 
-// What this call needs.
-static size_t workspace_need(int M, int N, int K) {
-  if (!few_rows(M, N, K)) return kLinHeader;
+// What a call that streams its weights needs.
+static size_t stream_need(int M, int N, int K) {
   return kLinHeader + sizeof(int32_t) * s8b_gemm_tc_split_count(M, N, K) * M * N;
 }
 
 // What every call of up to M rows needs, for M <= 256.
 extern "C" size_t s8b_linear_workspace_size(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0 || M > 256 || K % 128 != 0 || N > kMaxSide) return kLinHeader;
-  while (M > 1 && !few_rows(M, N, K)) --M;
-  return workspace_need(M, N, K);
+  if (M > kTileM && few_rows_limit(M, N, K) <= kTileM) M = kTileM;  // none of the second token tile
+  const int most = few_rows_limit(M, N, K);
+  return stream_need(M < most ? M : most, N, K);
 }
 
 extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *w,
@@ -514,7 +516,8 @@ extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *
   if (!aligned(xq, 16) || !aligned(w, 16) || !aligned(xs, 4) || !aligned(ws, 4) ||
       !aligned(y, 2) || !aligned(bias, 2) || !aligned(residual, 2))
     return S8B_ERR_ALIGN;
-  if (!workspace || workspace_bytes < (M ? workspace_need(M, N, K) : kLinHeader))
+  const bool few = M > 0 && few_rows(M, N, K);
+  if (!workspace || workspace_bytes < (few ? stream_need(M, N, K) : kLinHeader))
     return S8B_ERR_WORKSPACE;
   if (!aligned(workspace, 256)) return S8B_ERR_ALIGN;
   if (M == 0) return S8B_OK;
@@ -531,7 +534,7 @@ extern "C" int s8b_linear_w8a8(const int8_t *xq, const float *xs, const int8_t *
   a.vec = N % 8 == 0 && aligned(y, 16) && aligned(bias, 16) && aligned(residual, 16) &&
           aligned(ws, 16);
   S8B_DISPATCH_DTYPE(dtype, T, {
-    if (few_rows(M, N, K)) return launch_few<T>(xq, xs, w, a, K, workspace, dtype, stream);
+    if (few) return launch_few<T>(xq, xs, w, a, K, workspace, dtype, stream);
     auto st = (cudaStream_t)stream;
     const bool act = activation != kActNone;
     if (pick_width(M, N) == 256)

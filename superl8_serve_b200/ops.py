@@ -158,7 +158,7 @@ def _status_word(dev: torch.device) -> torch.Tensor:
     any other call, one of the graph's own."""
     ws = _status.get(dev.index)
     if ws is None:
-        with _on(dev):
+        with _on(dev), torch.inference_mode(False):  # (whatever the first caller is in)
             ws = torch.zeros(256, dtype=torch.uint8, device=dev)
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream(dev).synchronize()  # other streams may use it at once

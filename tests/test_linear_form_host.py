@@ -37,3 +37,16 @@ def test_what_a_call_needs(lib):
 def test_sides_whose_last_tile_passes_32_bits_are_refused(lib, M, N, K):
     assert lib.s8b_linear_w8a8(OK, OK, OK, OK, None, 0, None, OK, M, N, K, 0, OK, 2 ** 62, None) == -1
     assert lib.s8b_linear_workspace_size(M, N, K) == 256
+
+
+@pytest.mark.parametrize("N,K", [(151936, 4096), (24576, 1024), (4096, 12288)])
+def test_asking_for_the_size_is_quick(lib, N, K):
+    """A call without a workspace asks every time: well below the launch's own host time."""
+    import time
+
+    took = []
+    for _ in range(200):
+        t = time.perf_counter()
+        lib.s8b_linear_workspace_size(256, N, K)
+        took.append(time.perf_counter() - t)
+    assert min(took) < 20e-6

@@ -341,3 +341,23 @@ def test_the_pipelines_fused_layer_is_the_operator(batch):
     want = ops.moe_layer(y, q, s, mw.router, mw.gu_w, mw.gu_s, mw.d_w, mw.d_s, mw.top_k,
                          norm_topk_prob=mw.norm_topk_prob, scaling=mw.scaling)
     assert torch.equal(r.h[:batch], want)
+
+
+def test_status_word_made_in_inference_mode():
+    """The device's word, first asked for by a layer under inference_mode, can be cleared outside of it."""
+    from superl8_serve_b200 import _lib, ops
+    from superl8_serve_b200.layers import LinearW8A8
+    from superl8_serve_b200.weights import QTensor
+
+    kept = ops._status.pop(0, None)
+    try:
+        g = _gen(2)
+        w, ws = _weight(g, 64, 128)
+        x = torch.randn(5, 128, generator=g, device=DEV).bfloat16()
+        with torch.inference_mode():
+            LinearW8A8(QTensor(w, ws, "per_row_i8"))(x)
+        ops._status[0][:4].view(torch.int32).fill_(_lib.ERR_TIMEOUT)
+        assert ops.linear_status(DEV) == _lib.ERR_TIMEOUT and ops.linear_status(DEV) == 0
+    finally:
+        if kept is not None:
+            ops._status[0] = kept
