@@ -17,8 +17,8 @@
 // ascending expert order: the result does not depend on timing.
 //
 // Measured (2048 x 768, 8 of 128 experts; us, in a graph / by the call, beside the bytes at the copy
-// rate): one row 18.1 / 22.5 (6.0), eight rows 60 / 62 (37.6; 4.1 TB/s); 16 rows of 1040 x 272, 3 of
-// 20, 22.9 / 25.2 (2.4). The seven launches on the same rows, with every layer's weights from HBM:
+// rate): one row 19.4 / 22 (6.0), eight rows 63 / 64 (37.6; 3.9 TB/s); 16 rows of 1040 x 272, 3 of
+// 20, 23.6 / 25.3 (2.4). The seven launches on the same rows, with every layer's weights from HBM:
 // 81, 123 and 31 beside 20, 65 and 25. The kernel spills 124 bytes a thread of its 128 registers.
 // One row's time is latency: the phases wait for one another, each with its own cold loads; eight
 // rows' is the stream of weights. Rings of bulk copies per warp were slower (about 125 cycles of
@@ -59,29 +59,33 @@ struct MoeArgs {
 };
 
 // Every thread's writes before are seen by every thread of the grid after. Bounded: false after
-// about a second, with the status word set. `status` (thread 0) is that word as the kernel found it:
-// where an earlier launch gave up, its arrivals may be missing from the counter, and a barrier would
-// open before all CTAs came. Then no CTA arrives or goes on, until the caller has zeroed both.
-__device__ bool grid_barrier(uint8_t *ws, int *ok, int32_t status) {
+// about a second, with the status word set. A CTA that gives up also sets the counter's top bit: the
+// other CTAs, and those of every later launch, then neither wait nor go on, for the arrivals of
+// a launch that gave up are not a multiple of the grid, and a barrier counted on them would open before
+// all CTAs came. The caller zeroes both. (The bit comes with the arrival itself; reading the
+// status word first took 0.4 us of one row's 19.4.)
+constexpr unsigned long long kGaveUp = 1ull << 63;
+__device__ bool grid_barrier(uint8_t *ws, int *ok) {
   __syncthreads();
-  if (threadIdx.x == 0 && status != 0) *ok = 0;
-  if (threadIdx.x == 0 && status == 0) {
+  if (threadIdx.x == 0) {
     unsigned long long *ctr = reinterpret_cast<unsigned long long *>(ws + ml::kOffBar);
     const unsigned long long n = gridDim.x;
     __threadfence();
-    const unsigned long long goal = (atomicAdd(ctr, 1ull) / n + 1) * n;
+    const unsigned long long old = atomicAdd(ctr, 1ull), goal = (old / n + 1) * n;
     const uint32_t t0 = static_cast<uint32_t>(clock());
-    *ok = 1;
-    while (true) {
+    bool came = (old & kGaveUp) == 0;
+    while (came) {
       unsigned long long v;
       asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(ctr) : "memory");
-      if (v >= goal) break;
-      if (static_cast<uint32_t>(clock()) - t0 > 2000000000u) {
+      if (v & kGaveUp) came = false;
+      else if (v >= goal) break;
+      else if (static_cast<uint32_t>(clock()) - t0 > 2000000000u) {
+        atomicOr(ctr, kGaveUp);
         *reinterpret_cast<volatile int32_t *>(ws) = S8B_ERR_TIMEOUT;
-        *ok = 0;
-        break;
+        came = false;
       }
     }
+    *ok = came;
     __threadfence();
   }
   __syncthreads();
@@ -214,7 +218,6 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   __shared__ int before[kMaxA + 1];    // cost of a pair of every chosen expert before
   __shared__ uint8_t slot_of[kMaxE];  // its place among the chosen experts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int32_t status = threadIdx.x == 0 ? *reinterpret_cast<volatile int32_t *>(a.ws) : 0;
   const int T_ = a.T, H = a.H, F = a.F, E = a.E, k = a.k, A = T_ * k;
   float *logits = reinterpret_cast<float *>(a.ws + kLogits);
   float *act = reinterpret_cast<float *>(a.ws + kAct);
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
   }
   for (int i = threadIdx.x; i < E; i += kThreads) members[i] = 0u;
   if (threadIdx.x < T_) xs_s[threadIdx.x] = a.xs[threadIdx.x];
-  if (!grid_barrier(a.ws, &ok_s, status)) return;
+  if (!grid_barrier(a.ws, &ok_s)) return;
 
   // ---- B: each row's experts, then their gate_up and SwiGLU ----
   if (warp < T_) {
@@ -381,7 +384,7 @@ __global__ void __launch_bounds__(ml::kThreads, 1) moe_layer_kernel(const MoeArg
       u += 1 + two;
     }
   }
-  if (!grid_barrier(a.ws, &ok_s, status)) return;
+  if (!grid_barrier(a.ws, &ok_s)) return;
 
   // ---- C: act codes, then this CTA's columns of the down products ----
   if (nh == 0) return;
